@@ -505,9 +505,70 @@ int vpf_augment_points(const float* pts, int B, int N, int C, const uint32_t* rn
  * (mean3 / std3: HOST arrays of 3 floats; rng_state nullable = no flip; flips_out nullable u8 [B]). */
 int vpf_image_u8_normalize(const void* img_u8, int B, int H, int W, const float* mean3_host, const float* std3_host,
                            const uint32_t* rng_state, uint32_t site, float p_flip, float* out, void* flips_out, void* stream);
+/* sizeof(VpfCaFront) is vpf_abi_sizeof(7), sizeof(VpfRotary) (8), sizeof(VpfGatedNorm) (9), sizeof(VpfWindowAttn) (10) */
 /* sizeof(VpfSaLayerBwd) is vpf_abi_sizeof(3), sizeof(VpfPgradJob) (4), sizeof(VpfAdapterKv) (5), sizeof(VpfAdapterKvBwd) (6) */
 /* sizeof(VpfPackJob) (which = 0) / sizeof(VpfSaLayerFwd) (1) / sizeof(VpfWgradJob) (2): lets a binding verify its struct layout */
 int vpf_abi_sizeof(int which);
+
+/* ------------------------------------------------------------------ operators of a transformer block over long sequences
+ * Rotary positions with several axes, attention inside a sliding window with first tokens that stay visible, and the norms around a
+ * block with its gate and residual scale.  They take their element type per CALL (VPF_T_*), every stride in ELEMENTS (last dimension
+ * contiguous), and write every element of their outputs. */
+#define VPF_T_F32 0
+#define VPF_T_F16 1
+#define VPF_T_BF16 2
+#define VPF_POS_F32 0
+#define VPF_POS_F64 1
+#define VPF_POS_I32 2
+#define VPF_POS_I64 3
+#define VPF_ROTARY_HALF 0       /* pair p = channels (p, p + P) */
+#define VPF_ROTARY_PAIR 1       /* pair p = channels (2p, 2p + 1) */
+#define VPF_ROTARY_MAX_AXES 8
+#define VPF_ROTARY_MAX_DIM 1024
+
+/* (x0, x1) of pair p -> (x0 cos t - x1 sin t, x1 cos t + x0 sin t), t = 2 pi * pos[axis[p]] * freq[p], for every head of q and k; the
+ * channels behind the 2 P rotated ones are copied.  inverse != 0 turns by -t: the gradient.  The angle is reduced in fp64.
+ * q [B, L, Hq, head_dim], k [B, L, Hk, head_dim] (Hk = 0: queries alone), oq / ok the results (may be q / k themselves: in place);
+ * pos [B, L, axes] with batch stride pos_sb (0: shared by the batch); freq: turns per unit of position, fp64 [P]; axis int32 [P],
+ * every entry in [0, axes). */
+typedef struct VpfRotary {
+    int B, L, Hq, Hk, head_dim, P, axes, layout, dtype, pos_type, inverse, pad_;
+    const void* q; const void* k; void* oq; void* ok;
+    long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, oq_sb, oq_sl, oq_sh, ok_sb, ok_sl, ok_sh;
+    const void* pos; long pos_sb;
+    const double* freq; const int* axis;
+} VpfRotary;
+int vpf_rotary_axes(const VpfRotary* a, void* stream);
+
+/* h = alpha * x + beta * gate * post(y);  n = pre(h):  the norm behind a block on its output y, the block's gate and the two scales of the
+ * residual stream, and the norm in front of the next block, in one pass.
+ *   kind 0: LayerNorm (z - mean) * rstd * w + b, 1: RMSNorm z * rstd * w (+ b); null w / b: 1 / 0.  has_post 0: post(y) = y; has_pre 0: no n.
+ *   x, h, dh, dx: [rows, D] of x_type; y, n, dn, dy: [rows, D] of y_type (x fp32 with any y, or both of one type); row strides D.
+ *   gate_mode 0: none; 1: fp32 [rows / gate_rows, D], one row of it for gate_rows consecutive rows; 2: y_type [rows, D].
+ *   stats (null where no gradient follows): fp32 [4][rows]: mean, rstd of y; mean, rstd of h.
+ * n is the norm of h before h is rounded to x_type. */
+#define VPF_GATE_NONE 0
+#define VPF_GATE_ROWS 1
+#define VPF_GATE_FULL 2
+#define VPF_GATED_NORM_MAX_D 8192
+typedef struct VpfGatedNorm {
+    long rows, gate_rows;
+    int D, kind, x_type, y_type, gate_mode, has_post, has_pre, pad_;
+    float alpha, beta, eps_post, eps_pre;
+    const void* x; const void* y; const void* gate;
+    const float* w_post; const float* b_post; const float* w_pre; const float* b_pre;
+    void* h; void* n; float* stats;
+    /* backward: dh, dn (null where has_pre == 0) in; dx, dy, dgate and the four parameter gradients out (null: not wanted).
+     * dgate: fp32 [rows / gate_rows, D] (mode 1) or y_type [rows, D] (mode 2); the parameter gradients are fp32 [D].  All overwritten. */
+    const void* dh; const void* dn; void* dx; void* dy; void* dgate;
+    float* dw_post; float* db_post; float* dw_pre; float* db_pre;
+    float* ws; long ws_floats;          /* backward: vpf_gated_norm_ws floats of scratch */
+} VpfGatedNorm;
+int vpf_gated_norm_fwd(const VpfGatedNorm* a, void* stream);
+/* Column sums over the rows are taken per workgroup and folded in a fixed order: the same call gives the same bits. */
+int vpf_gated_norm_bwd(const VpfGatedNorm* a, void* stream);
+/* floats that a->ws needs (host only; negative: VPF_ERR_*) */
+long vpf_gated_norm_ws(const VpfGatedNorm* a);
 
 #ifdef __cplusplus
 }

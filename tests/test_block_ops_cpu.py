@@ -1,0 +1,109 @@
+"""CPU: refusals of the transformer-block operators, of their Python entry points and of the C ABI (no launch happens)."""
+import ctypes
+
+import pytest
+import torch
+
+from vipformer_amd import _lib as L
+from vipformer_amd import build
+from vipformer_amd import ops_block as O
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    build.build(verbose=False)
+
+
+def refuses(match, fn, *a, **k):
+    with pytest.raises(L.VpfError, match=match):
+        fn(*a, **k)
+
+
+def test_structs_match_the_library():
+    for which, cls in ((8, L.Rotary), (9, L.GatedNorm)):
+        assert L.lib().vpf_abi_sizeof(which) == ctypes.sizeof(cls), cls.__name__
+
+
+def test_rotary_refusals():
+    plan = O.RotaryAxes((8, 8), 32)
+    q, k, pos = torch.zeros(2, 5, 4, 32), torch.zeros(2, 5, 2, 32), torch.zeros(5, 2)
+    refuses("no CPU fallback", O.rotary_axes, q, k, pos, plan)
+    refuses("head_dim", O.rotary_axes, q[0], k, pos, plan)
+    refuses("head_dim", O.rotary_axes, q, k[:, :4], pos, plan)
+    refuses("built for 32", O.rotary_axes, q[..., :16], k[..., :16], pos, plan)
+    refuses("one type", O.rotary_axes, q, k.half(), pos, plan)
+    refuses("one type", O.rotary_axes, q.double(), k.double(), pos, plan)
+    refuses("positions", O.rotary_axes, q, k, torch.zeros(5, 3), plan)
+    refuses("positions", O.rotary_axes, q, k, torch.zeros(4, 2), plan)
+    refuses("positions", O.rotary_axes, q, k, torch.zeros(3, 5, 2), plan)
+    refuses("positions are", O.rotary_axes, q, k, pos.half(), plan)
+    refuses("no gradient", O.rotary_axes, q, k, pos.clone().requires_grad_(), plan)
+    for bad in (dict(sections=(20,), head_dim=32), dict(sections=(), head_dim=32), dict(sections=(0, 0), head_dim=32), dict(sections=(-1, 4), head_dim=32),
+                dict(sections=(4,), head_dim=33), dict(sections=(4,), head_dim=2048), dict(sections=(1,) * 9, head_dim=32),
+                dict(sections=(4,), head_dim=32, base=0.0), dict(sections=(4,), head_dim=32, base=float("inf")),
+                dict(sections=(4,), head_dim=32, layout="odd"), dict(sections=(4,), head_dim=32, ladder="none")):
+        refuses("RotaryAxes", O.RotaryAxes, **bad)
+
+
+def test_rotary_frequencies():
+    f = O.RotaryAxes((2, 1), 8, base=100.0).frequencies()
+    assert torch.allclose(f, torch.tensor([1.0, 0.1, 1.0], dtype=torch.float64), rtol=1e-15)
+    f = O.RotaryAxes((2, 2), 8, base=10000.0, ladder="joint").frequencies()
+    assert torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14)
+
+
+def test_rotary_c_abi_refusals():
+    fn = L.lib().vpf_rotary_axes
+    fn.argtypes, fn.restype = L.SIGS["vpf_rotary_axes"], L.I
+    ok = dict(B=1, L=4, Hq=2, Hk=1, head_dim=32, P=16, axes=2, layout=0, dtype=1, pos_type=0)
+    call = lambda **k: fn(ctypes.byref(L.Rotary(**{**ok, **k})), None)
+    assert fn(None, None) == -5 and call() == -5                                  # null struct, null tensors
+    for bad in (dict(B=-1), dict(head_dim=0), dict(P=17), dict(P=0), dict(axes=0), dict(axes=9), dict(head_dim=1026), dict(Hq=5000)):
+        assert call(**bad) == -1, bad
+    for bad in (dict(layout=2), dict(dtype=3), dict(dtype=-1), dict(pos_type=4)):
+        assert call(**bad) == -3, bad
+    assert call(L=0) == 0                                                         # nothing to do
+    assert call(layout=1, q=2, k=4, oq=4, ok=4, pos=4, freq=8, axis=4) == -2      # pairs of 16-bit channels at an odd address
+
+
+def test_gated_norm_refusals():
+    x, y, w = torch.zeros(2, 5, 32), torch.zeros(2, 5, 32, dtype=torch.float16), torch.ones(32)
+    f = O.gated_norm_residual
+    refuses("no CPU fallback", f, x, y)
+    refuses("one shape", f, x, y[:, :4])
+    refuses("one shape", f, torch.zeros(2, 9000), torch.zeros(2, 9000))
+    refuses("one shape", f, torch.zeros(2, 0), torch.zeros(2, 0))
+    refuses("x is fp32", f, x.half(), y.float())
+    refuses("x is fp32", f, x.half(), y.bfloat16())
+    refuses("x is fp32", f, x.double(), y)
+    refuses("kind", f, x, y, kind="batch")
+    for gate in (torch.zeros(31), torch.zeros(2, 32), torch.zeros(3, 1, 32), torch.zeros(2, 5, 32), torch.zeros(5, 32)):
+        refuses("gate", f, x, y, gate=gate)
+    refuses("is fp32", f, x, y, gate=torch.zeros(32, dtype=torch.float16))
+    refuses("fp32 parameters", f, x, y, post=(w.half(), None))
+    refuses("fp32 parameters", f, x, y, pre=(w, w[:31]))
+    refuses("norm module or", f, x, y, pre=(w,))
+    refuses("LayerNorm", f, x, y, pre=torch.nn.LayerNorm(31))
+    refuses("LayerNorm", f, x, y, pre=torch.nn.RMSNorm(32))
+    refuses("RMSNorm", f, x, y, post=torch.nn.LayerNorm(32), kind="rms")
+
+
+def test_gated_norm_c_abi_refusals():
+    fwd, bwd, ws = L.lib().vpf_gated_norm_fwd, L.lib().vpf_gated_norm_bwd, L.lib().vpf_gated_norm_ws
+    fwd.argtypes = bwd.argtypes = L.SIGS["vpf_gated_norm_fwd"]
+    ws.restype = L.L_
+    ok = dict(rows=6, gate_rows=3, D=32, kind=0, x_type=0, y_type=1, gate_mode=0, has_post=1, has_pre=1)
+    make = lambda **k: L.GatedNorm(**{**ok, **k})
+    for fn in (fwd, bwd):
+        assert fn(None, None) == -5 and fn(ctypes.byref(make()), None) == -5
+        for bad in (dict(rows=-1), dict(rows=1 << 31), dict(D=0), dict(D=8193), dict(kind=2), dict(gate_mode=1, gate_rows=4), dict(gate_mode=1, gate_rows=0)):
+            assert fn(ctypes.byref(make(**bad)), None) == -1, bad
+        for bad in (dict(gate_mode=3), dict(x_type=3), dict(y_type=-1), dict(x_type=1, y_type=0), dict(x_type=2, y_type=1)):
+            assert fn(ctypes.byref(make(**bad)), None) == -3, bad
+        assert fn(ctypes.byref(make(rows=0)), None) == 0
+    assert ws(ctypes.byref(make(rows=0))) == 0 and ws(ctypes.byref(make(D=0))) == -1
+    need = ws(ctypes.byref(make(gate_mode=1)))
+    assert need >= (4 + 2) * 32
+    # a workspace that is too small is refused before anything is launched
+    small = make(gate_mode=1, x=16, y=16, gate=16, dh=16, dn=16, stats=16, ws=16, ws_floats=need - 1)
+    assert bwd(ctypes.byref(small), None) == -1

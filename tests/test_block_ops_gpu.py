@@ -1,0 +1,318 @@
+"""GPU parity of the transformer-block operators (vipformer_amd/ops_block.py) against plain 64-bit implementations.
+
+Tolerances are elementwise: half a step of the output's type (finfo.eps / 2 relative: the one rounding at the end) plus a counted number of
+fp32 roundings, each at most 2^-24 of the sum of the magnitudes that meet in the element."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U24 = 2.0 ** -24
+TYPES = {"f32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def close(got, ref, slack, what):
+    """|got - ref| <= half a step of got's type at ref (and of its smallest number) + slack."""
+    fi = torch.finfo(got.dtype)
+    assert got.shape == ref.shape, what
+    tol = (fi.eps / 2) * (ref.abs() + slack) + fi.smallest_normal * fi.eps / 2 + slack
+    bad = (got.double() - ref).abs() - tol
+    assert torch.isfinite(got.double()).all() and float(bad.max()) <= 0.0, \
+        f"{what}: {int((bad > 0).sum())} of {bad.numel()} outside, worst {float((got.double() - ref).abs().max()):.3e} against {float(tol.flatten()[bad.flatten().argmax()]):.3e}"
+
+
+# ------------------------------------------------------------------------------------------ rotary positions with several axes
+def rotary_ref(x, pos, plan, sign=1.0):
+    """(rotated, sum of the magnitudes that meet) in 64 bits."""
+    f = plan.frequencies().cuda()
+    axis = torch.repeat_interleave(torch.arange(len(plan.sections), device="cuda"), torch.tensor(plan.sections, device="cuda"))
+    t = (pos if pos.dim() == 3 else pos[None]).double()[..., axis] * f * sign
+    c, s = t.cos()[:, :, None], t.sin()[:, :, None]
+    d, P = x.detach().double(), plan.pairs
+    if plan.layout == "half":
+        a, b, rest = d[..., :P], d[..., P:2 * P], d[..., 2 * P:]
+        join = lambda u, v: torch.cat([u, v, rest], -1)
+    else:
+        a, b, rest = d[..., 0:2 * P:2], d[..., 1:2 * P:2], d[..., 2 * P:]
+        join = lambda u, v: torch.cat([torch.stack([u, v], -1).flatten(-2), rest], -1)
+    mag = a.abs() + b.abs()
+    out = join(a * c - b * s, b * c + a * s)
+    size = join(mag, mag)
+    size[..., 2 * P:] = 0.0
+    return out, size
+
+
+# fp32 roundings of one element: the fraction of a turn (2^-25 turns are 3.2 units of 2^-24 rad), sincospi within 2 of its last places (4
+# units at most), two products, one sum: 10
+ROT = 10 * U24
+
+
+@pytest.mark.parametrize("layout", ["half", "pair"])
+@pytest.mark.parametrize("dtype", ["f32", "fp16", "bf16"])
+@pytest.mark.parametrize("B,L,Hq,Hk,dh,sections,ladder", [
+    (1, 1, 1, 1, 2, (1,), "axis"), (2, 96, 4, 4, 64, (16, 16), "axis"), (3, 145, 6, 2, 64, (8, 12, 12), "axis"),
+    (1, 1025, 16, 4, 128, (22, 21, 21), "joint"), (5, 33, 3, 1, 40, (7, 7, 6), "axis"), (2, 17, 2, 2, 80, (5, 0, 3), "joint"),
+    (1, 7, 70, 1, 1024, (512,), "axis"), (2, 0, 2, 2, 64, (32,), "axis"), (40, 3, 2, 1, 96, (1, 2, 3, 4, 5, 6, 7, 8), "axis")])
+def test_rotary_forward_and_gradient(B, L, Hq, Hk, dh, sections, ladder, dtype, layout):
+    from vipformer_amd.ops_block import RotaryAxes, rotary_axes
+    g, dt = gen(L + dh), TYPES[dtype]
+    plan = RotaryAxes(sections, dh, layout=layout, ladder=ladder)
+    q, k = randn(g, B, L, Hq, dh, dtype=dt).requires_grad_(), randn(g, B, L, Hk, dh, dtype=dt).requires_grad_()
+    pos = torch.rand(B, L, len(sections), generator=g, device="cuda") * 100 - 20
+    oq, ok = rotary_axes(q, k, pos, plan)
+    gq, gk = randn(g, *q.shape, dtype=dt), randn(g, *k.shape, dtype=dt)
+    dq, dk = torch.autograd.grad((oq, ok), (q, k), (gq, gk))
+    for got, x, sign, what in ((oq, q, 1.0, "q"), (ok, k, 1.0, "k"), (dq, gq, -1.0, "dq"), (dk, gk, -1.0, "dk")):
+        if L == 0:
+            assert got.shape == x.shape
+            continue
+        ref, size = rotary_ref(x, pos, plan, sign)
+        close(got.detach(), ref, ROT * size, what)
+
+
+@pytest.mark.parametrize("pdtype", [torch.int32, torch.int64, torch.float32, torch.float64])
+def test_rotary_positions_types_sharing_and_far_positions(pdtype):
+    from vipformer_amd.ops_block import RotaryAxes, rotary_axes
+    g = gen(3)
+    plan = RotaryAxes((10, 11, 11), 64)
+    q, k = randn(g, 2, 50, 4, 64), randn(g, 2, 50, 2, 64)
+    pos = torch.randint(0, 64, (50, 3), generator=g, device="cuda")
+    pos[:, 0] += 2 ** 24 - 30 if pdtype == torch.float32 else 10 ** 9          # fp32 holds whole numbers up to 2^24
+    pos = pos.to(pdtype)
+    for p in (pos, pos[None], pos[None].expand(2, 50, 3)):
+        oq, ok = rotary_axes(q, k, p, plan)
+        for got, x in ((oq, q), (ok, k)):
+            ref, size = rotary_ref(x, p, plan)
+            # the reference's own angle in 64 bits: 10^9 rad at 2^-53 is 1e-7 rad, two more units
+            close(got, ref, (ROT + 2 * U24) * size, "far")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "fp16"])
+@pytest.mark.parametrize("layout", ["half", "pair"])
+def test_rotary_strides_slices_and_single_tensor(dtype, layout):
+    """Slices of one projection's output, head-first tensors, odd base offsets, a transposed last dimension, q alone."""
+    from vipformer_amd.ops_block import RotaryAxes, rotary_axes
+    g, dt = gen(9), TYPES[dtype]
+    B, L, H, dh = 2, 37, 3, 48
+    plan = RotaryAxes((12, 12), dh, layout=layout)
+    pos = torch.randint(0, 9, (L, 2), generator=g, device="cuda")
+    qkv = randn(g, B, L, 3 * H * dh, dtype=dt)
+    q, k = qkv.view(B, L, 3, H, dh)[:, :, 0], qkv.view(B, L, 3, H, dh)[:, :, 1]
+    heads_first = randn(g, B, H, L, dh, dtype=dt).transpose(1, 2)
+    flat = randn(g, B * L * H * dh + 1, dtype=dt)[1:].view(B, L, H, dh)
+    turned = randn(g, B, L, dh, H, dtype=dt).transpose(2, 3)
+    rows = randn(g, B, L, H, dh + 1, dtype=dt)[..., :dh]                        # an odd row stride
+    before = qkv.clone()
+    for a, b in ((q, k), (heads_first, flat), (turned, rows), (rows, None)):
+        out = rotary_axes(a, b, pos, plan)
+        outs = (out,) if b is None else out
+        for got, x in zip(outs, (a, b)):
+            ref, size = rotary_ref(x, pos, plan)
+            close(got, ref, ROT * size, "strided")
+    assert torch.equal(qkv, before)
+
+
+# ------------------------------------------------------------------------------------------ norms around a block, gate and residual scale
+def norm_ref(x, y, gate, post, pre, kind, alpha, beta, eps, dh, dn):
+    """Outputs and gradients in 64 bits with, for each, the sum of the magnitudes that meet in it."""
+    d = lambda t: None if t is None else t.detach().double()
+    x, y, gate, dh, dn = d(x), d(y), d(gate), d(dh), d(dn)
+    layer = kind == "layer"
+    D = x.shape[-1]
+
+    def stats(z):
+        m = z.mean(-1, keepdim=True) if layer else torch.zeros_like(z[..., :1])
+        r = 1.0 / torch.sqrt(((z - m) ** 2).mean(-1, keepdim=True) + eps)
+        return m, r
+
+    def affine(wb):
+        w, b = (d(wb[0]), d(wb[1])) if wb is not None else (None, None)
+        return (torch.ones(D, device="cuda", dtype=torch.float64) if w is None else w), (torch.zeros(D, device="cuda", dtype=torch.float64) if b is None else b)
+
+    def back(e, zh, r):
+        out = e - zh * (e * zh).mean(-1, keepdim=True) - (e.mean(-1, keepdim=True) if layer else 0.0)
+        size = e.abs() + zh.abs() * (e * zh).abs().mean(-1, keepdim=True) + (e.abs().mean(-1, keepdim=True) if layer else 0.0)
+        return out * r, size * r
+
+    gt = torch.ones_like(x) if gate is None else gate.expand_as(x)
+    wp, bp = affine(post)
+    yh, ry = y, torch.ones_like(y[..., :1])
+    ysize = y.abs()
+    if post is not None:
+        my, ry = stats(y)
+        yh = (y - my) * ry
+        ysize = (y.abs() + y.abs().mean(-1, keepdim=True)) * ry
+    u, usize = yh * wp + bp, ysize * wp.abs() + bp.abs()
+    h = alpha * x + beta * gt * u
+    hsize = abs(alpha) * x.abs() + abs(beta) * gt.abs() * usize
+    out = {"h": (h, hsize)}
+    dH, dHsize = dh, dh.abs()
+    if pre is not None:
+        wn, bn = affine(pre)
+        mh, rh = stats(h)
+        hh = (h - mh) * rh
+        # an error of h reaches every channel of its row through the statistics
+        rel = hsize + hsize.mean(-1, keepdim=True) + hh.abs() * (hsize * hh.abs()).mean(-1, keepdim=True)
+        hhsize = rel * rh
+        out["n"] = (hh * wn + bn, hhsize * wn.abs() + bn.abs())
+        e = dn * wn
+        part, psize = back(e, hh, rh)
+        # hh enters the gradient twice and rh once: their errors on top
+        grown = rh * (hhsize * (e * hh).abs().mean(-1, keepdim=True) + hh.abs() * (e.abs() * hhsize).mean(-1, keepdim=True))
+        grown = grown + psize * (hhsize * hh.abs()).mean(-1, keepdim=True)
+        dH, dHsize = dh + part, dh.abs() + psize + grown
+        out["dw_pre"] = ((dn * hh).flatten(0, -2).sum(0), (dn.abs() * (hh.abs() + hhsize)).flatten(0, -2).sum(0))
+        out["db_pre"] = (dn.flatten(0, -2).sum(0), dn.abs().flatten(0, -2).sum(0))
+    out["dx"] = (alpha * dH, abs(alpha) * dHsize)
+    if gate is not None:
+        full, fsize = beta * dH * u, abs(beta) * (dHsize * u.abs() + dH.abs() * usize)
+        shape = gate.shape
+        if gate.shape == x.shape:
+            out["dgate"] = (full, fsize)
+        elif gate.dim() == 1:
+            out["dgate"] = (full.flatten(0, -2).sum(0), fsize.flatten(0, -2).sum(0))
+        else:
+            out["dgate"] = (full.reshape(shape[0], -1, D).sum(1).view(shape), fsize.reshape(shape[0], -1, D).sum(1).view(shape))
+    f, fs = beta * gt * dH, abs(beta) * gt.abs() * dHsize
+    if post is not None:
+        out["dw_post"] = ((f * yh).flatten(0, -2).sum(0), (fs * yh.abs() + f.abs() * ysize).flatten(0, -2).sum(0))
+        out["db_post"] = (f.flatten(0, -2).sum(0), fs.flatten(0, -2).sum(0))
+        dy, dysize = back(f * wp, yh, ry)
+        _, more = back(fs * wp.abs(), yh, ry)
+        fw = (f * wp).abs()
+        grown = ry * (ysize * (fw * yh.abs()).mean(-1, keepdim=True) + yh.abs() * (fw * ysize).mean(-1, keepdim=True))
+        grown = grown + dysize * (ysize * yh.abs()).mean(-1, keepdim=True)
+        out["dy"] = (dy, dysize + more + grown)
+    else:
+        out["dy"] = (f, fs)
+    return out
+
+
+# fp32 roundings on the longest path of one element: 8 products and sums in a thread, 10 levels of the joining tree, twice (mean, variance),
+# for two norms, root, scale, gate and residual: under 64; forward values enter the gradient once more: under 128
+FWD_N, BWD_N = 64 * U24, 128 * U24
+
+
+def norm_case(shape, kind, gate, x, y, post, pre, alpha=0.9, beta=0.75, eps=1e-5, seed=0, bias=None):
+    from vipformer_amd.ops_block import gated_norm_residual
+    g, tx, ty = gen(seed + shape[-1]), TYPES[x], TYPES[y]
+    D = shape[-1]
+    X, Y = randn(g, *shape, dtype=tx, scale=2.0).requires_grad_(), (randn(g, *shape, scale=0.7) + 0.3).to(ty).requires_grad_()
+    aff = lambda: (1.0 + randn(g, D, scale=0.2)).requires_grad_()
+    bias = (kind == "layer") if bias is None else bias
+    P = (aff(), aff() if bias else None) if post else None
+    N = (aff(), aff() if bias else None) if pre else None
+    gshape = {"none": None, "channel": (D,), "sample": (shape[0],) + (1,) * (len(shape) - 2) + (D,), "token": shape}[gate]
+    G = None if gshape is None else randn(g, *gshape, dtype=ty if gate == "token" else torch.float32, scale=0.5).requires_grad_()
+    h, n = gated_norm_residual(X, Y, gate=G, post=P, pre=N, kind=kind, alpha=alpha, beta=beta, eps=eps)
+    dh, dn = randn(g, *shape, dtype=tx), (randn(g, *shape, dtype=ty) if pre else None)
+    names = {"dx": X, "dy": Y, "dgate": G, "dw_post": P and P[0], "db_post": P and P[1], "dw_pre": N and N[0], "db_pre": N and N[1]}
+    names = {k: v for k, v in names.items() if v is not None}
+    outs, douts = ([h], [dh]) if n is None else ([h, n], [dh, dn])
+    grads = torch.autograd.grad(outs, list(names.values()), douts)
+    ref = norm_ref(X, Y, G, P, N, kind, alpha, beta, eps, dh, dn)
+    assert h.dtype == tx and (n is None or n.dtype == ty)
+    close(h.detach(), *(ref["h"][0], FWD_N * ref["h"][1]), "h")
+    if n is not None:
+        close(n.detach(), ref["n"][0], FWD_N * ref["n"][1], "n")
+    for name, got in zip(names, grads):
+        assert got.dtype == names[name].dtype
+        close(got, ref[name][0], BWD_N * ref[name][1], name)
+    with torch.no_grad():
+        h2, n2 = gated_norm_residual(X, Y, gate=G, post=P, pre=N, kind=kind, alpha=alpha, beta=beta, eps=eps)
+    assert torch.equal(h2, h) and (n is None or torch.equal(n2, n))
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "token"])
+@pytest.mark.parametrize("x,y", [("f32", "fp16"), ("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("shape", [(2, 70, 256), (3, 37, 1001), (1, 1, 40)])
+def test_gated_norm_forward_and_gradients(shape, x, y, gate, kind):
+    norm_case(shape, kind, gate, x, y, True, True)
+
+
+@pytest.mark.parametrize("x,y", [("f32", "bf16"), ("fp16", "fp16")])
+@pytest.mark.parametrize("D", [8, 13, 128, 136, 384, 520, 1024, 1032, 2048, 2055, 4096, 4104, 8185, 8192])
+def test_gated_norm_widths(D, x, y):
+    norm_case((2, 9, D), "layer", "sample", x, y, True, True)
+
+
+@pytest.mark.parametrize("post,pre", [(True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+def test_gated_norm_with_one_norm_or_none(post, pre, gate):
+    norm_case((4, 65, 264), "layer", gate, "f32", "fp16", post, pre)
+    norm_case((4, 65, 264), "rms", gate, "fp16", "fp16", post, pre, bias=True)
+
+
+@pytest.mark.parametrize("shape", [(5, 1, 64), (700, 2, 64), (257, 96), (2, 3, 4, 5, 72), (4096, 3, 16), (33, 1000, 256)])
+def test_gated_norm_many_samples_and_ranks(shape):
+    norm_case(shape, "layer", "sample", "f32", "fp16", True, True)
+
+
+def test_gated_norm_modules_identity_and_unused_outputs():
+    from vipformer_amd.ops_block import gated_norm_residual
+    g = gen(11)
+    x, y = randn(g, 2, 50, 256).requires_grad_(), randn(g, 2, 50, 256, dtype=torch.float16)
+    ln, rms = torch.nn.LayerNorm(256, eps=1e-3).cuda(), torch.nn.RMSNorm(256).cuda()
+    h, n = gated_norm_residual(x, y, post=ln, pre=torch.nn.LayerNorm(256, elementwise_affine=False).cuda())
+    ref = norm_ref(x, y, None, (ln.weight, ln.bias), (None, None), "layer", 1.0, 1.0, 1e-3, h, y)
+    close(h.detach(), ref["h"][0], FWD_N * ref["h"][1], "module eps")
+    gated_norm_residual(x, y, post=rms, pre=rms, kind="rms")
+    # the same parameters in both places: their gradient is the sum of the two
+    w = (1.0 + randn(g, 256, scale=0.1)).requires_grad_()
+    h, n = gated_norm_residual(x, y, post=(w, None), pre=(w, None), kind="rms", eps=1e-5)
+    dh, dn = randn(g, *h.shape), randn(g, *n.shape, dtype=torch.float16)
+    (dw,) = torch.autograd.grad((h, n), (w,), (dh, dn))
+    ref = norm_ref(x, y, None, (w, None), (w, None), "rms", 1.0, 1.0, 1e-5, dh, dn)
+    close(dw, ref["dw_post"][0] + ref["dw_pre"][0], BWD_N * (ref["dw_post"][1] + ref["dw_pre"][1]), "shared weight")
+    # a loss that uses one output only
+    h, n = gated_norm_residual(x, y, post=(w, None), pre=(w, None), kind="rms", eps=1e-5)
+    (dx,) = torch.autograd.grad(h, (x,), dh)
+    assert torch.equal(dx, dh)
+
+
+def test_gated_norm_is_bitwise_reproducible():
+    from vipformer_amd.ops_block import gated_norm_residual
+    g = gen(12)
+    x, y = randn(g, 64, 128, 256).requires_grad_(), randn(g, 64, 128, 256, dtype=torch.float16).requires_grad_()
+    gate, w, b = randn(g, 256).requires_grad_(), randn(g, 256).requires_grad_(), randn(g, 256).requires_grad_()
+    dh, dn = randn(g, 64, 128, 256), randn(g, 64, 128, 256, dtype=torch.float16)
+    runs = []
+    for _ in range(3):
+        h, n = gated_norm_residual(x, y, gate=gate, post=(w, b), pre=(w, b))
+        runs.append([h.detach(), n.detach(), *torch.autograd.grad((h, n), (x, y, gate, w, b), (dh, dn))])
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+def test_gated_norm_under_internal_grad_scale():
+    """Parameters get their gradient in the loss's own units; the gradient that flows on keeps the scale."""
+    from vipformer_amd import ops
+    from vipformer_amd.ops_block import gated_norm_residual
+    g = gen(13)
+    x, y = randn(g, 4, 16, 64).requires_grad_(), randn(g, 4, 16, 64, dtype=torch.float16).requires_grad_()
+    gate, w = torch.nn.Parameter(randn(g, 64)), torch.nn.Parameter(1.0 + randn(g, 64, scale=0.1))
+    dh = randn(g, 4, 16, 64, scale=1e-4)
+
+    def grads(on):
+        with ops.internal_grad_scale(on) as holder:
+            h, _ = gated_norm_residual(x, y, gate=gate, post=(w, None))
+            out = ops.ScaleGradFn.apply(h, holder) if on else h
+        return torch.autograd.grad(out, (x, gate, w), dh)
+
+    plain, scaled = grads(False), grads(True)
+    s = float(scaled[0].abs().max() / plain[0].abs().max())
+    assert s > 1024 and math.log2(s) == int(math.log2(s))
+    assert torch.equal(scaled[1], plain[1]) and torch.equal(scaled[2], plain[2])

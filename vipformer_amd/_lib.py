@@ -157,6 +157,9 @@ SIGS = {
     "vpf_ce_smooth": [VP, L_, VP, L_, I, F, VP, VP, VP, L_, VP],
     "vpf_augment_points": [VP, I, I, I, VP, U32, VP, VP, VP],
     "vpf_image_u8_normalize": [VP, I, I, I, VP, VP, VP, U32, F, VP, VP, VP],
+    "vpf_rotary_axes": [VP, VP],
+    "vpf_gated_norm_fwd": [VP, VP],
+    "vpf_gated_norm_bwd": [VP, VP],
 }
 
 
@@ -226,6 +229,28 @@ class SaLayerBwd(ctypes.Structure):
                 ("dqkv", VP), ("WqkvT", VP), ("base", VP), ("mean1", VP), ("rstd1", VP), ("ln1_g", VP),
                 ("dbase", VP), ("dsum", VP),
                 ("pgrad1", VP), ("dsum_init", I)]
+
+
+class Rotary(ctypes.Structure):
+    """struct VpfRotary (include/vipformer_hip.h)."""
+    _fields_ = [("B", I), ("L", I), ("Hq", I), ("Hk", I), ("head_dim", I), ("P", I), ("axes", I), ("layout", I), ("dtype", I),
+                ("pos_type", I), ("inverse", I), ("pad_", I),
+                ("q", VP), ("k", VP), ("oq", VP), ("ok", VP),
+                ("q_sb", L_), ("q_sl", L_), ("q_sh", L_), ("k_sb", L_), ("k_sl", L_), ("k_sh", L_),
+                ("oq_sb", L_), ("oq_sl", L_), ("oq_sh", L_), ("ok_sb", L_), ("ok_sl", L_), ("ok_sh", L_),
+                ("pos", VP), ("pos_sb", L_), ("freq", VP), ("axis", VP)]
+
+
+class GatedNorm(ctypes.Structure):
+    """struct VpfGatedNorm (include/vipformer_hip.h)."""
+    _fields_ = [("rows", L_), ("gate_rows", L_),
+                ("D", I), ("kind", I), ("x_type", I), ("y_type", I), ("gate_mode", I), ("has_post", I), ("has_pre", I), ("pad_", I),
+                ("alpha", F), ("beta", F), ("eps_post", F), ("eps_pre", F),
+                ("x", VP), ("y", VP), ("gate", VP), ("w_post", VP), ("b_post", VP), ("w_pre", VP), ("b_pre", VP),
+                ("h", VP), ("n", VP), ("stats", VP),
+                ("dh", VP), ("dn", VP), ("dx", VP), ("dy", VP), ("dgate", VP),
+                ("dw_post", VP), ("db_post", VP), ("dw_pre", VP), ("db_pre", VP),
+                ("ws", VP), ("ws_floats", L_)]
 
 
 def call_struct(name: str, struct, *extra) -> None:

@@ -25,6 +25,7 @@ ARCH = "gfx950"
 # -fno-vectorize (round 3): the LOOP vectoriser formed the same instructions in 14 small kernels (BatchNorm pieces, LayerNorm taps ...);
 # check_no_packed_f32 below found them in the round-2 library that was believed to be free of them.
 COMMON = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-fno-slp-vectorize", "-fno-vectorize",
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           "-I" + os.path.join(os.path.dirname(HERE), "include")]
 # preproc.hip: bit-exact kernels -- no fused multiply-adds the source does not spell out
 PER_FILE = {"preproc.hip": ["-ffp-contract=off"]}

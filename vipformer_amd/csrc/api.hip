@@ -44,6 +44,8 @@ extern "C" int vpf_abi_sizeof(int which)
         case 5: return (int)sizeof(VpfAdapterKv);
         case 6: return (int)sizeof(VpfAdapterKvBwd);
         case 7: return (int)sizeof(VpfCaFront);
+        case 8: return (int)sizeof(VpfRotary);
+        case 9: return (int)sizeof(VpfGatedNorm);
         default: return -1;
     }
 }

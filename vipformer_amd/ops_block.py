@@ -1,0 +1,287 @@
+"""Operators of a transformer block over long token sequences (image patches, point groups, video patches), beside the attention,
+LayerNorm and residual pieces of ops.py:
+
+  rotary_axes           rotary positions with several axes (height / width, x / y / z, time / height / width) on queries and keys
+  window_attention      attention inside a sliding window with first tokens that stay visible; training, prompts, single tokens over a cache
+  gated_norm_residual   h = alpha x + beta gate * post(y), n = pre(h): the norms around a block with its gate and residual scale
+
+Heads are a dimension of their own ([B, L, heads, head_dim], any strides whose last dimension is contiguous: slices of one projection's
+output go in as they are).  fp16 and bf16 are chosen by the tensors, per call; the library's build-time operand type does not matter here.
+Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once, and may be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import ops
+
+F32 = torch.float32
+_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}                   # VPF_T_*
+_POS = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}       # VPF_POS_*
+
+
+def _on(device):
+    """The library launches on the CURRENT device's stream: make it the tensors'."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _same_device(what: str, first: torch.Tensor, *rest) -> None:
+    L.need_cuda(first, *rest)
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise L.VpfError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _ptr(t) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    """Batch, token and head stride; 0 where the size is 1 (torch leaves any number there)."""
+    s = t.stride()
+    return tuple(s[i] if t.shape[i] > 1 else 0 for i in range(3))
+
+
+# --------------------------------------------------------------------------- rotary positions with several axes
+class RotaryAxes:
+    """How the channel pairs of a head turn: ``sections[a]`` pairs belong to axis ``a`` of the positions, the channels behind the
+    ``2 * sum(sections)`` rotated ones stay as they are.
+
+    ladder "axis":  pair j of the n pairs of an axis turns by  position * base ** (-j / n)   (every axis sees all wavelengths)
+    ladder "joint": pair p of all P pairs turns by             position[its axis] * base ** (-p / P)
+    layout "half":  pair p is the channels (p, p + P);  "pair": the channels (2 p, 2 p + 1)
+
+    Build it once per model; its tables (fp64 frequencies, axis numbers) are made once per device."""
+
+    def __init__(self, sections: Sequence[int], head_dim: int, base: float = 10000.0, layout: str = "half", ladder: str = "axis"):
+        self.sections, self.head_dim, self.base = tuple(int(n) for n in sections), int(head_dim), float(base)
+        P = sum(self.sections)
+        if not 1 <= len(self.sections) <= 8 or min(self.sections) < 0 or P < 1:
+            raise L.VpfError(f"RotaryAxes: sections {tuple(sections)}: 1 to 8 axes with at least one pair in all")
+        if self.head_dim % 2 or not 2 * P <= self.head_dim <= 1024:
+            raise L.VpfError(f"RotaryAxes: {P} pairs do not fit an even head_dim of at most 1024 (got {head_dim})")
+        if not (math.isfinite(self.base) and self.base > 0.0):
+            raise L.VpfError(f"RotaryAxes: base must be positive and finite (got {base})")
+        if layout not in ("half", "pair") or ladder not in ("axis", "joint"):
+            raise L.VpfError(f"RotaryAxes: layout is 'half' or 'pair', ladder 'axis' or 'joint' (got {layout!r}, {ladder!r})")
+        self.layout, self.ladder, self.pairs = layout, ladder, P
+        self._tables = {}
+
+    def frequencies(self) -> torch.Tensor:
+        """Radians per unit of position of every pair, fp64 on the host."""
+        if self.ladder == "joint":
+            return self.base ** (-torch.arange(self.pairs, dtype=torch.float64) / self.pairs)
+        return torch.cat([self.base ** (-torch.arange(n, dtype=torch.float64) / max(n, 1)) for n in self.sections])
+
+    def tables(self, device: torch.device):
+        t = self._tables.get(device)
+        if t is None:
+            axis = torch.repeat_interleave(torch.arange(len(self.sections), dtype=torch.int32), torch.tensor(self.sections))
+            t = self._tables[device] = ((self.frequencies() / (2.0 * math.pi)).to(device), axis.to(device))
+        return t
+
+
+def _rotary_call(plan, pos, tensors, outs, inverse):
+    q, k = (tensors + (None,))[:2]
+    oq, ok = (outs + (None,))[:2]
+    B, Lt, Hq, dh = q.shape
+    freq, axis = plan.tables(q.device)
+    zero = (0, 0, 0)
+    s = L.Rotary(B, Lt, Hq, 0 if k is None else k.shape[2], dh, plan.pairs, len(plan.sections), int(plan.layout == "pair"), _TYPE[q.dtype],
+                 _POS[pos.dtype], int(inverse), 0, _ptr(q), _ptr(k), _ptr(oq), _ptr(ok), *_strides(q), *(zero if k is None else _strides(k)),
+                 *_strides(oq), *(zero if k is None else _strides(ok)), _ptr(pos),
+                 pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, _ptr(freq), _ptr(axis))
+    with _on(q.device):
+        L.call_struct("vpf_rotary_axes", s)
+
+
+def _rotary_ready(t):
+    """The kernel takes any strides with a contiguous, pair-aligned last dimension; everything else is copied."""
+    if t.stride(3) != 1 or any(s % 2 for s in _strides(t)) or t.data_ptr() % (2 * t.element_size()):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _rotary_run(plan, pos, tensors, inverse):
+    tensors = tuple(_rotary_ready(t) for t in tensors)
+    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors)
+    _rotary_call(plan, pos, tensors, outs, inverse)
+    return outs
+
+
+class RotaryAxesFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, pos, *tensors):
+        ctx.plan = plan
+        ctx.save_for_backward(pos)
+        return _rotary_run(plan, pos, tensors, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        (pos,) = ctx.saved_tensors
+        return (None, None) + _rotary_run(ctx.plan, pos, grads, True)
+
+
+def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryAxes):
+    """Turn the channel pairs of q [B, L, heads, head_dim] and k [B, L, key heads, head_dim] (or None) by their tokens' positions.
+
+    positions: [L, axes] or [B, L, axes] (or [1, L, axes]), integers or fp32 / fp64 coordinates; no gradient reaches them.  Angles are
+    formed in fp64, so positions far into a stream keep their fraction of a turn.  fp32, fp16 and bf16, rounded once.
+    Returns new contiguous tensors (q, k), or q alone where k is None."""
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise L.VpfError(f"rotary_axes: q [B, L, heads, head_dim] and k of the same B, L and head_dim (got {tuple(q.shape)}, "
+                         f"{None if k is None else tuple(k.shape)})")
+    if q.shape[3] != plan.head_dim:
+        raise L.VpfError(f"rotary_axes: head_dim {q.shape[3]}, the plan was built for {plan.head_dim}")
+    if q.dtype not in _TYPE or (k is not None and k.dtype != q.dtype):
+        raise L.VpfError(f"rotary_axes: q and k of one type out of fp32, fp16, bf16 (got {q.dtype}, {None if k is None else k.dtype})")
+    if positions.dim() not in (2, 3) or positions.shape[-2:] != (q.shape[1], len(plan.sections)) or \
+            (positions.dim() == 3 and positions.shape[0] not in (1, q.shape[0])):
+        raise L.VpfError(f"rotary_axes: positions [L, axes] or [B, L, axes] = [({q.shape[0]},) {q.shape[1]}, {len(plan.sections)}] "
+                         f"(got {tuple(positions.shape)})")
+    if positions.dtype not in _POS:
+        raise L.VpfError(f"rotary_axes: positions are int32, int64, fp32 or fp64 (got {positions.dtype})")
+    if positions.requires_grad:
+        raise L.VpfError("rotary_axes: no gradient with respect to the positions (detach them)")
+    _same_device("rotary_axes", q, k, positions)
+    tensors = (q,) if k is None else (q, k)
+    pos = positions.contiguous()
+    outs = RotaryAxesFn.apply(plan, pos, *tensors) if _wants_grad(*tensors) else _rotary_run(plan, pos, tensors, False)
+    return outs[0] if k is None else outs
+
+
+# --------------------------------------------------------------------------- norms around a block, its gate and residual scale
+def _norm_struct(cfg, x, y, gate, params):
+    """The arguments both directions share.  cfg: (kind, gate_mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre)."""
+    kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = cfg
+    D = x.shape[-1]
+    s = L.GatedNorm(x.numel() // D, gate_rows, D, kind, _TYPE[x.dtype], _TYPE[y.dtype], mode, has_post, has_pre, 0, alpha, beta, eps_post, eps_pre,
+                    _ptr(x), _ptr(y), _ptr(gate))
+    s.w_post, s.b_post, s.w_pre, s.b_pre = (_ptr(p) for p in params)
+    return s
+
+
+def _norm_forward(cfg, x, y, gate, params, keep):
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = torch.empty(y.shape, dtype=y.dtype, device=y.device) if cfg[4] else None
+    stats = torch.empty(4, x.numel() // x.shape[-1], dtype=F32, device=x.device) if keep else None
+    s = _norm_struct(cfg, x, y, gate, params)
+    s.h, s.n, s.stats = _ptr(h), _ptr(n), _ptr(stats)
+    with _on(x.device):
+        L.call_struct("vpf_gated_norm_fwd", s)
+    return h, n, stats
+
+
+class GatedNormFn(torch.autograd.Function):
+    """Gradients of parameters go back through autograd, divided by the internal gradient scale the forward ran under (ops.py)."""
+
+    @staticmethod
+    def forward(ctx, cfg, x, y, gate, *params):
+        h, n, stats = _norm_forward(cfg, x, y, gate, params, True)
+        ctx.cfg, ctx.iscale, ctx.gate_is_param = cfg, ops._current_iscale(), isinstance(gate, torch.nn.Parameter)
+        ctx.save_for_backward(x, y, gate, stats, *params)
+        return (h, n) if n is not None else h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh, dn=None):
+        x, y, gate, stats, *params = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dev, D = x.device, x.shape[-1]
+        dh = dh.contiguous()
+        dn = None if dn is None else dn.contiguous()
+        dx = torch.empty_like(x) if need[1] else None
+        dy = torch.empty_like(y) if need[2] else None
+        dgate = torch.empty_like(gate) if need[3] else None
+        s = _norm_struct(ctx.cfg, x, y, gate, params)
+        flat = torch.empty(4, D, dtype=F32, device=dev)
+        grads = [flat[i].view_as(p) if p is not None and need[4 + i] else None for i, p in enumerate(params)]
+        s.stats, s.dh, s.dn, s.dx, s.dy, s.dgate = (_ptr(t) for t in (stats, dh, dn, dx, dy, dgate))
+        s.dw_post, s.db_post, s.dw_pre, s.db_pre = (_ptr(g) for g in grads)
+        floats = L.lib().vpf_gated_norm_ws
+        floats.restype = L.L_
+        ws = torch.empty(max(int(floats(ctypes.byref(s))), 4), dtype=F32, device=dev)
+        s.ws, s.ws_floats = _ptr(ws), ws.numel()
+        with _on(dev):
+            L.call_struct("vpf_gated_norm_bwd", s)
+        inv = ctx.iscale.inv if ctx.iscale is not None else None
+        if inv is not None:
+            flat.mul_(inv)
+            if dgate is not None and ctx.gate_is_param:
+                dgate.mul_(inv)
+        return (None, dx, dy, dgate, *grads)
+
+
+def _norm_params(what, wb, kind, eps, x):
+    """(weight, bias) of one norm, each fp32 [D] or None, and its epsilon."""
+    if wb is None:
+        return (None, None), eps
+    if isinstance(wb, torch.nn.Module):
+        want = {"layer": torch.nn.LayerNorm, "rms": torch.nn.RMSNorm}[kind]
+        if not isinstance(wb, want) or tuple(wb.normalized_shape) != (x.shape[-1],):
+            raise L.VpfError(f"gated_norm_residual: {what}: a {want.__name__} over {x.shape[-1]} channels for kind {kind!r} (got {wb})")
+        eps = torch.finfo(x.dtype).eps if wb.eps is None else wb.eps
+        wb = (wb.weight, getattr(wb, "bias", None))
+    if len(wb) != 2:
+        raise L.VpfError(f"gated_norm_residual: {what} is a norm module or (weight, bias)")
+    for p in wb:
+        if p is not None and (p.dtype != F32 or tuple(p.shape) != (x.shape[-1],)):
+            raise L.VpfError(f"gated_norm_residual: {what}: fp32 parameters of shape ({x.shape[-1]},) (got {p.dtype}, {tuple(p.shape)})")
+    return tuple(None if p is None else p.contiguous() for p in wb), eps
+
+
+def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor] = None, *, post=None, pre=None, kind: str = "layer",
+                        alpha: float = 1.0, beta: float = 1.0, eps: float = 1e-5):
+    """h = alpha * x + beta * gate * post(y);  n = pre(h).  Returns (h, n); n is None where ``pre`` is None.
+
+    x: the residual stream, y: the block's output, both [..., D] with D <= 8192; x is fp32, or x and y are of one type (fp16, bf16).  h has
+    x's type, n has y's; n is taken from h before h is rounded.
+    post / pre: (weight, bias) with fp32 [D] tensors or None entries, a LayerNorm / RMSNorm module, or None for no norm there.
+    kind: "layer" or "rms" (biased variance, ``eps`` inside the root) for both norms; a module brings its own eps.
+    gate: None, fp32 [D], one fp32 row of D per sample (x [B, ..., D]: gate [B, 1, .., D]), or one of x's shape and y's type."""
+    if x.dim() < 1 or x.shape != y.shape or not 1 <= x.shape[-1] <= 8192:
+        raise L.VpfError(f"gated_norm_residual: x and y of one shape [..., D], 1 <= D <= 8192 (got {tuple(x.shape)}, {tuple(y.shape)})")
+    if x.dtype not in _TYPE or y.dtype not in _TYPE or (x.dtype != F32 and x.dtype != y.dtype):
+        raise L.VpfError(f"gated_norm_residual: x is fp32, or x and y are both fp16 or both bf16 (got {x.dtype}, {y.dtype})")
+    if kind not in ("layer", "rms"):
+        raise L.VpfError(f"gated_norm_residual: kind is 'layer' or 'rms' (got {kind!r})")
+    D = x.shape[-1]
+    rows = x.numel() // D
+    if rows >= 1 << 31:
+        raise L.VpfError(f"gated_norm_residual: {rows} rows; at most 2^31 - 1")
+    mode, gate_rows = 0, 1
+    if gate is not None:
+        per_sample = x.dim() >= 2 and gate.dim() == x.dim() and tuple(gate.shape) == (x.shape[0],) + (1,) * (x.dim() - 2) + (D,)
+        if tuple(gate.shape) == (D,):
+            mode, gate_rows = 1, max(rows, 1)
+        elif gate.shape == x.shape and gate.dtype == y.dtype:
+            mode = 2
+        elif per_sample:
+            mode, gate_rows = 1, max(rows // max(x.shape[0], 1), 1)
+        else:
+            raise L.VpfError(f"gated_norm_residual: gate [D], one row per sample or x's shape in y's type (got {tuple(gate.shape)}, {gate.dtype})")
+        if mode == 1 and gate.dtype != F32:
+            raise L.VpfError(f"gated_norm_residual: a gate that is shared by rows is fp32 (got {gate.dtype})")
+    wb_post, eps_post = _norm_params("post", post, kind, eps, x)
+    wb_pre, eps_pre = _norm_params("pre", pre, kind, eps, x)
+    params = wb_post + wb_pre
+    _same_device("gated_norm_residual", x, y, gate, *params)
+    cfg = (int(kind == "rms"), mode, gate_rows, int(post is not None), int(pre is not None), float(alpha), float(beta), float(eps_post),
+           float(eps_pre))
+    x, y, gate = x.contiguous(), y.contiguous(), None if gate is None else gate.contiguous()
+    if not _wants_grad(x, y, gate, *params):
+        return _norm_forward(cfg, x, y, gate, params, False)[:2]
+    out = GatedNormFn.apply(cfg, x, y, gate, *params)
+    return out if pre is not None else (out, None)
