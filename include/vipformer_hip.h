@@ -570,6 +570,31 @@ int vpf_gated_norm_bwd(const VpfGatedNorm* a, void* stream);
 /* floats that a->ws needs (host only; negative: VPF_ERR_*) */
 long vpf_gated_norm_ws(const VpfGatedNorm* a);
 
+/* Attention inside a sliding window with first tokens that stay visible.  n = lens[b] (clamped to 0 .. Lkv; null: Lkv) keys are in use;
+ * query i stands at position p = n - Lq + i (the last query at the last key in use) and sees key j where
+ *   j < n,  j <= p + right,  (j >= p - left or j < sinks),  pad[b, j] == 0        (left / right < 0: open on that side; causal: right = 0)
+ * out = softmax(scale * q k^T over the visible keys) v; a query that sees no key gets zeros and passes no gradient.  Keys and values that
+ * no query sees (behind n, padding, slid out of the window) are never used: they may hold anything, also NaN.
+ * q, out, dout, dq [B, Lq, Hq, head_dim]; k, v, dk, dv [B, Lkv, Hk, head_dim]: fp16 or bf16, 16-byte aligned, strides multiples of 8;
+ * Hk divides Hq, query heads h Hq / Hk .. share key head h.  head_dim a multiple of 8 up to 128.  pad uint8 [B, Lkv], lens int32 [B] (device).
+ * lse fp32 [B, Hk, Lq * Hq / Hk]: log2 of the sum of the exponentials (+inf: nothing visible); forward writes it (null: no gradient follows).
+ * backward needs q, k, v, out, lse of the forward call and its masks; dq, dk, dv are overwritten whole.  Sums are taken in a fixed order. */
+#define VPF_WINDOW_MAX_DIM 128
+typedef struct VpfWindowAttn {
+    int B, Lq, Lkv, Hq, Hk, head_dim, left, right, sinks, dtype;
+    float scale; int pad_;
+    const void* q; const void* k; const void* v; const void* pad; const int* lens;
+    void* out; float* lse;
+    const void* dout; void* dq; void* dk; void* dv;
+    float* ws; long ws_floats;          /* vpf_window_attn_ws floats of scratch (forward: may be null where that is 0) */
+    long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, o_sb, o_sl, o_sh, do_sb, do_sl, do_sh;
+    long dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
+} VpfWindowAttn;
+int vpf_window_attn_fwd(const VpfWindowAttn* a, void* stream);
+int vpf_window_attn_bwd(const VpfWindowAttn* a, void* stream);
+/* floats that a->ws needs (host only; negative: VPF_ERR_*) */
+long vpf_window_attn_ws(const VpfWindowAttn* a, int backward);
+
 #ifdef __cplusplus
 }
 #endif

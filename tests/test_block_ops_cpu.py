@@ -107,3 +107,57 @@ def test_gated_norm_c_abi_refusals():
     # a workspace that is too small is refused before anything is launched
     small = make(gate_mode=1, x=16, y=16, gate=16, dh=16, dn=16, stats=16, ws=16, ws_floats=need - 1)
     assert bwd(ctypes.byref(small), None) == -1
+
+
+def test_window_attention_refusals():
+    assert L.lib().vpf_abi_sizeof(10) == ctypes.sizeof(L.WindowAttn)
+    H = torch.float16
+    q, k = torch.zeros(2, 5, 4, 32, dtype=H), torch.zeros(2, 9, 2, 32, dtype=H)
+    f = O.window_attention
+    refuses("no CPU fallback", f, q, k, k)
+    for a, b, c in ((q[0], k, k), (q, k, k[:, :8]), (q[:1], k, k), (q[..., :16], k, k), (q[:, :, :3], k, k), (q, k[:, :, :0], k[:, :, :0])):
+        refuses("key heads dividing heads", f, a, b, c)
+    refuses("all fp16 or all bf16", f, q.float(), k.float(), k.float())
+    refuses("all fp16 or all bf16", f, q, k.bfloat16(), k)
+    for dh in (4, 20, 136):
+        t = torch.zeros(1, 3, 1, dh, dtype=H)
+        refuses("multiple of 8", f, t, t, t)
+    for w in ((-1, 0), (0, -2), (1.5, 0), (True, 0)):
+        refuses("side of the window", f, q, k, k, w)
+    for s in (-1, 1.0, True):
+        refuses("sinks", f, q, k, k, sinks=s)
+    for s in (0.0, -1.0, float("inf"), float("nan")):
+        refuses("scale", f, q, k, k, scale=s)
+    refuses("pad_mask", f, q, k, k, pad_mask=torch.zeros(2, 9))
+    refuses("pad_mask", f, q, k, k, pad_mask=torch.zeros(2, 5, dtype=torch.bool))
+    refuses("kv_lens", f, q, k, k, kv_lens=torch.zeros(2))
+    refuses("kv_lens", f, q, k, k, kv_lens=torch.zeros(3, dtype=torch.int32))
+    many = torch.zeros(1, 1, 1, 8, dtype=H).expand(1, 1 << 17, 128, 8)
+    refuses("index range", f, many, torch.zeros(1, 9, 1, 8, dtype=H), torch.zeros(1, 9, 1, 8, dtype=H))
+
+
+def test_window_attention_c_abi_refusals():
+    fwd, bwd, ws = L.lib().vpf_window_attn_fwd, L.lib().vpf_window_attn_bwd, L.lib().vpf_window_attn_ws
+    fwd.argtypes = bwd.argtypes = L.SIGS["vpf_window_attn_fwd"]
+    ws.restype = L.L_
+    ok = dict(B=2, Lq=5, Lkv=9, Hq=4, Hk=2, head_dim=32, left=3, right=0, sinks=1, dtype=1, scale=0.2)
+    make = lambda **k: L.WindowAttn(**{**ok, **k})
+    for fn in (fwd, bwd):
+        assert fn(None, None) == -5 and fn(ctypes.byref(make()), None) == -5
+        for bad in (dict(B=-1), dict(Lq=-1), dict(Lkv=1 << 30), dict(Hk=0), dict(Hk=3), dict(head_dim=4), dict(head_dim=36), dict(head_dim=136),
+                    dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(Lq=1 << 29, Hq=8)):
+            assert fn(ctypes.byref(make(**bad)), None) == -1, bad
+        for bad in (dict(dtype=0), dict(dtype=3)):
+            assert fn(ctypes.byref(make(**bad)), None) == -3, bad
+        assert fn(ctypes.byref(make(B=0)), None) == 0
+    full = dict(q=16, k=16, v=16, out=16, lse=16, dout=16, dq=16, dk=16, dv=16, ws=16)
+    assert fwd(ctypes.byref(make(**{**full, "q": 8})), None) == -2                # not 16-byte aligned
+    assert fwd(ctypes.byref(make(**full, k_sl=12)), None) == -2                   # a row stride that is no multiple of 8
+    assert bwd(ctypes.byref(make(**full, dv_sh=4)), None) == -2
+    need = ws(ctypes.byref(make()), 1)
+    assert need >= 2 * 2 * 10 and ws(ctypes.byref(make(Hk=0)), 1) == -1
+    assert bwd(ctypes.byref(make(**full, ws_floats=need - 1)), None) == -1        # refused before anything is launched
+    step = dict(B=1, Lq=1, Lkv=65536, left=-1, sinks=0)
+    need = ws(ctypes.byref(make(**step)), 0)
+    assert need > 0 and fwd(ctypes.byref(make(**{**step, **full}, ws_floats=need - 1)), None) == -1
+    assert fwd(ctypes.byref(make(**{**step, **full, "ws": 0})), None) == -5

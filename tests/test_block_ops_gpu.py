@@ -316,3 +316,183 @@ def test_gated_norm_under_internal_grad_scale():
     s = float(scaled[0].abs().max() / plain[0].abs().max())
     assert s > 1024 and math.log2(s) == int(math.log2(s))
     assert torch.equal(scaled[1], plain[1]) and torch.equal(scaled[2], plain[2])
+
+
+# ------------------------------------------------------------------------------------------ attention inside a sliding window
+def seen_mask(B, Lq, Lkv, window, sinks, pad, lens):
+    """[B, Lq, Lkv] True = visible, straight from the definition."""
+    left, right = ((1 << 40) if s is None else s for s in window)
+    n = torch.full((B,), Lkv) if lens is None else lens.cpu().long().clamp(0, Lkv)
+    p = (n[:, None] - Lq + torch.arange(Lq))[:, :, None]
+    j = torch.arange(Lkv)[None, None, :]
+    m = (j < n[:, None, None]) & (j <= p + right) & ((j >= p - left) | (j < sinks))
+    return m.cuda() if pad is None else m.cuda() & ~pad[:, None, :]
+
+
+def attention_ref(q, k, v, mask, scale, dout=None):
+    """out (and dq, dk, dv) in 64 bits, with the magnitudes their roundings scale with (root of the sums of squares)."""
+    B, Lq, Hq, dh = q.shape
+    Hk = k.shape[2]
+    g = Hq // Hk
+    Q, K, V = (t.detach().double().transpose(1, 2) for t in (q, k, v))                 # [B, H, L, dh]
+    K, V = K.repeat_interleave(g, 1), V.repeat_interleave(g, 1)
+    M = mask[:, None]
+    K, V = (torch.where(mask.any(1)[:, None, :, None], t, 0.0) for t in (K, V))        # keys nobody sees hold anything
+    S = (Q @ K.transpose(-1, -2) * scale).masked_fill(~M, -math.inf)
+    P = torch.nan_to_num(torch.softmax(S, -1), nan=0.0) * M
+    res = {"out": (P @ V, ((P ** 2) @ (V ** 2)).sqrt())}
+    if dout is not None:
+        G = dout.double().transpose(1, 2)
+        dP = G @ V.transpose(-1, -2)
+        delta = (G * res["out"][0]).sum(-1, keepdim=True)
+        dS = P * (dP - delta)
+        # an element of dS carries: its own rounding, P's error through dP - delta, and delta's (out is rounded: half a step of every G out)
+        ddelta = ((G * res["out"][0]) ** 2).sum(-1, keepdim=True).sqrt()
+        e = dS.abs() + P * ddelta
+        group = lambda t: t.reshape(B, Hk, g, *t.shape[2:]).sum(2)
+        res["dq"] = (scale * dS @ K, scale * (e ** 2 @ K ** 2).sqrt())
+        res["dk"] = (group(scale * dS.transpose(-1, -2) @ Q), scale * group((e ** 2).transpose(-1, -2) @ Q ** 2).sqrt())
+        res["dv"] = (group(P.transpose(-1, -2) @ G), group((P ** 2).transpose(-1, -2) @ G ** 2).sqrt())
+    return {n: (a.transpose(1, 2), b.transpose(1, 2)) for n, (a, b) in res.items()}
+
+
+def attention_close(got, ref, size, what):
+    """Elementwise: half a step for the output's rounding, and for the rounding of the weights (P, dS) to the same type, independent from element
+    to element and at most half a step each: the root of the sum of squares times half a step is their standard deviation's bound, 8 of
+    them the limit for any of up to 10^7 elements; fp32 sums of up to 2^15 terms add less than 2^-12 of it.  fp16 weights below 2^-14 are
+    spaced 2^-24: half of that for each of the terms, relative to operands of size 1."""
+    fi = torch.finfo(got.dtype)
+    half = fi.eps / 2
+    tol = half * ref.abs() + 8 * half * size + 1e-6
+    if got.dtype == torch.float16:
+        tol = tol + 8 * 2.0 ** -25 * math.sqrt(ref.shape[1]) * 4
+    d = (got.double() - ref).abs()
+    assert got.shape == ref.shape and torch.isfinite(got.double()).all(), what
+    bad = d - tol
+    assert d.numel() == 0 or float(bad.max()) <= 0.0, f"{what}: {int((bad > 0).sum())} of {d.numel()} outside, worst {float(d.max()):.3e}"
+
+
+def attention_case(B, Lq, Lkv, Hq, Hk, dh, window, sinks, dtype, pad=None, lens=None, train=True, scale=None, seed=0, garbage=True, views=False):
+    from vipformer_amd.ops_block import window_attention
+    g, dt = gen(seed + Lq + 7 * Lkv + dh), TYPES[dtype]
+    if views:
+        buf = randn(g, B, Lq, 3, Hq, dh, dtype=dt)
+        q, k, v = (buf[:, :, i].detach() for i in range(3))
+    else:
+        q, k, v = randn(g, B, Lq, Hq, dh, dtype=dt), randn(g, B, Lkv, Hk, dh, dtype=dt), randn(g, B, Lkv, Hk, dh, dtype=dt)
+    mask = seen_mask(B, Lq, Lkv, window, sinks, pad, lens)
+    if garbage:                                                                        # what no query sees holds NaN and infinities
+        hidden = ~mask.any(1)
+        for t in (k, v):
+            t[hidden] = float("nan")
+            t[:, ::3][hidden[:, ::3]] = float("inf")
+    if train:
+        for t in (q, k, v):
+            t.requires_grad_()
+    out = window_attention(q, k, v, window, sinks=sinks, pad_mask=pad, kv_lens=lens, scale=scale)
+    sc = dh ** -0.5 if scale is None else scale
+    dout = randn(g, B, Lq, Hq, dh, dtype=dt) if train else None
+    ref = attention_ref(q, k, v, mask, sc, dout)
+    attention_close(out.detach(), *ref["out"], "out")
+    empty = ~mask.any(-1)
+    assert float(out.detach()[empty].abs().sum()) == 0.0
+    if not train:
+        return
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    for got, name in zip(grads, ("dq", "dk", "dv")):
+        attention_close(got, *ref[name], name)
+    assert float(grads[0][empty].abs().sum()) == 0.0
+    hidden = ~mask.any(1)
+    assert float(grads[1][hidden].abs().sum()) == 0.0 and float(grads[2][hidden].abs().sum()) == 0.0
+    with torch.no_grad():
+        assert torch.equal(window_attention(q, k, v, window, sinks=sinks, pad_mask=pad, kv_lens=lens, scale=scale), out)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,L,Hq,Hk,dh,window,sinks", [
+    (1, 1, 1, 1, 8, (None, None), 0), (1, 1, 4, 2, 64, (0, 0), 1), (2, 31, 2, 2, 32, (5, 5), 0), (2, 32, 2, 1, 40, (None, 0), 0),
+    (1, 96, 4, 4, 64, (24, 24), 1), (2, 97, 6, 2, 64, (16, 0), 4), (3, 130, 3, 3, 96, (40, 7), 3), (1, 257, 8, 1, 128, (None, None), 0),
+    (2, 333, 4, 2, 80, (100, 60), 70), (1, 700, 2, 2, 64, (0, 0), 0), (1, 1025, 6, 6, 64, (128, 128), 1), (1, 1500, 4, 1, 128, (200, 0), 130),
+    (1, 900, 2, 1, 24, (0, 0), 5), (1, 640, 5, 1, 64, (3, None), 2), (2, 300, 3, 1, 48, (None, 9), 4)])
+def test_window_attention_forward_and_gradients(B, L, Hq, Hk, dh, window, sinks, dtype):
+    attention_case(B, L, L, Hq, Hk, dh, window, sinks, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dh", [32, 56, 96, 120, 128])
+def test_window_attention_every_workgroup_shape(dh, dtype):
+    """Enough rows for workgroups of 128, 64 and 32 of them, with and without shared key heads and padding."""
+    g = gen(dh)
+    for B, L, Hq, Hk in ((32, 190, 8, 8), (64, 65, 8, 2), (64, 100, 2, 2), (3, 60, 2, 2)):
+        pad = torch.arange(L, device="cuda")[None, :] >= torch.randint(1, L + 1, (B, 1), generator=g, device="cuda")
+        attention_case(B, L, L, Hq, Hk, dh, (33, 21), 2, dtype)
+        attention_case(B, L, L, Hq, Hk, dh, (40, 0), 3, dtype, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("Lq,Lkv,window,sinks", [(5, 200, (30, 0), 2), (200, 5, (30, 0), 2), (64, 64, (10, 10), 0), (1, 1000, (100, 0), 4), (130, 300, (None, 0), 0),
+                                                 (3, 0, (4, 4), 1), (0, 3, (4, 4), 1)])
+def test_window_attention_padding_lengths_and_other_query_counts(Lq, Lkv, window, sinks, dtype):
+    g = gen(Lq + Lkv)
+    pad = torch.rand(3, Lkv, generator=g, device="cuda") < 0.4
+    pad[1] = True                                                                      # a sample without any key
+    attention_case(3, Lq, Lkv, 4, 2, 64, window, sinks, dtype, pad=pad)
+    lens = torch.tensor([Lkv, Lkv // 3, 0], device="cuda", dtype=torch.int64 if Lq % 2 else torch.int32)
+    attention_case(3, Lq, Lkv, 4, 4, 64, window, sinks, dtype, lens=lens)
+    attention_case(3, Lq, Lkv, 6, 2, 72, window, sinks, dtype, lens=lens, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lkv,Hq,Hk,dh,left,sinks", [(8, 1, 4096, 16, 4, 128, 1023, 4), (1, 1, 30000, 8, 8, 64, None, 0), (2, 1, 77, 4, 1, 40, 20, 3),
+                                                        (3, 2, 9000, 32, 8, 128, 4000, 1), (16, 1, 5000, 6, 6, 64, 300, 64), (1, 40, 6000, 8, 2, 128, 2000, 4),
+                                                        (1, 1, 1, 64, 1, 128, 0, 0), (5, 3, 2500, 96, 2, 96, 1000, 200)])
+def test_window_attention_single_tokens_over_a_cache(B, Lq, Lkv, Hq, Hk, dh, left, sinks, dtype):
+    """Few queries over a long cache: the keys are split over workgroups; slots outside the window and behind the length hold NaN."""
+    lens = torch.tensor([max(1, Lkv - b * Lkv // B) for b in range(B)], device="cuda", dtype=torch.int32)
+    attention_case(B, Lq, Lkv, Hq, Hk, dh, (left, 0), sinks, dtype, lens=lens, train=False)
+
+
+def test_window_attention_strides_views_scale_and_alignment():
+    from vipformer_amd.ops_block import window_attention
+    attention_case(2, 150, 150, 6, 6, 64, (30, 30), 1, "fp16", views=True, garbage=False)
+    attention_case(1, 200, 200, 4, 4, 128, (64, 0), 2, "bf16", views=True, garbage=False, scale=0.31)
+    g = gen(5)
+    q = randn(g, 2, 4, 60, 64, dtype=torch.float16).transpose(1, 2)                    # heads first
+    odd = randn(g, 2 * 60 * 4 * 64 + 3, dtype=torch.float16)[3:].view(2, 60, 4, 64)    # a base that is not 16-byte aligned
+    rows = randn(g, 2, 60, 4, 68, dtype=torch.float16)[..., :64]                       # a head stride that is no multiple of 8
+    wide = randn(g, 1, 60, 1, 64, dtype=torch.float16).expand(2, 60, 4, 64)            # one tensor for every sample and head
+    for a, b, c in ((q, odd, rows), (odd, wide, q), (rows, q, wide)):
+        a, b, c = (t.detach().requires_grad_() for t in (a, b, c))
+        out = window_attention(a, b, c, (9, 3), sinks=2)
+        dout = randn(g, 2, 4, 60, 64, dtype=torch.float16).transpose(1, 2)
+        ref = attention_ref(a, b, c, seen_mask(2, 60, 60, (9, 3), 2, None, None), 0.125, dout)
+        attention_close(out.detach(), *ref["out"], "out")
+        for got, name in zip(torch.autograd.grad(out, (a, b, c), dout), ("dq", "dk", "dv")):
+            attention_close(got, *ref[name], name)
+
+
+def test_window_attention_large_scores_and_growing_maxima():
+    """Scores from -300 to 300 whose maximum rises along the keys (the running maximum moves many times) and falls."""
+    from vipformer_amd.ops_block import window_attention
+    g = gen(6)
+    for sign in (1.0, -1.0):
+        q, k, v = randn(g, 1, 100, 2, 64), randn(g, 1, 400, 2, 64), randn(g, 1, 400, 2, 64)
+        q[..., 0], k[..., 0] = 20.0, sign * torch.linspace(-12, 12, 400, device="cuda")[None, :, None]
+        q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+        out = window_attention(q, k, v, scale=1.0)
+        ref = attention_ref(q, k, v, torch.ones(1, 100, 400, dtype=torch.bool, device="cuda"), 1.0)
+        # fp32 scores of 300 carry 2^-24 * 300 * log2(e) / 2 + 64 sums: 1e-4 relative in the weights, below half a step of bf16
+        attention_close(out, *ref["out"], "out")
+
+
+def test_window_attention_is_bitwise_reproducible():
+    from vipformer_amd.ops_block import window_attention
+    g = gen(8)
+    q, k, v = (randn(g, 2, 900, h, 64, dtype=torch.bfloat16).requires_grad_() for h in (8, 2, 2))
+    dout = randn(g, 2, 900, 8, 64, dtype=torch.bfloat16)
+    runs = []
+    for _ in range(3):
+        out = window_attention(q, k, v, (60, 0), sinks=4)
+        runs.append([out.detach(), *torch.autograd.grad(out, (q, k, v), dout)])
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))

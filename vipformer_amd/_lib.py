@@ -160,6 +160,8 @@ SIGS = {
     "vpf_rotary_axes": [VP, VP],
     "vpf_gated_norm_fwd": [VP, VP],
     "vpf_gated_norm_bwd": [VP, VP],
+    "vpf_window_attn_fwd": [VP, VP],
+    "vpf_window_attn_bwd": [VP, VP],
 }
 
 
@@ -251,6 +253,15 @@ class GatedNorm(ctypes.Structure):
                 ("dh", VP), ("dn", VP), ("dx", VP), ("dy", VP), ("dgate", VP),
                 ("dw_post", VP), ("db_post", VP), ("dw_pre", VP), ("db_pre", VP),
                 ("ws", VP), ("ws_floats", L_)]
+
+
+class WindowAttn(ctypes.Structure):
+    """struct VpfWindowAttn (include/vipformer_hip.h)."""
+    _fields_ = [("B", I), ("Lq", I), ("Lkv", I), ("Hq", I), ("Hk", I), ("head_dim", I), ("left", I), ("right", I), ("sinks", I), ("dtype", I),
+                ("scale", F), ("pad_", I),
+                ("q", VP), ("k", VP), ("v", VP), ("pad", VP), ("lens", VP), ("out", VP), ("lse", VP),
+                ("dout", VP), ("dq", VP), ("dk", VP), ("dv", VP), ("ws", VP), ("ws_floats", L_)] + \
+               [(f"{t}_{s}", L_) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("sb", "sl", "sh")]
 
 
 def call_struct(name: str, struct, *extra) -> None:

@@ -46,6 +46,7 @@ extern "C" int vpf_abi_sizeof(int which)
         case 7: return (int)sizeof(VpfCaFront);
         case 8: return (int)sizeof(VpfRotary);
         case 9: return (int)sizeof(VpfGatedNorm);
+        case 10: return (int)sizeof(VpfWindowAttn);
         default: return -1;
     }
 }

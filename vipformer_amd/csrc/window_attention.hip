@@ -1,0 +1,900 @@
+// window_attention.hip -- attention inside a sliding window with first tokens that stay visible (gfx950), fp16 and bf16.
+//
+// Query i of a sample stands at position p = n - Lq + i (n keys in use) and sees key j where
+//   j < n,  j <= p + right,  (j >= p - left  or  j < sinks),  and j is not padding.
+// out = softmax(scale q k^T over the visible keys) v; a query that sees nothing gets zeros.
+//
+// Shared key heads: the g = Hq / Hk query heads of a key head are rows of ONE matrix, row r = query r / g, head r % g, so a tile of K and V
+// serves all of them and a single token over a cache still fills a matrix tile.
+//
+// Layout of the products (key index in registers, row on the lane), as in attention.hip:
+//   S^T[key, row] = K[key, :] . Q[row, :]        A = K rows (LDS), B = Q (registers)
+//   O^T[d, row] += V^T[d, key] . P^T[key, row]   A = V columns (LDS, transposing reads), B = P straight from the accumulators of S^T
+// Statistics are per-lane scalars in fp32, in units of log2; P is rounded to the tensors' type for the second product (at most half a step of
+// 2^-9 / 2^-12 relative for each weight, the size of the output's own rounding).
+//
+// LDS tiles hold rows of NC 16-byte chunks without padding; chunk c of row r sits at c ^ swz(r).  Over 64 banks of 4 bytes a fragment read
+// takes the same chunk of 16 consecutive rows (they must differ modulo 16 chunks) and a transposing read takes 4 chunks side by side of 4
+// consecutive rows (they must fall into the 4 groups of 4 chunks): swz does both.
+#include "vpf_elem.h"
+
+typedef __attribute__((ext_vector_type(4))) short wa_s16x4;
+typedef __attribute__((ext_vector_type(8))) short wa_s16x8;
+typedef __attribute__((ext_vector_type(16))) float wa_f32x16;
+#define WA_LOG2E 1.4426950408889634f
+#define WA_THREADS 256
+#define WA_FAR (1 << 30)                // an open side of the window; positions and lengths stay below it
+
+template <typename T> struct WaMma;
+template <> struct WaMma<vpf_f16> {
+    typedef __attribute__((ext_vector_type(8))) vpf_f16 v8;
+    static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct WaMma<vpf_bf16> {
+    typedef __attribute__((ext_vector_type(8))) vpf_bf16 v8;
+    static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+struct WaArgs {
+    VpfWindowAttn a;
+    int g, rows;                // query heads per key head; rows of one (sample, key head)
+    uint32_t magic;             // r / g == umulhi(r, magic) for r < 2^32 / g (g > 1)
+    int tiles, splits;          // row tiles; parts of a row tile's keys
+    float c;                    // scale * log2(e)
+    int ktiles, sink_tiles, chunks, chunk_rows;      // backward: key tiles, those with sinks, pieces of the rows far behind those and their size
+};
+
+__device__ __forceinline__ int wa_query(const WaArgs& w, int r) { return w.g == 1 ? r : (int)__umulhi((uint32_t)r, w.magic); }
+__device__ __forceinline__ float wa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float wa_half_max(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float wa_half_sum(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ wa_f32x16 wa_zero16()
+{
+    wa_f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+template <typename T> __device__ __forceinline__ typename WaMma<T>::v8 wa_pack8(const float* f)
+{
+    typename WaMma<T>::v8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)f[i];
+    return v;
+}
+
+// ------------------------------------------------------------------ LDS tiles
+template <int DP> struct WaTile {
+    static constexpr int CH = DP / 8;                                       // 16-byte chunks of a row that hold data
+    static constexpr int NC = DP <= 32 ? 4 : DP <= 64 ? 8 : 16;             // chunks of a row in LDS
+    static constexpr int PITCH = NC * 16;
+    static __device__ __forceinline__ int swz(int r)
+    {
+        return NC == 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : NC == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3;
+    }
+    static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ swz(r)) << 4); }
+};
+// element (row0 + (lane & 31), 16 s + 8 (lane >> 5) + j): operand fragment from rows of the tile
+template <typename T, int DP> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_row(const char* t, int row0, int s)
+{
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const typename WaMma<T>::v8*>(t + WaTile<DP>::at(row0 + (lane & 31), 2 * s + (lane >> 5)));
+}
+// element (k, 32 dt + (lane & 31)) with k in the order of an accumulator used as operand: slot (h, j) <-> k = row0 + 8 (j >> 2) + 4 h + (j & 3)
+template <typename T, int DP> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_col(const char* t, int row0, int dt)
+{
+    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3, h = g >> 1;
+    const int row = row0 + 4 * h + q, c = 4 * dt + 2 * (g & 1) + (p >> 1);
+    typedef wa_s16x4 __attribute__((address_space(3)))* lds_p;
+    const wa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + WaTile<DP>::at(row, c) + 8 * (p & 1)));
+    const wa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + WaTile<DP>::at(row + 8, c) + 8 * (p & 1)));
+    const wa_s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename WaMma<T>::v8, v);
+}
+
+// ------------------------------------------------------------------ what a sample's rows see
+struct WaSeen { int n, off; };                                              // keys in use; position of query 0
+__device__ __forceinline__ WaSeen wa_seen(const WaArgs& w, int b)
+{
+    WaSeen s;
+    s.n = w.a.Lkv;
+    if (w.a.lens) s.n = max(0, min(w.a.lens[b], w.a.Lkv));
+    s.off = s.n - w.a.Lq;
+    return s;
+}
+// The keys a block of rows at positions pmin .. pmax can see: the first `first` ones, then lo .. hi; walked in stages of `stage` keys
+struct WaSpan { int first, lo, hi, nfirst, total; };
+__device__ __forceinline__ WaSpan wa_span(const WaArgs& w, const WaSeen& s, int pmin, int pmax, int stage)
+{
+    WaSpan k;
+    k.hi = max(0, min(pmax + w.a.right + 1, s.n));
+    k.lo = min(max(0, pmin - w.a.left), k.hi);
+    k.first = min(w.a.sinks, k.lo);
+    k.nfirst = (k.first + stage - 1) / stage;
+    k.total = k.nfirst + (k.hi - k.lo + stage - 1) / stage;
+    return k;
+}
+
+// Consecutive workgroups go to different XCDs (8, each with an L2 of its own): give each XCD a run of consecutive items, whose rows share
+// their keys.
+__device__ __forceinline__ int wa_item(int id, int total)
+{
+    const int per = total / 8, cut = per * 8;
+    return id < cut ? (id & 7) * per + (id >> 3) : id;
+}
+
+// A thread's part of a stage of ROWS rows: chunk i of it is row (tid + 256 i) / CH, chunk (tid + 256 i) % CH
+template <int DP, int ROWS> struct WaStage {
+    static constexpr int CH = WaTile<DP>::CH, N = ROWS * CH, PER = (N + WA_THREADS - 1) / WA_THREADS;
+    uint4 v[PER];
+    template <typename F> __device__ __forceinline__ void load(int dh, F src)   // src(row): address of the row or null
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * WA_THREADS, row = c / CH, ch = c % CH;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (c < N && 8 * ch < dh) {
+                const char* p = (const char*)src(row);
+                if (p) v[i] = *reinterpret_cast<const uint4*>(p + 16 * ch);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* t) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = threadIdx.x + i * WA_THREADS;
+            if (c < N) *reinterpret_cast<uint4*>(t + WaTile<DP>::at(c / CH, c % CH)) = v[i];
+        }
+    }
+};
+
+// Scores of one 32-key block (accumulator order: key kk + (r & 3) + 8 (r >> 2) + 4 hl) that the lane's row does not see -> -inf
+__device__ __forceinline__ void wa_hide(wa_f32x16& s, int kk, int hl, int top, int low, int sinks, const uint32_t* padw)
+{
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int j = kk + (r & 3) + 8 * (r >> 2) + 4 * hl;
+        bool see = j <= top && (j >= low || j < sinks);
+        if (padw) see = see && !((padw[2 * (r >> 2) + hl] >> (8 * (r & 3))) & 0xffu);
+        s[r] = see ? s[r] : -INFINITY;
+    }
+}
+
+// ------------------------------------------------------------------ forward
+// Workgroup = 4 waves = RB blocks of 32 rows x KS parts of a stage's keys (SUBK each); K and V are double-buffered in LDS, the loads of the
+// next stage are in flight during the products of this one.  splits > 1: the stages of a row tile are divided over workgroups, whose
+// (maximum, sum, unnormalised output) wa_join_kernel joins.
+template <typename T, int DP, int RB, int KS, int SUBK>
+__global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
+{
+    using Tile = WaTile<DP>;
+    constexpr int STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char lds[];               // [2][K, V][STAGE rows], [2][STAGE] padding bytes
+    const VpfWindowAttn& a = w.a;
+    char* const pads = lds + 4 * BUF;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
+    const int item = wa_item(blockIdx.x, gridDim.x);
+    const int split = item % w.splits, tile = item / w.splits % w.tiles, bh = item / w.splits / w.tiles, b = bh / a.Hk, hk = bh % a.Hk;
+    const WaSeen seen = wa_seen(w, b);
+    const int r0 = tile * 32 * RB, rend = min(r0 + 32 * RB, w.rows);
+    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1), STAGE);
+    const int t0 = (int)((long)span.total * split / w.splits), t1 = (int)((long)span.total * (split + 1) / w.splits);
+
+    // this lane's row
+    const int row = r0 + rb * 32 + (lane & 31), rq = min(row, w.rows - 1), qi = wa_query(w, rq);
+    const int pos = seen.off + qi, wlast = min(r0 + rb * 32 + 31, w.rows - 1);
+    const bool live = r0 + rb * 32 < w.rows;
+    const int wmin = seen.off + wa_query(w, min(r0 + rb * 32, w.rows - 1)), wmax = seen.off + wa_query(w, wlast);
+    typename WaMma<T>::v8 qf[KST];
+    {
+        const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + (hk * w.g + (rq - qi * w.g)) * a.q_sh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            const int d = 16 * s + 8 * hl;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (d < a.head_dim) u = *reinterpret_cast<const uint4*>(qp + d);
+            qf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
+        }
+    }
+    const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
+    const char* vp = (const char*)((const T*)a.v + b * a.v_sb + hk * a.v_sh);
+    const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
+
+    wa_f32x16 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = wa_zero16();
+    float m = -INFINITY, l = 0.f;
+
+    WaStage<DP, STAGE> rk, rv;
+    uint8_t rp = 0;
+    auto bounds = [&](int t, int& k0, int& kend) {
+        if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
+        else { k0 = span.lo + (t - span.nfirst) * STAGE; kend = span.hi; }
+    };
+    auto load = [&](int t) {
+        int k0, kend;
+        bounds(t, k0, kend);
+        rk.load(a.head_dim, [&](int r) { return k0 + r < kend ? kp + (size_t)(k0 + r) * a.k_sl * sizeof(T) : nullptr; });
+        // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
+        rv.load(a.head_dim, [&](int r) { return k0 + r < kend && !(pad && pad[k0 + r]) ? vp + (size_t)(k0 + r) * a.v_sl * sizeof(T) : nullptr; });
+        if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
+    };
+    auto store = [&](int buf) {
+        rk.store(lds + buf * 2 * BUF);
+        rv.store(lds + buf * 2 * BUF + BUF);
+        if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+    };
+    if (t0 < t1) { load(t0); store(t0 & 1); }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        if (t + 1 < t1) load(t + 1);
+        int k0, kend;
+        bounds(t, k0, kend);
+        k0 += ks * SUBK;
+        const char* sk = lds + (t & 1) * 2 * BUF;
+        const char* sv = sk + BUF;
+        const int top = min(kend - 1, pos + a.right), low = pos - a.left;
+        // nothing of this part is visible to the wave's rows / everything is
+        const bool none = !live || k0 >= kend || k0 > wmax + a.right || (k0 + SUBK <= wmin - a.left && k0 >= a.sinks);
+        if (!none) {
+            wa_f32x16 s[NB];
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                s[kb] = wa_zero16();
+#pragma unroll
+                for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T, DP>(sk, ks * SUBK + 32 * kb, i), qf[i], s[kb]);
+            }
+            const bool all = !pad && k0 + SUBK <= kend && k0 + SUBK - 1 <= wmin + a.right && (k0 >= wmax - a.left || k0 + SUBK <= a.sinks);
+            if (!all) {
+#pragma unroll
+                for (int kb = 0; kb < NB; ++kb)
+                    wa_hide(s[kb], k0 + 32 * kb, hl, top, low, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+            mx = wa_half_max(mx) * w.c;
+            // The running maximum only has to keep exp2 in range: it moves when a row has outgrown it by 2^8 (weights up to 256 fit every type)
+            if (__any(mx > m + 8.f)) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : wa_exp2(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+            }
+            const float base = m == -INFINITY ? 0.f : m;                     // a row that has seen nothing yet: every weight is exp2(-inf)
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb) {
+                float p[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) { p[r] = wa_exp2(fmaf(s[kb][r], w.c, -base)); l += p[r]; }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sv, ks * SUBK + 32 * kb + 16 * i, dt), pf, o[dt]);
+                }
+            }
+        }
+        if (t + 1 < t1) store((t + 1) & 1);
+        __syncthreads();
+    }
+    if (KS > 1) {                                                            // join the key parts through LDS (the stages are done with)
+        float* slots = reinterpret_cast<float*>(lds);
+        constexpr int SLOT = (DT * 16 + 2) * 64;
+        static_assert((KS / 2) * RB * SLOT * 4 <= 4 * BUF, "the partial results fit the stage buffers");
+#pragma unroll
+        for (int step = KS / 2; step >= 1; step >>= 1) {
+            if (ks >= step && ks < 2 * step) {
+                float* slot = slots + ((ks - step) * RB + rb) * SLOT + lane;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) slot[(dt * 16 + r) * 64] = o[dt][r];
+                slot[DT * 16 * 64] = m; slot[(DT * 16 + 1) * 64] = l;
+            }
+            __syncthreads();
+            if (ks < step) {
+                const float* slot = slots + (ks * RB + rb) * SLOT + lane;
+                const float m2 = slot[DT * 16 * 64], mn = fmaxf(m, m2);
+                const float f1 = m == -INFINITY ? 0.f : wa_exp2(m - mn), f2 = m2 == -INFINITY ? 0.f : wa_exp2(m2 - mn);
+                l = l * f1 + slot[(DT * 16 + 1) * 64] * f2;
+                m = mn;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * f1 + slot[(dt * 16 + r) * 64] * f2;
+            }
+            if (step > 1) __syncthreads();
+        }
+    }
+    if (ks != 0 || row >= w.rows) return;
+    l = wa_half_sum(l);
+    if (w.splits > 1) {
+        const size_t at = ((size_t)split * a.B * a.Hk + bh) * w.rows + row;
+        float* part = a.ws + at * DP;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4*>(part + 32 * dt + 8 * j + 4 * hl) = make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+        if (hl == 0) reinterpret_cast<float2*>(a.ws + (size_t)w.splits * a.B * a.Hk * w.rows * DP)[at] = make_float2(m, l);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* op = (T*)a.out + b * a.o_sb + qi * a.o_sl + (hk * w.g + (rq - qi * w.g)) * a.o_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * dt + 8 * j + 4 * hl;
+            const float v[4] = {o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv, o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv};
+            if (d < a.head_dim) vpf_store<T, 4>(op + d, v);
+        }
+    if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// parts of the keys -> output: one wave per row, the lanes hold DP / 64 channels each
+template <typename T, int DP>
+__global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
+{
+    const VpfWindowAttn& a = w.a;
+    const size_t all = (size_t)a.B * a.Hk * w.rows, at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (at >= all) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + (size_t)w.splits * all * DP);
+    float m = -INFINITY;
+    for (int s = 0; s < w.splits; ++s) m = fmaxf(m, ml[s * all + at].x);
+    constexpr int N = (DP + 63) / 64;
+    float l = 0.f, o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.f;
+    for (int s = 0; s < w.splits; ++s) {
+        const float2 p = ml[s * all + at];
+        const float f = p.x == -INFINITY ? 0.f : wa_exp2(p.x - m);
+        l += p.y * f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (lane + 64 * i < DP) o[i] += a.ws[(s * all + at) * DP + lane + 64 * i] * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int bh = (int)(at / w.rows), row = (int)(at % w.rows), qi = wa_query(w, row);
+    T* op = (T*)a.out + bh / a.Hk * a.o_sb + qi * a.o_sl + (bh % a.Hk * w.g + (row - qi * w.g)) * a.o_sh;
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (lane + 64 * i < a.head_dim) op[lane + 64 * i] = (T)(o[i] * inv);
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// ------------------------------------------------------------------ backward: queries
+// dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO . O);  dQ = scale dS K.  The walk over the keys is the forward kernel's; delta is
+// kept for the kernel of the keys.  dS is rounded to the tensors' type for its product, as P is.
+template <typename T, int DP, int RB, int KS>
+__global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
+{
+    using Tile = WaTile<DP>;
+    constexpr int SUBK = KS == 4 ? 32 : 64, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const VpfWindowAttn& a = w.a;
+    char* const pads = lds + 4 * BUF;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
+    const int item = wa_item(blockIdx.x, gridDim.x);
+    const int tile = item % w.tiles, bh = item / w.tiles, b = bh / a.Hk, hk = bh % a.Hk;
+    const WaSeen seen = wa_seen(w, b);
+    const int r0 = tile * 32 * RB, rend = min(r0 + 32 * RB, w.rows);
+    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1), STAGE);
+    const int row = r0 + rb * 32 + (lane & 31), rq = min(row, w.rows - 1), qi = wa_query(w, rq), head = hk * w.g + (rq - qi * w.g);
+    const int pos = seen.off + qi, wlast = min(r0 + rb * 32 + 31, w.rows - 1);
+    const bool live = r0 + rb * 32 < w.rows;
+    const int wmin = seen.off + wa_query(w, min(r0 + rb * 32, w.rows - 1)), wmax = seen.off + wa_query(w, wlast);
+    typename WaMma<T>::v8 qf[KST], gf[KST];
+    float delta = 0.f;
+    {
+        const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + head * a.q_sh;
+        const T* gp = (const T*)a.dout + b * a.do_sb + qi * a.do_sl + head * a.do_sh;
+        const T* op = (const T*)a.out + b * a.o_sb + qi * a.o_sl + head * a.o_sh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            const int d = 16 * s + 8 * hl;
+            uint4 u = make_uint4(0, 0, 0, 0), v = u, x = u;
+            if (d < a.head_dim) { u = *reinterpret_cast<const uint4*>(qp + d); v = *reinterpret_cast<const uint4*>(gp + d); x = *reinterpret_cast<const uint4*>(op + d); }
+            qf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
+            gf[s] = __builtin_bit_cast(typename WaMma<T>::v8, v);
+            const typename WaMma<T>::v8 of = __builtin_bit_cast(typename WaMma<T>::v8, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * (float)of[i];
+        }
+        delta = wa_half_sum(delta);
+        if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
+    }
+    const float lse = a.lse[(size_t)bh * w.rows + rq];
+    const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
+    const char* vp = (const char*)((const T*)a.v + b * a.v_sb + hk * a.v_sh);
+    const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
+    wa_f32x16 dq[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dq[dt] = wa_zero16();
+
+    WaStage<DP, STAGE> rk, rv;
+    uint8_t rp = 0;
+    auto bounds = [&](int t, int& k0, int& kend) {
+        if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
+        else { k0 = span.lo + (t - span.nfirst) * STAGE; kend = span.hi; }
+    };
+    auto load = [&](int t) {
+        int k0, kend;
+        bounds(t, k0, kend);
+        rk.load(a.head_dim, [&](int r) { return k0 + r < kend && !(pad && pad[k0 + r]) ? kp + (size_t)(k0 + r) * a.k_sl * sizeof(T) : nullptr; });
+        rv.load(a.head_dim, [&](int r) { return k0 + r < kend ? vp + (size_t)(k0 + r) * a.v_sl * sizeof(T) : nullptr; });
+        if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
+    };
+    auto store = [&](int buf) {
+        rk.store(lds + buf * 2 * BUF);
+        rv.store(lds + buf * 2 * BUF + BUF);
+        if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+    };
+    if (span.total > 0) { load(0); store(0); }
+    __syncthreads();
+    for (int t = 0; t < span.total; ++t) {
+        if (t + 1 < span.total) load(t + 1);
+        int k0, kend;
+        bounds(t, k0, kend);
+        k0 += ks * SUBK;
+        const char* sk = lds + (t & 1) * 2 * BUF;
+        const char* sv = sk + BUF;
+        const int top = min(kend - 1, pos + a.right), low = pos - a.left;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) {
+            const int kk = k0 + 32 * kb;
+            if (!live || kk >= kend || kk > wmax + a.right || (kk + 32 <= wmin - a.left && kk >= a.sinks)) continue;
+            wa_f32x16 s = wa_zero16(), dp = wa_zero16();
+#pragma unroll
+            for (int i = 0; i < KST; ++i) {
+                s = WaMma<T>::mma(wa_frag_row<T, DP>(sk, ks * SUBK + 32 * kb, i), qf[i], s);
+                dp = WaMma<T>::mma(wa_frag_row<T, DP>(sv, ks * SUBK + 32 * kb, i), gf[i], dp);
+            }
+            const bool all = !pad && kk + 32 <= kend && kk + 31 <= wmin + a.right && (kk >= wmax - a.left || kk + 32 <= a.sinks);
+            if (!all) wa_hide(s, kk, hl, top, low, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = wa_exp2(fmaf(s[r], w.c, -lse));
+                ds[r] = p * (dp[r] - delta);
+                if (!all) ds[r] = s[r] == -INFINITY ? 0.f : ds[r];           // what a hidden key holds stays out
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const typename WaMma<T>::v8 df = wa_pack8<T>(ds + 8 * i);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sk, ks * SUBK + 32 * kb + 16 * i, dt), df, dq[dt]);
+            }
+        }
+        if (t + 1 < span.total) store((t + 1) & 1);
+        __syncthreads();
+    }
+    if (KS > 1) {
+        float* slots = reinterpret_cast<float*>(lds);
+        constexpr int SLOT = DT * 16 * 64;
+        static_assert((KS / 2) * RB * SLOT * 4 <= 4 * BUF, "the partial results fit the stage buffers");
+#pragma unroll
+        for (int step = KS / 2; step >= 1; step >>= 1) {
+            if (ks >= step && ks < 2 * step) {
+                float* slot = slots + ((ks - step) * RB + rb) * SLOT + lane;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) slot[(dt * 16 + r) * 64] = dq[dt][r];
+            }
+            __syncthreads();
+            if (ks < step) {
+                const float* slot = slots + (ks * RB + rb) * SLOT + lane;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dq[dt][r] += slot[(dt * 16 + r) * 64];
+            }
+            if (step > 1) __syncthreads();
+        }
+    }
+    if (ks != 0 || row >= w.rows) return;
+    T* op = (T*)a.dq + b * a.dq_sb + qi * a.dq_sl + head * a.dq_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * dt + 8 * j + 4 * hl;
+            const float v[4] = {dq[dt][4 * j] * a.scale, dq[dt][4 * j + 1] * a.scale, dq[dt][4 * j + 2] * a.scale, dq[dt][4 * j + 3] * a.scale};
+            if (d < a.head_dim) vpf_store<T, 4>(op + d, v);
+        }
+}
+
+// ------------------------------------------------------------------ backward: keys
+// dV = P^T dO, dK = scale dS^T Q, summed over the rows (queries and heads) that see the key, in one fixed order.
+// Workgroup = 64 keys: 2 blocks of 32 keys x 2 halves of a 64-row stage of Q and dO (double-buffered in LDS); K and V of the wave's keys stay in
+// registers as operands (key on the lane).  The first tokens are seen by every row behind them: the rows beyond their window are cut into
+// pieces of chunk_rows, one workgroup each, and wa_sink_join_kernel adds the pieces.
+#define WA_KT 64
+struct WaRowRange { int lo, hi; };
+__device__ __forceinline__ WaRowRange wa_rows_of(const WaArgs& w, const WaSeen& s, int k0)
+{
+    // positions k0 - right .. k0 + 63 + left; queries 0 .. Lq - 1 stand at off ..
+    const long lo = max((long)k0 - w.a.right - s.off, 0L), hi = min((long)k0 + WA_KT - 1 + w.a.left - s.off + 1, (long)w.a.Lq);
+    WaRowRange r;
+    r.lo = (int)min(lo, (long)w.a.Lq) * w.g;
+    r.hi = max((int)max(hi, 0L) * w.g, r.lo);
+    return r;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
+{
+    using Tile = WaTile<DP>;
+    constexpr int ROWS = 64, KST = DP / 16, DT = DP / 32, BUF = ROWS * Tile::PITCH;
+    extern __shared__ __attribute__((aligned(16))) char lds[];               // [2][Q, dO][64 rows], [2][lse, delta, position][64]
+    const VpfWindowAttn& a = w.a;
+    float* const stats = reinterpret_cast<float*>(lds + 4 * BUF);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, kb = wave & 1, qs = wave >> 1;
+    const int item = wa_item(blockIdx.x, gridDim.x), items = w.ktiles + w.sink_tiles * w.chunks;
+    const int bh = item / items, it = item % items, b = bh / a.Hk, hk = bh % a.Hk;
+    const bool far = it >= w.ktiles;
+    const int kt = far ? (it - w.ktiles) / w.chunks : it, chunk = far ? (it - w.ktiles) % w.chunks : 0, kt0 = kt * WA_KT;
+    const WaSeen seen = wa_seen(w, b);
+    WaRowRange rr = wa_rows_of(w, seen, kt0);
+    if (kt0 >= seen.n) rr.hi = rr.lo;                                        // keys behind the ones in use
+    else if (kt0 < a.sinks) {
+        if (w.chunks == 0) rr.hi = max(rr.hi, w.rows);
+        else if (far) { const int f = rr.hi; rr.lo = max(f, chunk * w.chunk_rows); rr.hi = min(w.rows, (chunk + 1) * w.chunk_rows); }
+    }
+
+    const int key = kt0 + 32 * kb + (lane & 31), kc = min(key, a.Lkv - 1);
+    const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
+    const bool kok = key < seen.n && !(pad && pad[kc]);
+    typename WaMma<T>::v8 kf[KST], vf[KST];
+    {
+        const T* kp = (const T*)a.k + b * a.k_sb + kc * a.k_sl + hk * a.k_sh;
+        const T* vp = (const T*)a.v + b * a.v_sb + kc * a.v_sl + hk * a.v_sh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            const int d = 16 * s + 8 * hl;
+            uint4 u = make_uint4(0, 0, 0, 0), v = u;
+            if (d < a.head_dim && kok) { u = *reinterpret_cast<const uint4*>(kp + d); v = *reinterpret_cast<const uint4*>(vp + d); }
+            kf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
+            vf[s] = __builtin_bit_cast(typename WaMma<T>::v8, v);
+        }
+    }
+    wa_f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) { dk[dt] = wa_zero16(); dv[dt] = wa_zero16(); }
+    const int kmin = kt0 + 32 * kb, kmax = kmin + 31;
+    const bool whole = !pad && kmax < seen.n;
+
+    WaStage<DP, ROWS> rq, rg;
+    float r_lse = 0.f, r_delta = 0.f;
+    int r_pos = 0;
+    auto load = [&](int r0) {
+        auto src = [&](const void* base, long sb, long sl, long sh, int r) -> const char* {
+            if (r0 + r >= rr.hi) return nullptr;
+            const int qi = wa_query(w, r0 + r);
+            return (const char*)((const T*)base + b * sb + qi * sl + (hk * w.g + (r0 + r - qi * w.g)) * sh);
+        };
+        rq.load(a.head_dim, [&](int r) { return src(a.q, a.q_sb, a.q_sl, a.q_sh, r); });
+        rg.load(a.head_dim, [&](int r) { return src(a.dout, a.do_sb, a.do_sl, a.do_sh, r); });
+        if (threadIdx.x < ROWS) {
+            const int r = r0 + threadIdx.x, rc = min(r, w.rows - 1);
+            r_lse = r < rr.hi ? a.lse[(size_t)bh * w.rows + rc] : INFINITY;  // weight 0
+            r_delta = a.ws[(size_t)bh * w.rows + rc];
+            r_pos = seen.off + wa_query(w, rc);
+        }
+    };
+    auto store = [&](int buf) {
+        rq.store(lds + buf * 2 * BUF);
+        rg.store(lds + buf * 2 * BUF + BUF);
+        if (threadIdx.x < ROWS) {
+            float* s = stats + buf * 3 * ROWS + threadIdx.x;
+            s[0] = r_lse; s[ROWS] = r_delta; reinterpret_cast<int*>(s)[2 * ROWS] = r_pos;
+        }
+    };
+    const int steps = (rr.hi - rr.lo + ROWS - 1) / ROWS;
+    if (steps > 0) { load(rr.lo); store(0); }
+    __syncthreads();
+    for (int t = 0; t < steps; ++t) {
+        if (t + 1 < steps) load(rr.lo + (t + 1) * ROWS);
+        const char* sq = lds + (t & 1) * 2 * BUF;
+        const char* sg = sq + BUF;
+        const float* st = stats + (t & 1) * 3 * ROWS + 32 * qs + 4 * hl;
+        const int* sp = reinterpret_cast<const int*>(stats + (t & 1) * 3 * ROWS + 2 * ROWS + 32 * qs);
+        const int rlo = rr.lo + t * ROWS + 32 * qs;
+        const int pmin = sp[0], pmax = sp[31];
+        if (rlo < rr.hi && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
+            wa_f32x16 s = wa_zero16(), dp = wa_zero16();
+#pragma unroll
+            for (int i = 0; i < KST; ++i) {
+                s = WaMma<T>::mma(wa_frag_row<T, DP>(sq, 32 * qs, i), kf[i], s);
+                dp = WaMma<T>::mma(wa_frag_row<T, DP>(sg, 32 * qs, i), vf[i], dp);
+            }
+            const bool all = whole && kmax <= pmin + a.right && (kmin >= pmax - a.left || kmax < a.sinks);
+            float p[16], ds[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 lse = *reinterpret_cast<const float4*>(st + 8 * j), dl = *reinterpret_cast<const float4*>(st + ROWS + 8 * j);
+                const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
+                const int4 po = *reinterpret_cast<const int4*>(sp + 4 * hl + 8 * j);
+                const int ps[4] = {po.x, po.y, po.z, po.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * j + e;
+                    p[r] = wa_exp2(fmaf(s[r], w.c, -ls[e]));
+                    ds[r] = p[r] * (dp[r] - de[e]);
+                    if (!all) {
+                        const bool see = kok && key <= ps[e] + a.right && (key >= ps[e] - a.left || key < a.sinks);
+                        p[r] = see ? p[r] : 0.f;
+                        ds[r] = see ? ds[r] : 0.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i), df = wa_pack8<T>(ds + 8 * i);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    dv[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sg, 32 * qs + 16 * i, dt), pf, dv[dt]);
+                    dk[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sq, 32 * qs + 16 * i, dt), df, dk[dt]);
+                }
+            }
+        }
+        if (t + 1 < steps) store((t + 1) & 1);
+        __syncthreads();
+    }
+    // the two halves of the rows: through LDS, dV first
+    float* slot = reinterpret_cast<float*>(lds) + kb * (DT * 16 * 64) + lane;
+    static_assert(2 * DT * 16 * 64 * 4 <= 4 * BUF, "the partial results fit the stage buffers");
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        wa_f32x16* acc = pass ? dk : dv;
+        if (pass) __syncthreads();
+        if (qs == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) slot[(dt * 16 + r) * 64] = acc[dt][r];
+        }
+        __syncthreads();
+        if (qs == 0) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[dt][r] += slot[(dt * 16 + r) * 64];
+        }
+    }
+    if (qs != 0) return;
+    if (kt < w.sink_tiles && w.chunks > 0) {                                 // one of the pieces of a tile with first tokens
+        const size_t piece = ((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1) + (far ? chunk + 1 : 0);
+        float* part = a.ws + (size_t)a.B * a.Hk * w.rows + (piece * WA_KT + 32 * kb + (lane & 31)) * 2 * DP;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 32 * dt + 8 * j + 4 * hl;
+                *reinterpret_cast<float4*>(part + d) = make_float4(dk[dt][4 * j], dk[dt][4 * j + 1], dk[dt][4 * j + 2], dk[dt][4 * j + 3]);
+                *reinterpret_cast<float4*>(part + DP + d) = make_float4(dv[dt][4 * j], dv[dt][4 * j + 1], dv[dt][4 * j + 2], dv[dt][4 * j + 3]);
+            }
+        return;
+    }
+    if (key >= a.Lkv) return;
+    T* okp = (T*)a.dk + b * a.dk_sb + key * a.dk_sl + hk * a.dk_sh;
+    T* ovp = (T*)a.dv + b * a.dv_sb + key * a.dv_sl + hk * a.dv_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int d = 32 * dt + 8 * j + 4 * hl;
+            const float x[4] = {dk[dt][4 * j] * a.scale, dk[dt][4 * j + 1] * a.scale, dk[dt][4 * j + 2] * a.scale, dk[dt][4 * j + 3] * a.scale};
+            const float y[4] = {dv[dt][4 * j], dv[dt][4 * j + 1], dv[dt][4 * j + 2], dv[dt][4 * j + 3]};
+            if (d < a.head_dim) { vpf_store<T, 4>(okp + d, x); vpf_store<T, 4>(ovp + d, y); }
+        }
+}
+
+// pieces of the key tiles with first tokens -> dk, dv: one workgroup per key and (sample, key head)
+template <typename T, int DP>
+__global__ void __launch_bounds__(2 * DP) wa_sink_join_kernel(WaArgs w)
+{
+    const VpfWindowAttn& a = w.a;
+    const int per = min(w.sink_tiles * WA_KT, a.Lkv), bh = blockIdx.x / per, key = blockIdx.x % per, kt = key / WA_KT, d = threadIdx.x % DP;
+    const bool is_v = threadIdx.x >= DP;
+    const float* p = a.ws + (size_t)a.B * a.Hk * w.rows + ((((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1)) * WA_KT + key % WA_KT) * 2 * DP + threadIdx.x;
+    float s = 0.f;
+    for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * WA_KT * 2 * DP];
+    if (d >= a.head_dim) return;
+    const int b = bh / a.Hk, hk = bh % a.Hk;
+    if (is_v) ((T*)a.dv)[b * a.dv_sb + key * a.dv_sl + hk * a.dv_sh + d] = (T)s;
+    else ((T*)a.dk)[b * a.dk_sb + key * a.dk_sl + hk * a.dk_sh + d] = (T)(s * a.scale);
+}
+
+// ------------------------------------------------------------------ host
+static int wa_dp(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
+
+static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
+{
+    if (!args) return VPF_ERR_NULL;
+    w = {};
+    w.a = *args;
+    VpfWindowAttn& a = w.a;
+    if (a.B < 0 || a.Lq < 0 || a.Lkv < 0 || a.Hk < 1 || a.Hq < a.Hk || a.Hq % a.Hk || a.head_dim < 8 || a.head_dim > VPF_WINDOW_MAX_DIM || a.head_dim % 8 ||
+        a.Lkv >= WA_FAR || a.Lq >= WA_FAR || a.sinks < 0 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return VPF_ERR_BADSHAPE;
+    if (a.dtype != VPF_T_F16 && a.dtype != VPF_T_BF16) return VPF_ERR_UNSUPPORTED;
+    a.left = a.left < 0 || a.left > WA_FAR ? WA_FAR : a.left;
+    a.right = a.right < 0 || a.right > WA_FAR ? WA_FAR : a.right;
+    a.sinks = a.sinks < a.Lkv ? a.sinks : a.Lkv;
+    if (a.left >= a.Lkv) a.sinks = 0;                            // everything behind a query is in its window
+    w.g = a.Hq / a.Hk;
+    if ((long)a.Lq * w.g * w.g >= 1L << 31 || (long)a.B * a.Hk >= 1L << 24) return VPF_ERR_BADSHAPE;
+    w.rows = a.Lq * w.g;
+    w.magic = w.g > 1 ? (uint32_t)((1ULL << 32) / w.g + 1) : 0;
+    w.c = a.scale * WA_LOG2E;
+    return VPF_OK;
+}
+static bool wa_aligned(const void* p, long sb, long sl, long sh) { return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0; }
+
+// Row blocks of 32 per workgroup (4, 2 or 1; the waves that are left split a stage's keys): as many as leave a workgroup for each of the 256 CUs.
+// Then, where even single blocks are too few, parts of the keys: two workgroups per CU, each with at least two stages.
+static void wa_plan_fwd(WaArgs& w, int& rb)
+{
+    const long bh = (long)w.a.B * w.a.Hk;
+    rb = bh * vpf_cdiv(w.rows, 128) >= 256 ? 4 : bh * vpf_cdiv(w.rows, 64) >= 256 ? 2 : 1;
+    w.tiles = vpf_cdiv(w.rows, 32 * rb);
+    w.splits = 1;
+    const long wgs = bh * w.tiles;
+    if (rb == 1 && wgs < 256) {
+        const long span = (long)w.a.left + w.a.right + 1 + 31 / w.g + w.a.sinks, keys = span < w.a.Lkv ? span : w.a.Lkv;
+        const long stages = (keys + 127) / 128, want = (512 + wgs - 1) / wgs;
+        w.splits = (int)(want < stages / 2 ? want : stages / 2);
+        if (w.splits < 1) w.splits = 1;
+    }
+}
+static long wa_fwd_ws(const WaArgs& w) { return w.splits > 1 ? (long)w.splits * w.a.B * w.a.Hk * w.rows * (wa_dp(w.a.head_dim) + 2) : 0; }
+
+// The rows behind a sink tile's own window are cut into pieces about as long as the row range of an ordinary tile, where that leaves
+// more than one of them.
+static void wa_plan_bwd(WaArgs& w)
+{
+    const VpfWindowAttn& a = w.a;
+    w.ktiles = vpf_cdiv(a.Lkv, WA_KT);
+    w.sink_tiles = vpf_cdiv(a.sinks, WA_KT);
+    w.chunks = 0;
+    const long range = ((long)a.left + a.right + WA_KT) * w.g;
+    if (w.sink_tiles > 0 && w.rows > 2 * range) {
+        long rows = range > 512 ? range : 512;
+        w.chunk_rows = (int)((rows + 63) / 64 * 64);
+        w.chunks = vpf_cdiv(w.rows, w.chunk_rows);
+    }
+}
+static long wa_bwd_ws(const WaArgs& w)
+{
+    const long rows = ((long)w.a.B * w.a.Hk * w.rows + 3) / 4 * 4;
+    return rows + (w.chunks ? (long)w.a.B * w.a.Hk * w.sink_tiles * (w.chunks + 1) * WA_KT * 2 * wa_dp(w.a.head_dim) : 0);
+}
+
+// more than 64 KB of LDS has to be asked for, once per kernel and device
+template <typename K> static int wa_lds(K kernel, size_t bytes, VpfPerDevice& done)
+{
+    bool& d = done();
+    if (!d && bytes > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) return VPF_ERR_HIP;
+    d = true;
+    return VPF_OK;
+}
+
+template <typename T, int DP, int RB, int KS, int SUBK> static int wa_launch_fwd(const WaArgs& w, hipStream_t st)
+{
+    constexpr size_t lds = 4 * SUBK * KS * WaTile<DP>::PITCH + 2 * SUBK * KS;
+    static VpfPerDevice done;
+    if (const int rc = wa_lds(wa_fwd_kernel<T, DP, RB, KS, SUBK>, lds, done)) return rc;
+    const long grid = (long)w.a.B * w.a.Hk * w.tiles * w.splits;
+    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
+    hipLaunchKernelGGL((wa_fwd_kernel<T, DP, RB, KS, SUBK>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
+    if (w.splits > 1) hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3(vpf_cdiv((long)w.a.B * w.a.Hk * w.rows, 4)), dim3(WA_THREADS), 0, st, w);
+    VPF_CHECK_LAUNCH();
+    return VPF_OK;
+}
+template <typename T, int DP> static int wa_fwd(const WaArgs& w, int rb, hipStream_t st)
+{
+    if (rb == 4) return wa_launch_fwd<T, DP, 4, 1, 64>(w, st);
+    if (rb == 2) return wa_launch_fwd<T, DP, 2, 2, 64>(w, st);
+    return wa_launch_fwd<T, DP, 1, 4, 32>(w, st);
+}
+
+template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaArgs& w, hipStream_t st)
+{
+    constexpr int STAGE = (KS == 4 ? 32 : 64) * KS;
+    constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + 2 * STAGE;
+    static VpfPerDevice done;
+    if (const int rc = wa_lds(wa_dq_kernel<T, DP, RB, KS>, lds, done)) return rc;
+    hipLaunchKernelGGL((wa_dq_kernel<T, DP, RB, KS>), dim3((unsigned)((long)w.a.B * w.a.Hk * w.tiles)), dim3(WA_THREADS), lds, st, w);
+    VPF_CHECK_LAUNCH();
+    return VPF_OK;
+}
+template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
+{
+    const long bh = (long)w.a.B * w.a.Hk;
+    if (w.rows > 0) {
+        const int rb = bh * vpf_cdiv(w.rows, 128) >= 256 ? 4 : bh * vpf_cdiv(w.rows, 64) >= 256 ? 2 : 1;
+        w.tiles = vpf_cdiv(w.rows, 32 * rb);
+        const int rc = rb == 4 ? wa_launch_dq<T, DP, 4, 1>(w, st) : rb == 2 ? wa_launch_dq<T, DP, 2, 2>(w, st) : wa_launch_dq<T, DP, 1, 4>(w, st);
+        if (rc) return rc;
+    }
+    if (w.a.Lkv == 0) return VPF_OK;
+    constexpr size_t lds = 4 * 64 * WaTile<DP>::PITCH + 6 * 64 * 4;
+    static VpfPerDevice done;
+    if (const int rc = wa_lds(wa_dkv_kernel<T, DP>, lds, done)) return rc;
+    const long grid = bh * (w.ktiles + (long)w.sink_tiles * w.chunks);
+    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
+    hipLaunchKernelGGL((wa_dkv_kernel<T, DP>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
+    if (w.chunks) {
+        const int per = w.sink_tiles * WA_KT < w.a.Lkv ? w.sink_tiles * WA_KT : w.a.Lkv;
+        hipLaunchKernelGGL((wa_sink_join_kernel<T, DP>), dim3((unsigned)(bh * per)), dim3(2 * DP), 0, st, w);
+    }
+    VPF_CHECK_LAUNCH();
+    return VPF_OK;
+}
+
+#define WA_PICK(FN, ...) \
+    switch (wa_dp(w.a.head_dim)) { \
+        case 32: return w.a.dtype == VPF_T_F16 ? FN<vpf_f16, 32>(__VA_ARGS__) : FN<vpf_bf16, 32>(__VA_ARGS__); \
+        case 64: return w.a.dtype == VPF_T_F16 ? FN<vpf_f16, 64>(__VA_ARGS__) : FN<vpf_bf16, 64>(__VA_ARGS__); \
+        case 96: return w.a.dtype == VPF_T_F16 ? FN<vpf_f16, 96>(__VA_ARGS__) : FN<vpf_bf16, 96>(__VA_ARGS__); \
+        default: return w.a.dtype == VPF_T_F16 ? FN<vpf_f16, 128>(__VA_ARGS__) : FN<vpf_bf16, 128>(__VA_ARGS__); \
+    }
+
+extern "C" long vpf_window_attn_ws(const VpfWindowAttn* args, int backward)
+{
+    WaArgs w;
+    if (const int rc = wa_prepare(args, w)) return rc;
+    if ((long)w.a.B * w.rows == 0 && !backward) return 0;
+    int rb;
+    if (backward) { wa_plan_bwd(w); return wa_bwd_ws(w); }
+    wa_plan_fwd(w, rb);
+    return wa_fwd_ws(w);
+}
+
+extern "C" int vpf_window_attn_fwd(const VpfWindowAttn* args, void* stream)
+{
+    (void)hipGetLastError();
+    WaArgs w;
+    if (const int rc = wa_prepare(args, w)) return rc;
+    const VpfWindowAttn& a = w.a;
+    if ((long)a.B * w.rows == 0) return VPF_OK;
+    if (!a.q || !a.out || (a.Lkv > 0 && (!a.k || !a.v))) return VPF_ERR_NULL;
+    if (!wa_aligned(a.q, a.q_sb, a.q_sl, a.q_sh) || !wa_aligned(a.k, a.k_sb, a.k_sl, a.k_sh) || !wa_aligned(a.v, a.v_sb, a.v_sl, a.v_sh) ||
+        !wa_aligned(a.out, a.o_sb, a.o_sl, a.o_sh) || !vpf_aligned(a.ws, 16)) return VPF_ERR_BADALIGN;
+    int rb;
+    wa_plan_fwd(w, rb);
+    if (w.splits > 1 && (!a.ws || a.ws_floats < wa_fwd_ws(w))) return a.ws ? VPF_ERR_BADSHAPE : VPF_ERR_NULL;
+    WA_PICK(wa_fwd, w, rb, (hipStream_t)stream)
+}
+
+extern "C" int vpf_window_attn_bwd(const VpfWindowAttn* args, void* stream)
+{
+    (void)hipGetLastError();
+    WaArgs w;
+    if (const int rc = wa_prepare(args, w)) return rc;
+    const VpfWindowAttn& a = w.a;
+    if (a.B == 0 || (w.rows == 0 && a.Lkv == 0)) return VPF_OK;
+    if ((w.rows > 0 && (!a.q || !a.out || !a.dout || !a.lse || !a.dq || !a.ws)) || (a.Lkv > 0 && (!a.k || !a.v || !a.dk || !a.dv))) return VPF_ERR_NULL;
+    const struct { const void* p; long sb, sl, sh; } t[] = {{a.q, a.q_sb, a.q_sl, a.q_sh}, {a.k, a.k_sb, a.k_sl, a.k_sh}, {a.v, a.v_sb, a.v_sl, a.v_sh},
+        {a.out, a.o_sb, a.o_sl, a.o_sh}, {a.dout, a.do_sb, a.do_sl, a.do_sh}, {a.dq, a.dq_sb, a.dq_sl, a.dq_sh}, {a.dk, a.dk_sb, a.dk_sl, a.dk_sh},
+        {a.dv, a.dv_sb, a.dv_sl, a.dv_sh}, {a.ws, 0, 0, 0}};
+    for (const auto& x : t) if (!wa_aligned(x.p, x.sb, x.sl, x.sh)) return VPF_ERR_BADALIGN;
+    wa_plan_bwd(w);
+    if (a.ws_floats < wa_bwd_ws(w)) return VPF_ERR_BADSHAPE;
+    WA_PICK(wa_bwd, w, (hipStream_t)stream)
+}

@@ -285,3 +285,120 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
         return _norm_forward(cfg, x, y, gate, params, False)[:2]
     out = GatedNormFn.apply(cfg, x, y, gate, *params)
     return out if pre is not None else (out, None)
+
+
+# --------------------------------------------------------------------------- attention inside a sliding window
+def _attn_ready(t: torch.Tensor) -> torch.Tensor:
+    """16-byte rows: a contiguous last dimension, strides that are multiples of 8 elements and an aligned base; everything else is copied."""
+    if t.stride(3) != 1 or any(s % 8 for s in _strides(t)) or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _attn_struct(cfg, q, k, v, pad, lens, out, lse):
+    left, right, sinks, scale = cfg
+    B, Lq, Hq, dh = q.shape
+    s = L.WindowAttn(B, Lq, k.shape[1], Hq, k.shape[2], dh, left, right, sinks, _TYPE[q.dtype], scale, 0, _ptr(q), _ptr(k), _ptr(v), _ptr(pad),
+                     _ptr(lens), _ptr(out), _ptr(lse))
+    for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+        _attn_strides(s, name, t)
+    return s
+
+
+def _attn_strides(s, name, t):
+    sb, sl, sh = _strides(t)
+    setattr(s, name + "_sb", sb), setattr(s, name + "_sl", sl), setattr(s, name + "_sh", sh)
+
+
+def _attn_workspace(s, backward, device):
+    fn = L.lib().vpf_window_attn_ws
+    fn.restype = L.L_
+    n = int(fn(ctypes.byref(s), backward))
+    L.check(min(n, 0), "vpf_window_attn_ws")
+    ws = torch.empty(n, dtype=F32, device=device) if n else None
+    s.ws, s.ws_floats = _ptr(ws), n
+    return ws
+
+
+def _attn_forward(cfg, q, k, v, pad, lens, keep):
+    B, Lq, Hq, dh = q.shape
+    out = torch.empty(B, Lq, Hq, dh, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, k.shape[2], Lq * Hq // k.shape[2], dtype=F32, device=q.device) if keep else None
+    s = _attn_struct(cfg, q, k, v, pad, lens, out, lse)
+    ws = _attn_workspace(s, 0, q.device)        # noqa: F841  (alive until the launch is issued; the allocator orders its reuse by stream)
+    with _on(q.device):
+        L.call_struct("vpf_window_attn_fwd", s)
+    return out, lse
+
+
+class WindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, cfg, q, k, v, pad, lens):
+        q, k, v = _attn_ready(q), _attn_ready(k), _attn_ready(v)
+        out, lse = _attn_forward(cfg, q, k, v, pad, lens, True)
+        ctx.cfg = cfg
+        ctx.save_for_backward(q, k, v, out, lse, pad, lens)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, pad, lens = ctx.saved_tensors
+        dout = _attn_ready(dout)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        s = _attn_struct(ctx.cfg, q, k, v, pad, lens, out, lse)
+        s.dout, s.dq, s.dk, s.dv = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv)
+        for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
+            _attn_strides(s, name, t)
+        ws = _attn_workspace(s, 1, q.device)    # noqa: F841
+        with _on(q.device):
+            L.call_struct("vpf_window_attn_bwd", s)
+        return None, dq, dk, dv, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: Tuple[Optional[int], Optional[int]] = (None, None), *,
+                     sinks: int = 0, scale: Optional[float] = None, pad_mask: Optional[torch.Tensor] = None,
+                     kv_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale q k^T over the visible keys) v for q [B, Lq, heads, head_dim] and k, v [B, Lkv, key heads, head_dim]; fp16 or bf16.
+
+    window = (left, right): query at position p sees keys p - left .. p + right (None: open on that side; (n, 0) is causal), and of the first
+    ``sinks`` keys those up to p + right, however far behind they are.
+    With n keys in use the last query stands at the last of them: query i at position n - Lq + i.  n is Lkv, or kv_lens[b] (int32 / int64 [B],
+    on the device, read by the kernels: a captured graph follows it): a preallocated cache that is filled to different lengths.
+    pad_mask: bool [B, Lkv], True = this key is padding (as the ``pad_mask`` of the framework's encoders); it moves no positions.
+    Keys that no query sees may hold anything.  A query that sees nothing gets zeros (and passes no gradient).
+    Key heads are shared by heads / key heads consecutive query heads.  head_dim: a multiple of 8 up to 128; scale defaults to head_dim ** -0.5.
+    Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v.  There is no dropout on the weights here."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] < 1 or \
+            q.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise L.VpfError(f"window_attention: q [B, Lq, heads, head_dim], k and v [B, Lkv, key heads, head_dim], key heads dividing heads (got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise L.VpfError(f"window_attention: q, k and v all fp16 or all bf16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+    B, Lq, Hq, dh = q.shape
+    Lkv, g = k.shape[1], Hq // k.shape[2]
+    if dh % 8 or not 8 <= dh <= 128:
+        raise L.VpfError(f"window_attention: head_dim is a multiple of 8 up to 128 (got {dh})")
+    if Lkv >= 1 << 30 or Lq * g * g >= 1 << 31:
+        raise L.VpfError(f"window_attention: Lq {Lq}, Lkv {Lkv}, {g} heads per key head: beyond the kernels' index range")
+    left, right = window
+    for side in (left, right):
+        if side is not None and (isinstance(side, bool) or not isinstance(side, int) or side < 0):
+            raise L.VpfError(f"window_attention: a side of the window is None or a whole number >= 0 (got {window})")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+        raise L.VpfError(f"window_attention: sinks is a whole number >= 0 (got {sinks})")
+    scale = dh ** -0.5 if scale is None else float(scale)
+    if not (0.0 < scale < math.inf):
+        raise L.VpfError(f"window_attention: scale must be positive and finite (got {scale})")
+    if pad_mask is not None and (pad_mask.dtype != torch.bool or tuple(pad_mask.shape) != (B, Lkv)):
+        raise L.VpfError(f"window_attention: pad_mask is bool [B, Lkv] = {(B, Lkv)} (got {pad_mask.dtype}, {tuple(pad_mask.shape)})")
+    if kv_lens is not None and (kv_lens.dtype not in (torch.int32, torch.int64) or tuple(kv_lens.shape) != (B,)):
+        raise L.VpfError(f"window_attention: kv_lens is int32 or int64 [B] = {(B,)} (got {kv_lens.dtype}, {tuple(kv_lens.shape)})")
+    _same_device("window_attention", q, k, v, pad_mask, kv_lens)
+    top = (1 << 30) - 1
+    cfg = (-1 if left is None else min(left, top), -1 if right is None else min(right, top), min(sinks, top), scale)
+    pad = None if pad_mask is None else pad_mask.contiguous().view(torch.uint8)
+    lens = None if kv_lens is None else kv_lens.to(torch.int32).contiguous()
+    if not _wants_grad(q, k, v):
+        return _attn_forward(cfg, _attn_ready(q), _attn_ready(k), _attn_ready(v), pad, lens, False)[0]
+    return WindowAttentionFn.apply(cfg, q, k, v, pad, lens)
