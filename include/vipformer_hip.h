@@ -578,13 +578,15 @@ long vpf_gated_norm_ws(const VpfGatedNorm* a);
  * q, out, dout, dq [B, Lq, Hq, head_dim]; k, v, dk, dv [B, Lkv, Hk, head_dim]: fp16 or bf16, 16-byte aligned, strides multiples of 8;
  * Hk divides Hq, query heads h Hq / Hk .. share key head h.  head_dim a multiple of 8 up to 128.  pad uint8 [B, Lkv], lens int32 [B] (device).
  * lse fp32 [B, Hk, Lq * Hq / Hk]: log2 of the sum of the exponentials (+inf: nothing visible); forward writes it (null: no gradient follows).
- * backward needs q, k, v, out, lse of the forward call and its masks; dq, dk, dv are overwritten whole.  Sums are taken in a fixed order. */
+ * out_lo: out's type, [B, Hk, Lq * Hq / Hk, head_dim] contiguous: what rounding took from out (null with lse).
+ * backward needs q, k, v, out, out_lo, lse of the forward call and its masks; dq, dk, dv are overwritten whole.  Sums are taken in a fixed order. */
 #define VPF_WINDOW_MAX_DIM 128
+#define VPF_WINDOW_MAX_STRIDE (1L << 23)        /* token and head strides stay below it (elements) */
 typedef struct VpfWindowAttn {
     int B, Lq, Lkv, Hq, Hk, head_dim, left, right, sinks, dtype;
     float scale; int pad_;
     const void* q; const void* k; const void* v; const void* pad; const int* lens;
-    void* out; float* lse;
+    void* out; float* lse; void* out_lo;
     const void* dout; void* dq; void* dk; void* dv;
     float* ws; long ws_floats;          /* vpf_window_attn_ws floats of scratch (forward: may be null where that is 0) */
     long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, o_sb, o_sl, o_sh, do_sb, do_sl, do_sh;

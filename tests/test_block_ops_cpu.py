@@ -150,7 +150,7 @@ def test_window_attention_c_abi_refusals():
         for bad in (dict(dtype=0), dict(dtype=3)):
             assert fn(ctypes.byref(make(**bad)), None) == -3, bad
         assert fn(ctypes.byref(make(B=0)), None) == 0
-    full = dict(q=16, k=16, v=16, out=16, lse=16, dout=16, dq=16, dk=16, dv=16, ws=16)
+    full = dict(q=16, k=16, v=16, out=16, lse=16, out_lo=16, dout=16, dq=16, dk=16, dv=16, ws=16)
     assert fwd(ctypes.byref(make(**{**full, "q": 8})), None) == -2                # not 16-byte aligned
     assert fwd(ctypes.byref(make(**full, k_sl=12)), None) == -2                   # a row stride that is no multiple of 8
     assert bwd(ctypes.byref(make(**full, dv_sh=4)), None) == -2

@@ -82,23 +82,40 @@ template <int DP> struct WaTile {
     }
     static __device__ __forceinline__ int at(int r, int c) { return r * PITCH + ((c ^ swz(r)) << 4); }
 };
-// element (row0 + (lane & 31), 16 s + 8 (lane >> 5) + j): operand fragment from rows of the tile
-template <typename T, int DP> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_row(const char* t, int row0, int s)
+// Fragment addresses are LDS bytes.  The chunk number is XORed into bits that the row leaves zero, so ONE base per tile and lane reaches every
+// fragment: base ^ (a constant of the fragment) + (a constant of the row block).
+__device__ __forceinline__ uint32_t wa_lds_byte(const void* p) { return (uint32_t)(size_t)(__attribute__((address_space(3))) const char*)p; }
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"      // (LDS pointers are 32 bits wide)
+// operand from rows: element (row0 + (lane & 31), 16 s + 8 (lane >> 5) + j); `base` of wa_row_base, `at` = the bytes of row0 (a multiple of 16 rows)
+template <int DP> __device__ __forceinline__ uint32_t wa_row_base()
 {
     const int lane = threadIdx.x & 63;
-    return *reinterpret_cast<const typename WaMma<T>::v8*>(t + WaTile<DP>::at(row0 + (lane & 31), 2 * s + (lane >> 5)));
+    return WaTile<DP>::at(lane & 31, lane >> 5);
 }
-// element (k, 32 dt + (lane & 31)) with k in the order of an accumulator used as operand: slot (h, j) <-> k = row0 + 8 (j >> 2) + 4 h + (j & 3)
-template <typename T, int DP> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_col(const char* t, int row0, int dt)
+template <typename T> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_row(uint32_t base, int s, uint32_t at)
 {
-    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3, h = g >> 1;
-    const int row = row0 + 4 * h + q, c = 4 * dt + 2 * (g & 1) + (p >> 1);
+    typedef typename WaMma<T>::v8 __attribute__((address_space(3)))* lds_p;
+    return *(lds_p)((base ^ (uint32_t)(s << 5)) + at);
+}
+// operand from columns: element (k, 32 dt + (lane & 31)), k in the order of an accumulator used as operand: slot (h, j) <-> k = row0 + 8 (j >> 2) + 4 h + (j & 3)
+template <int DP> __device__ __forceinline__ uint32_t wa_col_base()
+{
+    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+    return WaTile<DP>::at(4 * (g >> 1) + q, 2 * (g & 1) + (p >> 1)) + 8 * (p & 1);
+}
+template <typename T, int DP> __device__ __forceinline__ typename WaMma<T>::v8 wa_frag_col(uint32_t base, int dt, uint32_t at)
+{
     typedef wa_s16x4 __attribute__((address_space(3)))* lds_p;
-    const wa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + WaTile<DP>::at(row, c) + 8 * (p & 1)));
-    const wa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(t + WaTile<DP>::at(row + 8, c) + 8 * (p & 1)));
+    const wa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)((base ^ (uint32_t)(dt << 6)) + at));
+    // eight rows on, the swizzle has turned chunk bit 1
+    const wa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)((base ^ (uint32_t)(dt << 6) ^ 32u) + at + 8 * WaTile<DP>::PITCH));
     const wa_s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename WaMma<T>::v8, v);
 }
+#pragma clang diagnostic pop
+// keeps the optimiser from holding every XORed address of a loop in a register of its own
+__device__ __forceinline__ uint32_t wa_opaque(uint32_t v) { asm volatile("" : "+v"(v)); return v; }
 
 // ------------------------------------------------------------------ what a sample's rows see
 struct WaSeen { int n, off; };                                              // keys in use; position of query 0
@@ -131,28 +148,53 @@ __device__ __forceinline__ int wa_item(int id, int total)
     return id < cut ? (id & 7) * per + (id >> 3) : id;
 }
 
-// A thread's part of a stage of ROWS rows: chunk i of it is row (tid + 256 i) / CH, chunk (tid + 256 i) % CH
+// Stages travel memory -> LDS without registers (global_load_lds, 16 bytes a lane): a wave instruction fills 1 KB of the tile, lane i its 16
+// bytes at + 16 i, so the swizzle is made on the global side: the lane fetches the chunk whose place it fills.  The rows a lane serves in
+// its instructions are STEP apart, a multiple of the swizzle's period, so row0 and the chunk are the same for all of them.
+// The instruction is issued from inline asm (through the builtin the compiler waits for it in front of every LDS read); a stage is awaited by
+// wa_stage_wait in front of the barrier that opens it.  Rows and chunks that do not exist are replaced by ones that do (finite where the
+// product takes a zero weight); keys that are padding come from wa_zeros.
+__device__ const uint4 wa_zeros[WA_THREADS / 64] = {};
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"          // (m0 is reserved: it is what the instruction takes its LDS address from)
+__device__ __forceinline__ void wa_dma(const void* base, uint32_t off, uint32_t lds_byte)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds_byte), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void wa_dma_any(const void* p, uint32_t lds_byte)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds_byte), "v"(p) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void wa_stage_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <int DP, int ROWS> struct WaStage {
-    static constexpr int CH = WaTile<DP>::CH, N = ROWS * CH, PER = (N + WA_THREADS - 1) / WA_THREADS;
-    uint4 v[PER];
-    template <typename F> __device__ __forceinline__ void load(int dh, F src)   // src(row): address of the row or null
+    static constexpr int PITCH = WaTile<DP>::PITCH, PER = ROWS * PITCH / 4096, STEP = 4096 / PITCH;      // wave instructions of one tile per wave
+    static_assert(ROWS * PITCH % 4096 == 0, "a stage is whole instructions of all four waves");
+    int row0;                   // this lane's row in the wave's first instruction
+    uint32_t col;               // its chunk, in bytes
+    uint32_t wave_byte;
+    __device__ __forceinline__ WaStage(int dh)
     {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int c = threadIdx.x + i * WA_THREADS, row = c / CH, ch = c % CH;
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (c < N && 8 * ch < dh) {
-                const char* p = (const char*)src(row);
-                if (p) v[i] = *reinterpret_cast<const uint4*>(p + 16 * ch);
-            }
-        }
+        const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = wave * 1024 + (threadIdx.x & 63) * 16;
+        row0 = at / PITCH;
+        const int c = (at % PITCH / 16) ^ WaTile<DP>::swz(row0);
+        col = 8 * c < dh ? 16 * c : 0;
+        wave_byte = wave * 1024;
     }
-    __device__ __forceinline__ void store(char* t) const
+    // rows 0 .. last (the others repeat the last one) of a matrix with `stride` bytes from row to row
+    __device__ __forceinline__ void rows(const char* base, uint32_t stride, int last, uint32_t tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) wa_dma(base, (uint32_t)min(row0 + i * STEP, last) * stride + col, tile + wave_byte + i * 4096);
+    }
+    // the same, with zeros where pad[row] is set
+    __device__ __forceinline__ void rows_padded(const char* base, uint32_t stride, int last, const uint8_t* pad, uint32_t tile) const
     {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int c = threadIdx.x + i * WA_THREADS;
-            if (c < N) *reinterpret_cast<uint4*>(t + WaTile<DP>::at(c / CH, c % CH)) = v[i];
+            const int r = min(row0 + i * STEP, last);
+            const char* p = pad[r] ? (const char*)wa_zeros : base + (size_t)r * stride + col;
+            wa_dma_any(p, tile + wave_byte + i * 4096);
         }
     }
 };
@@ -178,7 +220,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char lds[];               // [2][K, V][STAGE rows], [2][STAGE] padding bytes
+    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][K, V][STAGE rows], [2][STAGE] padding bytes
     const VpfWindowAttn& a = w.a;
     char* const pads = lds + 4 * BUF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
@@ -214,7 +256,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     for (int dt = 0; dt < DT; ++dt) o[dt] = wa_zero16();
     float m = -INFINITY, l = 0.f;
 
-    WaStage<DP, STAGE> rk, rv;
+    const WaStage<DP, STAGE> stage(a.head_dim);
+    const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
     uint8_t rp = 0;
     auto bounds = [&](int t, int& k0, int& kend) {
         if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
@@ -223,15 +266,19 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     auto load = [&](int t) {
         int k0, kend;
         bounds(t, k0, kend);
-        rk.load(a.head_dim, [&](int r) { return k0 + r < kend ? kp + (size_t)(k0 + r) * a.k_sl * sizeof(T) : nullptr; });
+        const int last = min(STAGE, kend - k0) - 1;
+        const char* kb = kp + (size_t)k0 * a.k_sl * sizeof(T);
+        const char* vb = vp + (size_t)k0 * a.v_sl * sizeof(T);
+        const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
         // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
-        rv.load(a.head_dim, [&](int r) { return k0 + r < kend && !(pad && pad[k0 + r]) ? vp + (size_t)(k0 + r) * a.v_sl * sizeof(T) : nullptr; });
+        if (pad) stage.rows_padded(vb, (uint32_t)(a.v_sl * sizeof(T)), last, pad + k0, at + BUF);
+        else stage.rows(vb, (uint32_t)(a.v_sl * sizeof(T)), last, at + BUF);
+        stage.rows(kb, (uint32_t)(a.k_sl * sizeof(T)), last, at);
         if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
     };
     auto store = [&](int buf) {
-        rk.store(lds + buf * 2 * BUF);
-        rv.store(lds + buf * 2 * BUF + BUF);
         if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+        wa_stage_wait();
     };
     if (t0 < t1) { load(t0); store(t0 & 1); }
     __syncthreads();
@@ -240,8 +287,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
         int k0, kend;
         bounds(t, k0, kend);
         k0 += ks * SUBK;
-        const char* sk = lds + (t & 1) * 2 * BUF;
-        const char* sv = sk + BUF;
+        const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), vcol = wa_opaque(col_base + sk + BUF);
         const int top = min(kend - 1, pos + a.right), low = pos - a.left;
         // nothing of this part is visible to the wave's rows / everything is
         const bool none = !live || k0 >= kend || k0 > wmax + a.right || (k0 + SUBK <= wmin - a.left && k0 >= a.sinks);
@@ -251,7 +297,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
             for (int kb = 0; kb < NB; ++kb) {
                 s[kb] = wa_zero16();
 #pragma unroll
-                for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T, DP>(sk, ks * SUBK + 32 * kb, i), qf[i], s[kb]);
+                for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s[kb]);
             }
             const bool all = !pad && k0 + SUBK <= kend && k0 + SUBK - 1 <= wmin + a.right && (k0 >= wmax - a.left || k0 + SUBK <= a.sinks);
             if (!all) {
@@ -285,7 +331,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
                 for (int i = 0; i < 2; ++i) {
                     const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i);
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sv, ks * SUBK + 32 * kb + 16 * i, dt), pf, o[dt]);
+                    for (int dt = 0; dt < DT; ++dt) o[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(vcol, dt, (32 * kb + 16 * i) * Tile::PITCH), pf, o[dt]);
                 }
             }
         }
@@ -342,7 +388,13 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
         for (int j = 0; j < 4; ++j) {
             const int d = 32 * dt + 8 * j + 4 * hl;
             const float v[4] = {o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv, o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv};
-            if (d < a.head_dim) vpf_store<T, 4>(op + d, v);
+            if (d < a.head_dim) {
+                vpf_store<T, 4>(op + d, v);
+                if (a.out_lo) {
+                    const float e[4] = {v[0] - (float)(T)v[0], v[1] - (float)(T)v[1], v[2] - (float)(T)v[2], v[3] - (float)(T)v[3]};
+                    vpf_store<T, 4>((T*)a.out_lo + ((size_t)bh * w.rows + row) * a.head_dim + d, e);
+                }
+            }
         }
     if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = l == 0.f ? INFINITY : m + log2f(l);
 }
@@ -373,19 +425,25 @@ __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
     const int bh = (int)(at / w.rows), row = (int)(at % w.rows), qi = wa_query(w, row);
     T* op = (T*)a.out + bh / a.Hk * a.o_sb + qi * a.o_sl + (bh % a.Hk * w.g + (row - qi * w.g)) * a.o_sh;
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (lane + 64 * i < a.head_dim) op[lane + 64 * i] = (T)(o[i] * inv);
+    for (int i = 0; i < N; ++i) if (lane + 64 * i < a.head_dim) {
+        const T v = (T)(o[i] * inv);
+        op[lane + 64 * i] = v;
+        if (a.out_lo) ((T*)a.out_lo)[at * a.head_dim + lane + 64 * i] = (T)(o[i] * inv - (float)v);
+    }
     if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // ------------------------------------------------------------------ backward: queries
 // dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO . O);  dQ = scale dS K.  The walk over the keys is the forward kernel's; delta is
-// kept for the kernel of the keys.  dS is rounded to the tensors' type for its product, as P is.
+// kept for the kernel of the keys.  dS is rounded to the tensors' type for its product, as P is.  delta takes O as forward had it before
+// rounding (out + out_lo): with the rounded O its error alone is as large as dS's own rounding (error of dq against 64 bits 1.6 instead of 1.4
+// times the output's rounding).
 template <typename T, int DP, int RB, int KS>
 __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int SUBK = KS == 4 ? 32 : 64, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const VpfWindowAttn& a = w.a;
     char* const pads = lds + 4 * BUF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
@@ -404,16 +462,20 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
         const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + head * a.q_sh;
         const T* gp = (const T*)a.dout + b * a.do_sb + qi * a.do_sl + head * a.do_sh;
         const T* op = (const T*)a.out + b * a.o_sb + qi * a.o_sl + head * a.o_sh;
+        const T* lp = (const T*)a.out_lo + ((size_t)bh * w.rows + rq) * a.head_dim;
 #pragma unroll
         for (int s = 0; s < KST; ++s) {
             const int d = 16 * s + 8 * hl;
-            uint4 u = make_uint4(0, 0, 0, 0), v = u, x = u;
-            if (d < a.head_dim) { u = *reinterpret_cast<const uint4*>(qp + d); v = *reinterpret_cast<const uint4*>(gp + d); x = *reinterpret_cast<const uint4*>(op + d); }
+            uint4 u = make_uint4(0, 0, 0, 0), v = u, x = u, y = u;
+            if (d < a.head_dim) {
+                u = *reinterpret_cast<const uint4*>(qp + d); v = *reinterpret_cast<const uint4*>(gp + d);
+                x = *reinterpret_cast<const uint4*>(op + d); y = *reinterpret_cast<const uint4*>(lp + d);
+            }
             qf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
             gf[s] = __builtin_bit_cast(typename WaMma<T>::v8, v);
-            const typename WaMma<T>::v8 of = __builtin_bit_cast(typename WaMma<T>::v8, x);
+            const typename WaMma<T>::v8 of = __builtin_bit_cast(typename WaMma<T>::v8, x), ol = __builtin_bit_cast(typename WaMma<T>::v8, y);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * (float)of[i];
+            for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * ((float)of[i] + (float)ol[i]);
         }
         delta = wa_half_sum(delta);
         if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
@@ -426,7 +488,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[dt] = wa_zero16();
 
-    WaStage<DP, STAGE> rk, rv;
+    const WaStage<DP, STAGE> stage(a.head_dim);
+    const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
     uint8_t rp = 0;
     auto bounds = [&](int t, int& k0, int& kend) {
         if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
@@ -435,14 +498,19 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     auto load = [&](int t) {
         int k0, kend;
         bounds(t, k0, kend);
-        rk.load(a.head_dim, [&](int r) { return k0 + r < kend && !(pad && pad[k0 + r]) ? kp + (size_t)(k0 + r) * a.k_sl * sizeof(T) : nullptr; });
-        rv.load(a.head_dim, [&](int r) { return k0 + r < kend ? vp + (size_t)(k0 + r) * a.v_sl * sizeof(T) : nullptr; });
+        const int last = min(STAGE, kend - k0) - 1;
+        const char* kb = kp + (size_t)k0 * a.k_sl * sizeof(T);
+        const char* vb = vp + (size_t)k0 * a.v_sl * sizeof(T);
+        const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
+        // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
+        if (pad) stage.rows_padded(kb, (uint32_t)(a.k_sl * sizeof(T)), last, pad + k0, at);
+        else stage.rows(kb, (uint32_t)(a.k_sl * sizeof(T)), last, at);
+        stage.rows(vb, (uint32_t)(a.v_sl * sizeof(T)), last, at + BUF);
         if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
     };
     auto store = [&](int buf) {
-        rk.store(lds + buf * 2 * BUF);
-        rv.store(lds + buf * 2 * BUF + BUF);
         if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+        wa_stage_wait();
     };
     if (span.total > 0) { load(0); store(0); }
     __syncthreads();
@@ -451,8 +519,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
         int k0, kend;
         bounds(t, k0, kend);
         k0 += ks * SUBK;
-        const char* sk = lds + (t & 1) * 2 * BUF;
-        const char* sv = sk + BUF;
+        const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), kcol = wa_opaque(col_base + sk);
         const int top = min(kend - 1, pos + a.right), low = pos - a.left;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
@@ -461,8 +528,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
-                s = WaMma<T>::mma(wa_frag_row<T, DP>(sk, ks * SUBK + 32 * kb, i), qf[i], s);
-                dp = WaMma<T>::mma(wa_frag_row<T, DP>(sv, ks * SUBK + 32 * kb, i), gf[i], dp);
+                s = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s);
+                dp = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH + BUF), gf[i], dp);
             }
             const bool all = !pad && kk + 32 <= kend && kk + 31 <= wmin + a.right && (kk >= wmax - a.left || kk + 32 <= a.sinks);
             if (!all) wa_hide(s, kk, hl, top, low, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
@@ -477,7 +544,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             for (int i = 0; i < 2; ++i) {
                 const typename WaMma<T>::v8 df = wa_pack8<T>(ds + 8 * i);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sk, ks * SUBK + 32 * kb + 16 * i, dt), df, dq[dt]);
+                for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(kcol, dt, (32 * kb + 16 * i) * Tile::PITCH), df, dq[dt]);
             }
         }
         if (t + 1 < span.total) store((t + 1) & 1);
@@ -541,7 +608,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int ROWS = 64, KST = DP / 16, DT = DP / 32, BUF = ROWS * Tile::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char lds[];               // [2][Q, dO][64 rows], [2][lse, delta, position][64]
+    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][Q, dO][64 rows], [2][lse, delta, position][64]
     const VpfWindowAttn& a = w.a;
     float* const stats = reinterpret_cast<float*>(lds + 4 * BUF);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, kb = wave & 1, qs = wave >> 1;
@@ -579,17 +646,23 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
     const int kmin = kt0 + 32 * kb, kmax = kmin + 31;
     const bool whole = !pad && kmax < seen.n;
 
-    WaStage<DP, ROWS> rq, rg;
+    const WaStage<DP, ROWS> stage(a.head_dim);
+    const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
+    const char* qp = (const char*)((const T*)a.q + b * a.q_sb + hk * w.g * a.q_sh);
+    const char* gp = (const char*)((const T*)a.dout + b * a.do_sb + hk * w.g * a.do_sh);
     float r_lse = 0.f, r_delta = 0.f;
     int r_pos = 0;
-    auto load = [&](int r0) {
-        auto src = [&](const void* base, long sb, long sl, long sh, int r) -> const char* {
-            if (r0 + r >= rr.hi) return nullptr;
-            const int qi = wa_query(w, r0 + r);
-            return (const char*)((const T*)base + b * sb + qi * sl + (hk * w.g + (r0 + r - qi * w.g)) * sh);
-        };
-        rq.load(a.head_dim, [&](int r) { return src(a.q, a.q_sb, a.q_sl, a.q_sh, r); });
-        rg.load(a.head_dim, [&](int r) { return src(a.dout, a.do_sb, a.do_sl, a.do_sh, r); });
+    auto load = [&](int r0, int buf) {
+        const int q0 = wa_query(w, r0), skip = r0 - q0 * w.g, last = min(ROWS, rr.hi - r0) - 1;
+        const char* qb = qp + (size_t)q0 * a.q_sl * sizeof(T);
+        const char* gb = gp + (size_t)q0 * a.do_sl * sizeof(T);
+        const uint32_t at = tiles_at + buf * 2 * BUF;
+#pragma unroll
+        for (int i = 0; i < stage.PER; ++i) {
+            const int r = skip + min(stage.row0 + i * stage.STEP, last), qi = wa_query(w, r), h = r - qi * w.g;
+            wa_dma(qb, (uint32_t)(qi * (int)a.q_sl + h * (int)a.q_sh) * (uint32_t)sizeof(T) + stage.col, at + stage.wave_byte + i * 4096);
+            wa_dma(gb, (uint32_t)(qi * (int)a.do_sl + h * (int)a.do_sh) * (uint32_t)sizeof(T) + stage.col, at + BUF + stage.wave_byte + i * 4096);
+        }
         if (threadIdx.x < ROWS) {
             const int r = r0 + threadIdx.x, rc = min(r, w.rows - 1);
             r_lse = r < rr.hi ? a.lse[(size_t)bh * w.rows + rc] : INFINITY;  // weight 0
@@ -598,20 +671,18 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
         }
     };
     auto store = [&](int buf) {
-        rq.store(lds + buf * 2 * BUF);
-        rg.store(lds + buf * 2 * BUF + BUF);
         if (threadIdx.x < ROWS) {
             float* s = stats + buf * 3 * ROWS + threadIdx.x;
             s[0] = r_lse; s[ROWS] = r_delta; reinterpret_cast<int*>(s)[2 * ROWS] = r_pos;
         }
+        wa_stage_wait();
     };
     const int steps = (rr.hi - rr.lo + ROWS - 1) / ROWS;
-    if (steps > 0) { load(rr.lo); store(0); }
+    if (steps > 0) { load(rr.lo, 0); store(0); }
     __syncthreads();
     for (int t = 0; t < steps; ++t) {
-        if (t + 1 < steps) load(rr.lo + (t + 1) * ROWS);
-        const char* sq = lds + (t & 1) * 2 * BUF;
-        const char* sg = sq + BUF;
+        if (t + 1 < steps) load(rr.lo + (t + 1) * ROWS, (t + 1) & 1);
+        const uint32_t sq = tiles_at + (t & 1) * 2 * BUF + 32 * qs * Tile::PITCH, qrow = wa_opaque(row_base + sq), qcol = wa_opaque(col_base + sq);
         const float* st = stats + (t & 1) * 3 * ROWS + 32 * qs + 4 * hl;
         const int* sp = reinterpret_cast<const int*>(stats + (t & 1) * 3 * ROWS + 2 * ROWS + 32 * qs);
         const int rlo = rr.lo + t * ROWS + 32 * qs;
@@ -620,8 +691,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
-                s = WaMma<T>::mma(wa_frag_row<T, DP>(sq, 32 * qs, i), kf[i], s);
-                dp = WaMma<T>::mma(wa_frag_row<T, DP>(sg, 32 * qs, i), vf[i], dp);
+                s = WaMma<T>::mma(wa_frag_row<T>(qrow, i, 0), kf[i], s);
+                dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), vf[i], dp);
             }
             const bool all = whole && kmax <= pmin + a.right && (kmin >= pmax - a.left || kmax < a.sinks);
             float p[16], ds[16];
@@ -648,8 +719,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
                 const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i), df = wa_pack8<T>(ds + 8 * i);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    dv[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sg, 32 * qs + 16 * i, dt), pf, dv[dt]);
-                    dk[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(sq, 32 * qs + 16 * i, dt), df, dk[dt]);
+                    dv[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(qcol, dt, 16 * i * Tile::PITCH + BUF), pf, dv[dt]);
+                    dk[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(qcol, dt, 16 * i * Tile::PITCH), df, dk[dt]);
                 }
             }
         }
@@ -744,7 +815,11 @@ static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
     w.c = a.scale * WA_LOG2E;
     return VPF_OK;
 }
-static bool wa_aligned(const void* p, long sb, long sl, long sh) { return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0; }
+// 16-byte rows; the offsets inside a stage (up to 128 keys, up to 64 + g rows of queries and heads) are 32-bit byte offsets
+static bool wa_aligned(const void* p, long sb, long sl, long sh)
+{
+    return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < VPF_WINDOW_MAX_STRIDE && sh >= 0 && sh < VPF_WINDOW_MAX_STRIDE;
+}
 
 // Row blocks of 32 per workgroup (4, 2 or 1; the waves that are left split a stage's keys): as many as leave a workgroup for each of the 256 CUs.
 // Then, where even single blocks are too few, parts of the keys: two workgroups per CU, each with at least two stages.
@@ -889,10 +964,10 @@ extern "C" int vpf_window_attn_bwd(const VpfWindowAttn* args, void* stream)
     if (const int rc = wa_prepare(args, w)) return rc;
     const VpfWindowAttn& a = w.a;
     if (a.B == 0 || (w.rows == 0 && a.Lkv == 0)) return VPF_OK;
-    if ((w.rows > 0 && (!a.q || !a.out || !a.dout || !a.lse || !a.dq || !a.ws)) || (a.Lkv > 0 && (!a.k || !a.v || !a.dk || !a.dv))) return VPF_ERR_NULL;
+    if ((w.rows > 0 && (!a.q || !a.out || !a.out_lo || !a.dout || !a.lse || !a.dq || !a.ws)) || (a.Lkv > 0 && (!a.k || !a.v || !a.dk || !a.dv))) return VPF_ERR_NULL;
     const struct { const void* p; long sb, sl, sh; } t[] = {{a.q, a.q_sb, a.q_sl, a.q_sh}, {a.k, a.k_sb, a.k_sl, a.k_sh}, {a.v, a.v_sb, a.v_sl, a.v_sh},
         {a.out, a.o_sb, a.o_sl, a.o_sh}, {a.dout, a.do_sb, a.do_sl, a.do_sh}, {a.dq, a.dq_sb, a.dq_sl, a.dq_sh}, {a.dk, a.dk_sb, a.dk_sl, a.dk_sh},
-        {a.dv, a.dv_sb, a.dv_sl, a.dv_sh}, {a.ws, 0, 0, 0}};
+        {a.dv, a.dv_sb, a.dv_sl, a.dv_sh}, {a.out_lo, 0, 0, 0}, {a.ws, 0, 0, 0}};
     for (const auto& x : t) if (!wa_aligned(x.p, x.sb, x.sl, x.sh)) return VPF_ERR_BADALIGN;
     wa_plan_bwd(w);
     if (a.ws_floats < wa_bwd_ws(w)) return VPF_ERR_BADSHAPE;

@@ -289,17 +289,19 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
 
 # --------------------------------------------------------------------------- attention inside a sliding window
 def _attn_ready(t: torch.Tensor) -> torch.Tensor:
-    """16-byte rows: a contiguous last dimension, strides that are multiples of 8 elements and an aligned base; everything else is copied."""
-    if t.stride(3) != 1 or any(s % 8 for s in _strides(t)) or t.data_ptr() % 16:
+    """16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8 elements, those of tokens and heads below 2^23;
+    everything else is copied."""
+    s = _strides(t)
+    if t.stride(3) != 1 or any(n % 8 for n in s) or max(s[1:]) >= 1 << 23 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _attn_struct(cfg, q, k, v, pad, lens, out, lse):
+def _attn_struct(cfg, q, k, v, pad, lens, out, lse, lo):
     left, right, sinks, scale = cfg
     B, Lq, Hq, dh = q.shape
     s = L.WindowAttn(B, Lq, k.shape[1], Hq, k.shape[2], dh, left, right, sinks, _TYPE[q.dtype], scale, 0, _ptr(q), _ptr(k), _ptr(v), _ptr(pad),
-                     _ptr(lens), _ptr(out), _ptr(lse))
+                     _ptr(lens), _ptr(out), _ptr(lse), _ptr(lo))
     for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
         _attn_strides(s, name, t)
     return s
@@ -324,29 +326,30 @@ def _attn_forward(cfg, q, k, v, pad, lens, keep):
     B, Lq, Hq, dh = q.shape
     out = torch.empty(B, Lq, Hq, dh, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, k.shape[2], Lq * Hq // k.shape[2], dtype=F32, device=q.device) if keep else None
-    s = _attn_struct(cfg, q, k, v, pad, lens, out, lse)
+    lo = torch.empty(B, Lq, Hq, dh, dtype=q.dtype, device=q.device) if keep else None
+    s = _attn_struct(cfg, q, k, v, pad, lens, out, lse, lo)
     ws = _attn_workspace(s, 0, q.device)        # noqa: F841  (alive until the launch is issued; the allocator orders its reuse by stream)
     with _on(q.device):
         L.call_struct("vpf_window_attn_fwd", s)
-    return out, lse
+    return out, lse, lo
 
 
 class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, q, k, v, pad, lens):
         q, k, v = _attn_ready(q), _attn_ready(k), _attn_ready(v)
-        out, lse = _attn_forward(cfg, q, k, v, pad, lens, True)
+        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, True)
         ctx.cfg = cfg
-        ctx.save_for_backward(q, k, v, out, lse, pad, lens)
+        ctx.save_for_backward(q, k, v, out, lse, lo, pad, lens)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, pad, lens = ctx.saved_tensors
+        q, k, v, out, lse, lo, pad, lens = ctx.saved_tensors
         dout = _attn_ready(dout)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        s = _attn_struct(ctx.cfg, q, k, v, pad, lens, out, lse)
+        s = _attn_struct(ctx.cfg, q, k, v, pad, lens, out, lse, lo)
         s.dout, s.dq, s.dk, s.dv = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv)
         for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
             _attn_strides(s, name, t)
