@@ -39,7 +39,7 @@ struct WaArgs {
     VpfWindowAttn a;
     int g, rows;                // query heads per key head; rows of one (sample, key head)
     uint32_t magic;             // r / g == umulhi(r, magic) for r < 2^32 / g (g > 1)
-    int tiles, splits;          // row tiles; parts of a row tile's keys
+    int tiles, splits, runs;    // row tiles; parts of a row tile's keys; order of the workgroups (wa_item)
     float c;                    // scale * log2(e)
     int ktiles, sink_tiles, chunks, chunk_rows;      // backward: key tiles, those with sinks, pieces of the rows far behind those and their size
 };
@@ -127,25 +127,34 @@ __device__ __forceinline__ WaSeen wa_seen(const WaArgs& w, int b)
     s.off = s.n - w.a.Lq;
     return s;
 }
-// The keys a block of rows at positions pmin .. pmax can see: the first `first` ones, then lo .. hi; walked in stages of `stage` keys
-struct WaSpan { int first, lo, hi, nfirst, total; };
-__device__ __forceinline__ WaSpan wa_span(const WaArgs& w, const WaSeen& s, int pmin, int pmax, int stage)
+// The keys a block of rows at positions pmin .. pmax can see, as one list: the `first` first ones, then lo .. hi.  Entry x is key x, or
+// x + shift from `first` on; a stage is a run of entries, so the first tokens share a stage with the window instead of having their own.
+struct WaSpan { int first, shift, total; };
+__device__ __forceinline__ WaSpan wa_span(const WaArgs& w, const WaSeen& s, int pmin, int pmax)
 {
     WaSpan k;
-    k.hi = max(0, min(pmax + w.a.right + 1, s.n));
-    k.lo = min(max(0, pmin - w.a.left), k.hi);
-    k.first = min(w.a.sinks, k.lo);
-    k.nfirst = (k.first + stage - 1) / stage;
-    k.total = k.nfirst + (k.hi - k.lo + stage - 1) / stage;
+    const int hi = max(0, min(pmax + w.a.right + 1, s.n)), lo = min(max(0, pmin - w.a.left), hi);
+    k.first = min(w.a.sinks, lo);
+    k.shift = lo - k.first;
+    k.total = hi - k.shift;
     return k;
 }
 
-// Consecutive workgroups go to different XCDs (8, each with an L2 of its own): give each XCD a run of consecutive items, whose rows share
-// their keys.
-__device__ __forceinline__ int wa_item(int id, int total)
+// Order of the workgroups; consecutive ones go round the 8 XCDs, each with an L2 of its own.  The (sample, key head) pairs run fastest, so each
+// XCD keeps few of them, and within a pair the longest walks start first.  With fewer than 8 pairs XCDs share one, and where all walks are
+// about as long (w.runs) each then takes a run of consecutive tiles, whose rows share their keys.  Measured, runs against pairs first: 4 pairs of
+// 256 tiles dQ 237 / 283 us, 1024 tiles forward 1362 / 1387 us; 96 pairs of 9 tiles forward 41.6 / 33.5 us, dQ 46 / 38 us.
+__device__ __forceinline__ void wa_item(const WaArgs& w, int& bh, int& tile, int& split)
 {
-    const int per = total / 8, cut = per * 8;
-    return id < cut ? (id & 7) * per + (id >> 3) : id;
+    const int pairs = w.a.B * w.a.Hk;
+    int id = blockIdx.x;
+    if (w.runs) {
+        const int per = gridDim.x / 8, cut = per * 8;
+        if (id < cut) id = (id & 7) * per + (id >> 3);
+        bh = id / w.tiles; tile = id % w.tiles; split = 0;
+        return;
+    }
+    bh = id % pairs; split = id / pairs % w.splits; tile = w.tiles - 1 - id / pairs / w.splits;
 }
 
 // Stages travel memory -> LDS without registers (global_load_lds, 16 bytes a lane): a wave instruction fills 1 KB of the tile, lane i its 16
@@ -187,25 +196,43 @@ template <int DP, int ROWS> struct WaStage {
 #pragma unroll
         for (int i = 0; i < PER; ++i) wa_dma(base, (uint32_t)min(row0 + i * STEP, last) * stride + col, tile + wave_byte + i * 4096);
     }
-    // the same, with zeros where pad[row] is set
-    __device__ __forceinline__ void rows_padded(const char* base, uint32_t stride, int last, const uint8_t* pad, uint32_t tile) const
+    // rows key(0) .. key(last) of it, with zeros where pad[key] is set (pad may be null)
+    template <typename F> __device__ __forceinline__ void rows_of(const char* base, long stride, int last, F key, const uint8_t* pad, uint32_t tile) const
     {
+        const char* p[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int r = min(row0 + i * STEP, last);
-            const char* p = pad[r] ? (const char*)wa_zeros : base + (size_t)r * stride + col;
-            wa_dma_any(p, tile + wave_byte + i * 4096);
+        for (int i = 0; i < PER; ++i) {                         // all padding bytes are on their way before the first is looked at
+            const int k = key(min(row0 + i * STEP, last));
+            p[i] = base + k * stride + col;
+            if (pad) p[i] = pad[k] ? (const char*)wa_zeros : p[i];
         }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) wa_dma_any(p[i], tile + wave_byte + i * 4096);
     }
 };
 
-// Scores of one 32-key block (accumulator order: key kk + (r & 3) + 8 (r >> 2) + 4 hl) that the lane's row does not see -> -inf
-__device__ __forceinline__ void wa_hide(wa_f32x16& s, int kk, int hl, int top, int low, int sinks, const uint32_t* padw)
+// Does a wave with rows at positions wmin .. wmax see nothing / all of the n list entries from x on?  (A block across the list's seam: neither.)
+__device__ __forceinline__ bool wa_none(const WaArgs& w, const WaSpan& s, int x, int n, int wmin, int wmax)
+{
+    if (x >= s.total) return true;
+    if (x < s.first && x + n > s.first) return false;
+    const int k = x < s.first ? x : x + s.shift;
+    return k > wmax + w.a.right || (k + n <= wmin - w.a.left && k >= w.a.sinks);
+}
+__device__ __forceinline__ bool wa_all(const WaArgs& w, const WaSpan& s, int x, int n, int wmin, int wmax)
+{
+    if (x + n > s.total || (x < s.first && x + n > s.first)) return false;
+    const int k = x < s.first ? x : x + s.shift;
+    return k + n - 1 <= wmin + w.a.right && (k >= wmax - w.a.left || k + n <= w.a.sinks);
+}
+
+// Scores of one block of 32 list entries (accumulator order: entry x + (r & 3) + 8 (r >> 2) + 4 hl) that the lane's row does not see -> -inf
+__device__ __forceinline__ void wa_hide(wa_f32x16& s, const WaSpan& span, int x, int hl, int top, int low, int sinks, const uint32_t* padw)
 {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int j = kk + (r & 3) + 8 * (r >> 2) + 4 * hl;
-        bool see = j <= top && (j >= low || j < sinks);
+        const int e = x + (r & 3) + 8 * (r >> 2) + 4 * hl, j = e < span.first ? e : e + span.shift;
+        bool see = e < span.total && j <= top && (j >= low || j < sinks);
         if (padw) see = see && !((padw[2 * (r >> 2) + hl] >> (8 * (r & 3))) & 0xffu);
         s[r] = see ? s[r] : -INFINITY;
     }
@@ -224,12 +251,13 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     const VpfWindowAttn& a = w.a;
     char* const pads = lds + 4 * BUF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
-    const int item = wa_item(blockIdx.x, gridDim.x);
-    const int split = item % w.splits, tile = item / w.splits % w.tiles, bh = item / w.splits / w.tiles, b = bh / a.Hk, hk = bh % a.Hk;
+    int bh, tile, split;
+    wa_item(w, bh, tile, split);
+    const int b = bh / a.Hk, hk = bh % a.Hk;
     const WaSeen seen = wa_seen(w, b);
     const int r0 = tile * 32 * RB, rend = min(r0 + 32 * RB, w.rows);
-    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1), STAGE);
-    const int t0 = (int)((long)span.total * split / w.splits), t1 = (int)((long)span.total * (split + 1) / w.splits);
+    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1));
+    const int stages = (span.total + STAGE - 1) / STAGE, t0 = (int)((long)stages * split / w.splits), t1 = (int)((long)stages * (split + 1) / w.splits);
 
     // this lane's row
     const int row = r0 + rb * 32 + (lane & 31), rq = min(row, w.rows - 1), qi = wa_query(w, rq);
@@ -259,22 +287,20 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
     uint8_t rp = 0;
-    auto bounds = [&](int t, int& k0, int& kend) {
-        if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
-        else { k0 = span.lo + (t - span.nfirst) * STAGE; kend = span.hi; }
-    };
     auto load = [&](int t) {
-        int k0, kend;
-        bounds(t, k0, kend);
-        const int last = min(STAGE, kend - k0) - 1;
-        const char* kb = kp + (size_t)k0 * a.k_sl * sizeof(T);
-        const char* vb = vp + (size_t)k0 * a.v_sl * sizeof(T);
+        const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
-        // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
-        if (pad) stage.rows_padded(vb, (uint32_t)(a.v_sl * sizeof(T)), last, pad + k0, at + BUF);
-        else stage.rows(vb, (uint32_t)(a.v_sl * sizeof(T)), last, at + BUF);
-        stage.rows(kb, (uint32_t)(a.k_sl * sizeof(T)), last, at);
-        if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
+        const long kst = a.k_sl * (long)sizeof(T), vst = a.v_sl * (long)sizeof(T);
+        if (pad || x0 < span.first) {
+            auto key = [&](int r) { return (long)(x0 + r < span.first ? x0 + r : x0 + r + span.shift); };
+            // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
+            stage.rows_of(kp, kst, last, key, nullptr, at);
+            stage.rows_of(vp, vst, last, key, pad, at + BUF);
+            if (pad && threadIdx.x < STAGE) rp = (int)threadIdx.x <= last ? pad[key(threadIdx.x)] : 1;
+        } else {
+            stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
+            stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
+        }
     };
     auto store = [&](int buf) {
         if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
@@ -284,14 +310,9 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         if (t + 1 < t1) load(t + 1);
-        int k0, kend;
-        bounds(t, k0, kend);
-        k0 += ks * SUBK;
+        const int x0 = t * STAGE + ks * SUBK;
         const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), vcol = wa_opaque(col_base + sk + BUF);
-        const int top = min(kend - 1, pos + a.right), low = pos - a.left;
-        // nothing of this part is visible to the wave's rows / everything is
-        const bool none = !live || k0 >= kend || k0 > wmax + a.right || (k0 + SUBK <= wmin - a.left && k0 >= a.sinks);
-        if (!none) {
+        if (live && !wa_none(w, span, x0, SUBK, wmin, wmax)) {
             wa_f32x16 s[NB];
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb) {
@@ -299,11 +320,10 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 #pragma unroll
                 for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s[kb]);
             }
-            const bool all = !pad && k0 + SUBK <= kend && k0 + SUBK - 1 <= wmin + a.right && (k0 >= wmax - a.left || k0 + SUBK <= a.sinks);
-            if (!all) {
+            if (pad || !wa_all(w, span, x0, SUBK, wmin, wmax)) {
 #pragma unroll
                 for (int kb = 0; kb < NB; ++kb)
-                    wa_hide(s[kb], k0 + 32 * kb, hl, top, low, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+                    wa_hide(s[kb], span, x0 + 32 * kb, hl, pos + a.right, pos - a.left, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
             }
             float mx = s[0][0];
 #pragma unroll
@@ -399,7 +419,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
-// parts of the keys -> output: one wave per row, the lanes hold DP / 64 channels each
+// parts of the keys -> output: one wave per row.  Lane i holds maximum and sum of part i (splits <= 64); the channels' loads of 4 parts are in
+// flight together.
 template <typename T, int DP>
 __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
 {
@@ -408,18 +429,17 @@ __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
     const int lane = threadIdx.x & 63;
     if (at >= all) return;
     const float2* ml = reinterpret_cast<const float2*>(a.ws + (size_t)w.splits * all * DP);
-    float m = -INFINITY;
-    for (int s = 0; s < w.splits; ++s) m = fmaxf(m, ml[s * all + at].x);
+    const float2 mine = lane < w.splits ? ml[lane * all + at] : make_float2(-INFINITY, 0.f);
+    const float m = wave_max(mine.x), f = mine.x == -INFINITY ? 0.f : wa_exp2(mine.x - m), l = wave_sum(mine.y * f);
     constexpr int N = (DP + 63) / 64;
-    float l = 0.f, o[N];
+    float o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = 0.f;
+#pragma unroll 4
     for (int s = 0; s < w.splits; ++s) {
-        const float2 p = ml[s * all + at];
-        const float f = p.x == -INFINITY ? 0.f : wa_exp2(p.x - m);
-        l += p.y * f;
+        const float fs = __shfl(f, s);
 #pragma unroll
-        for (int i = 0; i < N; ++i) if (lane + 64 * i < DP) o[i] += a.ws[(s * all + at) * DP + lane + 64 * i] * f;
+        for (int i = 0; i < N; ++i) if (lane + 64 * i < DP) o[i] += a.ws[(s * all + at) * DP + lane + 64 * i] * fs;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int bh = (int)(at / w.rows), row = (int)(at % w.rows), qi = wa_query(w, row);
@@ -442,16 +462,18 @@ template <typename T, int DP, int RB, int KS>
 __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
-    constexpr int SUBK = KS == 4 ? 32 : 64, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
+    constexpr int SUBK = KS == 1 ? 64 : 32, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const VpfWindowAttn& a = w.a;
     char* const pads = lds + 4 * BUF;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
-    const int item = wa_item(blockIdx.x, gridDim.x);
-    const int tile = item % w.tiles, bh = item / w.tiles, b = bh / a.Hk, hk = bh % a.Hk;
+    int bh, tile, split;
+    wa_item(w, bh, tile, split);
+    const int b = bh / a.Hk, hk = bh % a.Hk;
     const WaSeen seen = wa_seen(w, b);
     const int r0 = tile * 32 * RB, rend = min(r0 + 32 * RB, w.rows);
-    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1), STAGE);
+    const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1));
+    const int stages = (span.total + STAGE - 1) / STAGE;
     const int row = r0 + rb * 32 + (lane & 31), rq = min(row, w.rows - 1), qi = wa_query(w, rq), head = hk * w.g + (rq - qi * w.g);
     const int pos = seen.off + qi, wlast = min(r0 + rb * 32 + 31, w.rows - 1);
     const bool live = r0 + rb * 32 < w.rows;
@@ -491,48 +513,43 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
     uint8_t rp = 0;
-    auto bounds = [&](int t, int& k0, int& kend) {
-        if (t < span.nfirst) { k0 = t * STAGE; kend = span.first; }
-        else { k0 = span.lo + (t - span.nfirst) * STAGE; kend = span.hi; }
-    };
     auto load = [&](int t) {
-        int k0, kend;
-        bounds(t, k0, kend);
-        const int last = min(STAGE, kend - k0) - 1;
-        const char* kb = kp + (size_t)k0 * a.k_sl * sizeof(T);
-        const char* vb = vp + (size_t)k0 * a.v_sl * sizeof(T);
+        const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
-        // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
-        if (pad) stage.rows_padded(kb, (uint32_t)(a.k_sl * sizeof(T)), last, pad + k0, at);
-        else stage.rows(kb, (uint32_t)(a.k_sl * sizeof(T)), last, at);
-        stage.rows(vb, (uint32_t)(a.v_sl * sizeof(T)), last, at + BUF);
-        if (pad && threadIdx.x < STAGE) rp = k0 + (int)threadIdx.x < kend ? pad[k0 + threadIdx.x] : 1;
+        const long kst = a.k_sl * (long)sizeof(T), vst = a.v_sl * (long)sizeof(T);
+        if (pad || x0 < span.first) {
+            auto key = [&](int r) { return (long)(x0 + r < span.first ? x0 + r : x0 + r + span.shift); };
+            // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
+            stage.rows_of(kp, kst, last, key, pad, at);
+            stage.rows_of(vp, vst, last, key, nullptr, at + BUF);
+            if (pad && threadIdx.x < STAGE) rp = (int)threadIdx.x <= last ? pad[key(threadIdx.x)] : 1;
+        } else {
+            stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
+            stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
+        }
     };
     auto store = [&](int buf) {
         if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
         wa_stage_wait();
     };
-    if (span.total > 0) { load(0); store(0); }
+    if (stages > 0) { load(0); store(0); }
     __syncthreads();
-    for (int t = 0; t < span.total; ++t) {
-        if (t + 1 < span.total) load(t + 1);
-        int k0, kend;
-        bounds(t, k0, kend);
-        k0 += ks * SUBK;
+    for (int t = 0; t < stages; ++t) {
+        if (t + 1 < stages) load(t + 1);
+        const int x0 = t * STAGE + ks * SUBK;
         const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), kcol = wa_opaque(col_base + sk);
-        const int top = min(kend - 1, pos + a.right), low = pos - a.left;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
-            const int kk = k0 + 32 * kb;
-            if (!live || kk >= kend || kk > wmax + a.right || (kk + 32 <= wmin - a.left && kk >= a.sinks)) continue;
+            const int xb = x0 + 32 * kb;
+            if (!live || wa_none(w, span, xb, 32, wmin, wmax)) continue;
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
                 s = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s);
                 dp = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH + BUF), gf[i], dp);
             }
-            const bool all = !pad && kk + 32 <= kend && kk + 31 <= wmin + a.right && (kk >= wmax - a.left || kk + 32 <= a.sinks);
-            if (!all) wa_hide(s, kk, hl, top, low, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+            const bool all = !pad && wa_all(w, span, xb, 32, wmin, wmax);
+            if (!all) wa_hide(s, span, xb, hl, pos + a.right, pos - a.left, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -547,7 +564,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
                 for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(kcol, dt, (32 * kb + 16 * i) * Tile::PITCH), df, dq[dt]);
             }
         }
-        if (t + 1 < span.total) store((t + 1) & 1);
+        if (t + 1 < stages) store((t + 1) & 1);
         __syncthreads();
     }
     if (KS > 1) {
@@ -612,10 +629,9 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
     const VpfWindowAttn& a = w.a;
     float* const stats = reinterpret_cast<float*>(lds + 4 * BUF);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, kb = wave & 1, qs = wave >> 1;
-    const int item = wa_item(blockIdx.x, gridDim.x), items = w.ktiles + w.sink_tiles * w.chunks;
-    const int bh = item / items, it = item % items, b = bh / a.Hk, hk = bh % a.Hk;
-    const bool far = it >= w.ktiles;
-    const int kt = far ? (it - w.ktiles) / w.chunks : it, chunk = far ? (it - w.ktiles) % w.chunks : 0, kt0 = kt * WA_KT;
+    const int pairs = a.B * a.Hk, bh = blockIdx.x % pairs, it = blockIdx.x / pairs, b = bh / a.Hk, hk = bh % a.Hk, pieces = w.sink_tiles * w.chunks;
+    const bool far = it < pieces;
+    const int kt = far ? it / w.chunks : it - pieces, chunk = far ? it % w.chunks : 0, kt0 = kt * WA_KT;
     const WaSeen seen = wa_seen(w, b);
     WaRowRange rr = wa_rows_of(w, seen, kt0);
     if (kt0 >= seen.n) rr.hi = rr.lo;                                        // keys behind the ones in use
@@ -822,20 +838,28 @@ static bool wa_aligned(const void* p, long sb, long sl, long sh)
 }
 
 // Row blocks of 32 per workgroup (4, 2 or 1; the waves that are left split a stage's keys): as many as leave a workgroup for each of the 256 CUs.
-// Then, where even single blocks are too few, parts of the keys: two workgroups per CU, each with at least two stages.
+static int wa_row_blocks(const WaArgs& w)
+{
+    const long pairs = (long)w.a.B * w.a.Hk;
+    return pairs * vpf_cdiv(w.rows, 128) >= 256 ? 4 : pairs * vpf_cdiv(w.rows, 64) >= 256 ? 2 : 1;
+}
+// Walks of one length: the window leaves most of the keys out, so few tiles are cut short by the ends of the sequence.
+static int wa_runs(const WaArgs& w) { return (long)w.a.B * w.a.Hk < 8 && ((long)w.a.left + w.a.right) * 2 < w.a.Lkv; }
+// Where even single row blocks are too few, the keys are divided as well: one workgroup per CU (a stage of 128 keys is up to 64 KB of loads in flight),
+// each with at least two stages, and at most 64 parts (a wave of the join).
 static void wa_plan_fwd(WaArgs& w, int& rb)
 {
-    const long bh = (long)w.a.B * w.a.Hk;
-    rb = bh * vpf_cdiv(w.rows, 128) >= 256 ? 4 : bh * vpf_cdiv(w.rows, 64) >= 256 ? 2 : 1;
+    rb = wa_row_blocks(w);
     w.tiles = vpf_cdiv(w.rows, 32 * rb);
     w.splits = 1;
-    const long wgs = bh * w.tiles;
-    if (rb == 1 && wgs < 256) {
+    const long wgs = (long)w.a.B * w.a.Hk * w.tiles;
+    if (rb == 1 && wgs <= 128) {
         const long span = (long)w.a.left + w.a.right + 1 + 31 / w.g + w.a.sinks, keys = span < w.a.Lkv ? span : w.a.Lkv;
-        const long stages = (keys + 127) / 128, want = (512 + wgs - 1) / wgs;
-        w.splits = (int)(want < stages / 2 ? want : stages / 2);
+        const long stages = (keys + 127) / 128, want = 256 / wgs, most = stages / 2 < 64 ? stages / 2 : 64;
+        w.splits = (int)(want < most ? want : most);
         if (w.splits < 1) w.splits = 1;
     }
+    w.runs = w.splits == 1 && wa_runs(w);
 }
 static long wa_fwd_ws(const WaArgs& w) { return w.splits > 1 ? (long)w.splits * w.a.B * w.a.Hk * w.rows * (wa_dp(w.a.head_dim) + 2) : 0; }
 
@@ -884,13 +908,13 @@ template <typename T, int DP, int RB, int KS, int SUBK> static int wa_launch_fwd
 template <typename T, int DP> static int wa_fwd(const WaArgs& w, int rb, hipStream_t st)
 {
     if (rb == 4) return wa_launch_fwd<T, DP, 4, 1, 64>(w, st);
-    if (rb == 2) return wa_launch_fwd<T, DP, 2, 2, 64>(w, st);
+    if (rb == 2) return wa_launch_fwd<T, DP, 2, 2, 32>(w, st);
     return wa_launch_fwd<T, DP, 1, 4, 32>(w, st);
 }
 
 template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaArgs& w, hipStream_t st)
 {
-    constexpr int STAGE = (KS == 4 ? 32 : 64) * KS;
+    constexpr int STAGE = (KS == 1 ? 64 : 32) * KS;
     constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + 2 * STAGE;
     static VpfPerDevice done;
     if (const int rc = wa_lds(wa_dq_kernel<T, DP, RB, KS>, lds, done)) return rc;
@@ -902,8 +926,10 @@ template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
 {
     const long bh = (long)w.a.B * w.a.Hk;
     if (w.rows > 0) {
-        const int rb = bh * vpf_cdiv(w.rows, 128) >= 256 ? 4 : bh * vpf_cdiv(w.rows, 64) >= 256 ? 2 : 1;
+        const int rb = wa_row_blocks(w);
         w.tiles = vpf_cdiv(w.rows, 32 * rb);
+        w.splits = 1;
+        w.runs = wa_runs(w);
         const int rc = rb == 4 ? wa_launch_dq<T, DP, 4, 1>(w, st) : rb == 2 ? wa_launch_dq<T, DP, 2, 2>(w, st) : wa_launch_dq<T, DP, 1, 4>(w, st);
         if (rc) return rc;
     }
