@@ -41,8 +41,11 @@ struct WaArgs {
     uint32_t magic;             // r / g == umulhi(r, magic) for r < 2^32 / g (g > 1)
     int tiles, splits, runs;    // row tiles; parts of a row tile's keys; order of the workgroups (wa_item)
     float c;                    // scale * log2(e)
-    int ktiles, sink_tiles, chunks, chunk_rows;      // backward: key tiles, those with sinks, pieces of the rows far behind those and their size
+    int key_tile, ktiles, sink_tiles, chunks, chunk_rows;      // backward: keys of a tile, tiles, those with sinks, pieces of the rows far behind those and their size
+    int cycle;                  // row blocks between two common starting points of the key tiles' walks
 };
+// backward scratch: delta of every row (whole 16-byte pieces), then the pieces
+__host__ __device__ static inline size_t wa_delta_floats(const WaArgs& w) { return ((size_t)w.a.B * w.a.Hk * w.rows + 3) / 4 * 4; }
 
 __device__ __forceinline__ int wa_query(const WaArgs& w, int r) { return w.g == 1 ? r : (int)__umulhi((uint32_t)r, w.magic); }
 __device__ __forceinline__ float wa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -170,15 +173,19 @@ __device__ __forceinline__ void wa_dma(const void* base, uint32_t off, uint32_t 
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds_byte), "v"(off), "s"(base) : "memory", "m0");
 }
+__device__ __forceinline__ void wa_dma4(const void* base, uint32_t off, uint32_t lds_byte)      // 4 bytes a lane
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(lds_byte), "v"(off), "s"(base) : "memory", "m0");
+}
 __device__ __forceinline__ void wa_dma_any(const void* p, uint32_t lds_byte)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds_byte), "v"(p) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void wa_stage_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <int DP, int ROWS> struct WaStage {
-    static constexpr int PITCH = WaTile<DP>::PITCH, PER = ROWS * PITCH / 4096, STEP = 4096 / PITCH;      // wave instructions of one tile per wave
-    static_assert(ROWS * PITCH % 4096 == 0, "a stage is whole instructions of all four waves");
+template <int DP, int ROWS, int NW = 4> struct WaStage {
+    static constexpr int PITCH = WaTile<DP>::PITCH, ALL = NW * 1024, PER = ROWS * PITCH / ALL, STEP = ALL / PITCH;      // wave instructions of one tile per wave
+    static_assert(ROWS * PITCH % ALL == 0 && STEP % 16 == 0, "a stage is whole instructions of all waves, whole periods of the swizzle apart");
     int row0;                   // this lane's row in the wave's first instruction
     uint32_t col;               // its chunk, in bytes
     uint32_t wave_byte;
@@ -194,7 +201,7 @@ template <int DP, int ROWS> struct WaStage {
     __device__ __forceinline__ void rows(const char* base, uint32_t stride, int last, uint32_t tile) const
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) wa_dma(base, (uint32_t)min(row0 + i * STEP, last) * stride + col, tile + wave_byte + i * 4096);
+        for (int i = 0; i < PER; ++i) wa_dma(base, (uint32_t)min(row0 + i * STEP, last) * stride + col, tile + wave_byte + i * ALL);
     }
     // rows key(0) .. key(last) of it, with zeros where pad[key] is set (pad may be null)
     template <typename F> __device__ __forceinline__ void rows_of(const char* base, long stride, int last, F key, const uint8_t* pad, uint32_t tile) const
@@ -207,7 +214,7 @@ template <int DP, int ROWS> struct WaStage {
             if (pad) p[i] = pad[k] ? (const char*)wa_zeros : p[i];
         }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) wa_dma_any(p[i], tile + wave_byte + i * 4096);
+        for (int i = 0; i < PER; ++i) wa_dma_any(p[i], tile + wave_byte + i * ALL);
     }
 };
 
@@ -226,16 +233,24 @@ __device__ __forceinline__ bool wa_all(const WaArgs& w, const WaSpan& s, int x, 
     return k + n - 1 <= wmin + w.a.right && (k >= wmax - w.a.left || k + n <= w.a.sinks);
 }
 
-// Scores of one block of 32 list entries (accumulator order: entry x + (r & 3) + 8 (r >> 2) + 4 hl) that the lane's row does not see -> -inf
-__device__ __forceinline__ void wa_hide(wa_f32x16& s, const WaSpan& span, int x, int hl, int top, int low, int sinks, const uint32_t* padw)
+// Which of the 32 list entries from x on the lane's row sees, as bits: key in low .. top, or a first token up to top
+__device__ __forceinline__ uint32_t wa_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }      // the n lowest bits
+__device__ __forceinline__ uint32_t wa_window(int k, int top, int low, int sinks) { return wa_below(top + 1 - k) & (~wa_below(low - k) | wa_below(sinks - k)); }
+__device__ __forceinline__ uint32_t wa_visible(const WaSpan& s, int x, int top, int low, int sinks)
 {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int e = x + (r & 3) + 8 * (r >> 2) + 4 * hl, j = e < span.first ? e : e + span.shift;
-        bool see = e < span.total && j <= top && (j >= low || j < sinks);
-        if (padw) see = see && !((padw[2 * (r >> 2) + hl] >> (8 * (r & 3))) & 0xffu);
-        s[r] = see ? s[r] : -INFINITY;
+    uint32_t m = wa_window(x + s.shift, top, low, sinks);
+    if (x < s.first) {                                           // (uniform) in front of the list's seam: entry = key
+        const uint32_t f = wa_below(s.first - x);
+        m = (m & ~f) | (wa_window(x, top, low, sinks) & f);
     }
+    return m & wa_below(s.total - x);
+}
+// hidden scores -> -inf (accumulator order: entry (r & 3) + 8 (r >> 2) + 4 hl)
+__device__ __forceinline__ void wa_hide(wa_f32x16& s, uint32_t visible, int hl)
+{
+    visible >>= 4 * hl;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = visible & (1u << ((r & 3) + 8 * (r >> 2))) ? s[r] : -INFINITY;
 }
 
 // ------------------------------------------------------------------ forward
@@ -247,10 +262,10 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][K, V][STAGE rows], [2][STAGE] padding bytes
+    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][K, V][STAGE rows], pads
     const VpfWindowAttn& a = w.a;
-    char* const pads = lds + 4 * BUF;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
+    uint32_t* const pads = reinterpret_cast<uint32_t*>(lds + 4 * BUF);     // [2][STAGE / 32]: a bit for every key that is not padding
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), hl = lane >> 5, rb = wave % RB, ks = wave / RB;
     int bh, tile, split;
     wa_item(w, bh, tile, split);
     const int b = bh / a.Hk, hk = bh % a.Hk;
@@ -286,7 +301,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
-    uint8_t rp = 0;
+    bool kept = false;
     auto load = [&](int t) {
         const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
@@ -296,14 +311,17 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
             // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
             stage.rows_of(kp, kst, last, key, nullptr, at);
             stage.rows_of(vp, vst, last, key, pad, at + BUF);
-            if (pad && threadIdx.x < STAGE) rp = (int)threadIdx.x <= last ? pad[key(threadIdx.x)] : 1;
+            if (pad) kept = (int)threadIdx.x <= last && !pad[key(threadIdx.x)];
         } else {
             stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
             stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
         }
     };
     auto store = [&](int buf) {
-        if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+        if (pad) {
+            const uint64_t bits = __ballot(kept);                            // threads 64 i .. hold entries 64 i .. of the stage
+            if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[buf * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(bits >> (32 * lane));
+        }
         wa_stage_wait();
     };
     if (t0 < t1) { load(t0); store(t0 & 1); }
@@ -322,8 +340,11 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
             }
             if (pad || !wa_all(w, span, x0, SUBK, wmin, wmax)) {
 #pragma unroll
-                for (int kb = 0; kb < NB; ++kb)
-                    wa_hide(s[kb], span, x0 + 32 * kb, hl, pos + a.right, pos - a.left, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+                for (int kb = 0; kb < NB; ++kb) {
+                    uint32_t see = wa_visible(span, x0 + 32 * kb, pos + a.right, pos - a.left, a.sinks);
+                    if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + kb];
+                    wa_hide(s[kb], see, hl);
+                }
             }
             float mx = s[0][0];
 #pragma unroll
@@ -465,8 +486,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     constexpr int SUBK = KS == 1 ? 64 : 32, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const VpfWindowAttn& a = w.a;
-    char* const pads = lds + 4 * BUF;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, rb = wave % RB, ks = wave / RB;
+    uint32_t* const pads = reinterpret_cast<uint32_t*>(lds + 4 * BUF);     // [2][STAGE / 32]: a bit for every key that is not padding
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), hl = lane >> 5, rb = wave % RB, ks = wave / RB;
     int bh, tile, split;
     wa_item(w, bh, tile, split);
     const int b = bh / a.Hk, hk = bh % a.Hk;
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
-    uint8_t rp = 0;
+    bool kept = false;
     auto load = [&](int t) {
         const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
@@ -522,14 +543,17 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
             stage.rows_of(kp, kst, last, key, pad, at);
             stage.rows_of(vp, vst, last, key, nullptr, at + BUF);
-            if (pad && threadIdx.x < STAGE) rp = (int)threadIdx.x <= last ? pad[key(threadIdx.x)] : 1;
+            if (pad) kept = (int)threadIdx.x <= last && !pad[key(threadIdx.x)];
         } else {
             stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
             stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
         }
     };
     auto store = [&](int buf) {
-        if (pad && threadIdx.x < STAGE) pads[buf * STAGE + threadIdx.x] = rp;
+        if (pad) {
+            const uint64_t bits = __ballot(kept);                            // threads 64 i .. hold entries 64 i .. of the stage
+            if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[buf * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(bits >> (32 * lane));
+        }
         wa_stage_wait();
     };
     if (stages > 0) { load(0); store(0); }
@@ -549,7 +573,11 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
                 dp = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH + BUF), gf[i], dp);
             }
             const bool all = !pad && wa_all(w, span, xb, 32, wmin, wmax);
-            if (!all) wa_hide(s, span, xb, hl, pos + a.right, pos - a.left, a.sinks, pad ? (const uint32_t*)(pads + (t & 1) * STAGE + ks * SUBK + 32 * kb) : nullptr);
+            if (!all) {
+                uint32_t see = wa_visible(span, xb, pos + a.right, pos - a.left, a.sinks);
+                if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + kb];
+                wa_hide(s, see, hl);
+            }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -605,33 +633,39 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 
 // ------------------------------------------------------------------ backward: keys
 // dV = P^T dO, dK = scale dS^T Q, summed over the rows (queries and heads) that see the key, in one fixed order.
-// Workgroup = 64 keys: 2 blocks of 32 keys x 2 halves of a 64-row stage of Q and dO (double-buffered in LDS); K and V of the wave's keys stay in
-// registers as operands (key on the lane).  The first tokens are seen by every row behind them: the rows beyond their window are cut into
-// pieces of chunk_rows, one workgroup each, and wa_sink_join_kernel adds the pieces.
-#define WA_KT 64
+// Workgroup = KB blocks of 32 keys x 2 halves of a 64-row stage of Q and dO (double-buffered in LDS); K of the wave's keys stays in registers as
+// operand (key on the lane), V as well up to head dimension 96 -- at 128 the two accumulators, K and the scores leave no room for it and V is
+// read from LDS (a spill would be worse than slow: its reload waits behind the DMA of the next stage).
+// The row blocks are walked downwards from a block that is the same for all key tiles (w.cycle), wrapping round: tiles that run at the same
+// time then read the same rows of Q and dO at the same time.  Each starting at its own first row, the tiles of a long causal window had
+// their rows spread over the whole sequence and every stage came from beyond the L2.
+// The first tokens are seen by every row behind them: the rows beyond their window are cut into pieces of chunk_rows, one workgroup each, and
+// wa_sink_join_kernel adds the pieces.
+#define WA_ROWS 64
 struct WaRowRange { int lo, hi; };
 __device__ __forceinline__ WaRowRange wa_rows_of(const WaArgs& w, const WaSeen& s, int k0)
 {
-    // positions k0 - right .. k0 + 63 + left; queries 0 .. Lq - 1 stand at off ..
-    const long lo = max((long)k0 - w.a.right - s.off, 0L), hi = min((long)k0 + WA_KT - 1 + w.a.left - s.off + 1, (long)w.a.Lq);
+    // positions k0 - right .. k0 + key_tile - 1 + left; queries 0 .. Lq - 1 stand at off ..
+    const long lo = max((long)k0 - w.a.right - s.off, 0L), hi = min((long)k0 + w.key_tile + w.a.left - s.off, (long)w.a.Lq);
     WaRowRange r;
     r.lo = (int)min(lo, (long)w.a.Lq) * w.g;
     r.hi = max((int)max(hi, 0L) * w.g, r.lo);
     return r;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
+template <typename T, int DP, int KB>
+__global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
-    constexpr int ROWS = 64, KST = DP / 16, DT = DP / 32, BUF = ROWS * Tile::PITCH;
-    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][Q, dO][64 rows], [2][lse, delta, position][64]
+    constexpr int ROWS = WA_ROWS, KST = DP / 16, DT = DP / 32, BUF = ROWS * Tile::PITCH, KT = KB * 32;
+    constexpr bool VREG = DP <= 96;
+    extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][Q, dO][64 rows], V [KT] (!VREG), [2][lse, delta, position][64]
     const VpfWindowAttn& a = w.a;
-    float* const stats = reinterpret_cast<float*>(lds + 4 * BUF);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hl = lane >> 5, kb = wave & 1, qs = wave >> 1;
+    float* const stats = reinterpret_cast<float*>(lds + 4 * BUF + (VREG ? 0 : KT * Tile::PITCH));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), hl = lane >> 5, kb = wave % KB, qs = wave / KB;
     const int pairs = a.B * a.Hk, bh = blockIdx.x % pairs, it = blockIdx.x / pairs, b = bh / a.Hk, hk = bh % a.Hk, pieces = w.sink_tiles * w.chunks;
     const bool far = it < pieces;
-    const int kt = far ? it / w.chunks : it - pieces, chunk = far ? it % w.chunks : 0, kt0 = kt * WA_KT;
+    const int kt = far ? it / w.chunks : it - pieces, chunk = far ? it % w.chunks : 0, kt0 = kt * KT;
     const WaSeen seen = wa_seen(w, b);
     WaRowRange rr = wa_rows_of(w, seen, kt0);
     if (kt0 >= seen.n) rr.hi = rr.lo;                                        // keys behind the ones in use
@@ -643,7 +677,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
     const int key = kt0 + 32 * kb + (lane & 31), kc = min(key, a.Lkv - 1);
     const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
     const bool kok = key < seen.n && !(pad && pad[kc]);
-    typename WaMma<T>::v8 kf[KST], vf[KST];
+    typename WaMma<T>::v8 kf[KST], vf[VREG ? KST : 1];
     {
         const T* kp = (const T*)a.k + b * a.k_sb + kc * a.k_sl + hk * a.k_sh;
         const T* vp = (const T*)a.v + b * a.v_sb + kc * a.v_sl + hk * a.v_sh;
@@ -653,7 +687,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
             uint4 u = make_uint4(0, 0, 0, 0), v = u;
             if (d < a.head_dim && kok) { u = *reinterpret_cast<const uint4*>(kp + d); v = *reinterpret_cast<const uint4*>(vp + d); }
             kf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
-            vf[s] = __builtin_bit_cast(typename WaMma<T>::v8, v);
+            if constexpr (VREG) vf[s] = __builtin_bit_cast(typename WaMma<T>::v8, v);
+            else if (qs == 0) *reinterpret_cast<uint4*>(lds + 4 * BUF + Tile::at(32 * kb + (lane & 31), 2 * s + hl)) = v;
         }
     }
     wa_f32x16 dk[DT], dv[DT];
@@ -661,13 +696,14 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
     for (int dt = 0; dt < DT; ++dt) { dk[dt] = wa_zero16(); dv[dt] = wa_zero16(); }
     const int kmin = kt0 + 32 * kb, kmax = kmin + 31;
     const bool whole = !pad && kmax < seen.n;
+    // the positions that see the lane's key are key - right .. key + left (a first token: no upper end; a hidden key: none): one unsigned comparison
+    const int see_from = kok ? key - a.right : WA_FAR + WA_FAR / 2;
+    const uint32_t see_n = !kok ? 0u : key < a.sinks ? 0x7fffffffu : (uint32_t)a.left + (uint32_t)a.right;
 
-    const WaStage<DP, ROWS> stage(a.head_dim);
-    const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
+    const WaStage<DP, ROWS, 2 * KB> stage(a.head_dim);
+    const uint32_t tiles_at = wa_lds_byte(lds), stats_at = wa_lds_byte(stats), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
     const char* qp = (const char*)((const T*)a.q + b * a.q_sb + hk * w.g * a.q_sh);
     const char* gp = (const char*)((const T*)a.dout + b * a.do_sb + hk * w.g * a.do_sh);
-    float r_lse = 0.f, r_delta = 0.f;
-    int r_pos = 0;
     auto load = [&](int r0, int buf) {
         const int q0 = wa_query(w, r0), skip = r0 - q0 * w.g, last = min(ROWS, rr.hi - r0) - 1;
         const char* qb = qp + (size_t)q0 * a.q_sl * sizeof(T);
@@ -676,55 +712,60 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
 #pragma unroll
         for (int i = 0; i < stage.PER; ++i) {
             const int r = skip + min(stage.row0 + i * stage.STEP, last), qi = wa_query(w, r), h = r - qi * w.g;
-            wa_dma(qb, (uint32_t)(qi * (int)a.q_sl + h * (int)a.q_sh) * (uint32_t)sizeof(T) + stage.col, at + stage.wave_byte + i * 4096);
-            wa_dma(gb, (uint32_t)(qi * (int)a.do_sl + h * (int)a.do_sh) * (uint32_t)sizeof(T) + stage.col, at + BUF + stage.wave_byte + i * 4096);
+            wa_dma(qb, (uint32_t)(qi * (int)a.q_sl + h * (int)a.q_sh) * (uint32_t)sizeof(T) + stage.col, at + stage.wave_byte + i * stage.ALL);
+            wa_dma(gb, (uint32_t)(qi * (int)a.do_sl + h * (int)a.do_sh) * (uint32_t)sizeof(T) + stage.col, at + BUF + stage.wave_byte + i * stage.ALL);
         }
-        if (threadIdx.x < ROWS) {
-            const int r = r0 + threadIdx.x, rc = min(r, w.rows - 1);
-            r_lse = r < rr.hi ? a.lse[(size_t)bh * w.rows + rc] : INFINITY;  // weight 0
-            r_delta = a.ws[(size_t)bh * w.rows + rc];
-            r_pos = seen.off + wa_query(w, rc);
-        }
+        const int rc = min(lane, w.rows - 1 - r0);
+        const uint32_t stat = stats_at + buf * 3 * ROWS * 4;
+        if (wave == 0) wa_dma4(a.lse + (size_t)bh * w.rows + r0, 4 * rc, stat);
+        if (wave == 1) wa_dma4(a.ws + (size_t)bh * w.rows + r0, 4 * rc, stat + 4 * ROWS);
+        if (wave == 2) reinterpret_cast<int*>(stats)[buf * 3 * ROWS + 2 * ROWS + lane] = seen.off + wa_query(w, r0 + rc);
     };
-    auto store = [&](int buf) {
-        if (threadIdx.x < ROWS) {
-            float* s = stats + buf * 3 * ROWS + threadIdx.x;
-            s[0] = r_lse; s[ROWS] = r_delta; reinterpret_cast<int*>(s)[2 * ROWS] = r_pos;
-        }
-        wa_stage_wait();
-    };
-    const int steps = (rr.hi - rr.lo + ROWS - 1) / ROWS;
-    if (steps > 0) { load(rr.lo, 0); store(0); }
+    // row blocks b_lo .. b_hi - 1, whole 64-row blocks of the sample's rows: what a block holds beyond the tile's range is hidden by its position
+    const int b_lo = rr.lo / ROWS, b_hi = rr.hi > rr.lo ? (rr.hi + ROWS - 1) / ROWS : b_lo, steps = b_hi - b_lo;
+    int top = b_hi - 1;
+    { const int c = (top + 1) / w.cycle * w.cycle - 1; if (c >= b_lo) top = c; }
+    auto block = [&](int t) { const int i = top - t; return (i < b_lo ? i + steps : i) * ROWS; };
+    if (steps > 0) { load(block(0), 0); wa_stage_wait(); }
     __syncthreads();
     for (int t = 0; t < steps; ++t) {
-        if (t + 1 < steps) load(rr.lo + (t + 1) * ROWS, (t + 1) & 1);
+        if (t + 1 < steps) load(block(t + 1), (t + 1) & 1);
         const uint32_t sq = tiles_at + (t & 1) * 2 * BUF + 32 * qs * Tile::PITCH, qrow = wa_opaque(row_base + sq), qcol = wa_opaque(col_base + sq);
+        const uint32_t vrow = VREG ? 0 : wa_opaque(row_base + tiles_at + 4 * BUF + 32 * kb * Tile::PITCH);
         const float* st = stats + (t & 1) * 3 * ROWS + 32 * qs + 4 * hl;
         const int* sp = reinterpret_cast<const int*>(stats + (t & 1) * 3 * ROWS + 2 * ROWS + 32 * qs);
-        const int rlo = rr.lo + t * ROWS + 32 * qs;
-        const int pmin = sp[0], pmax = sp[31];
-        if (rlo < rr.hi && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
+        const int rlo = block(t) + 32 * qs;
+        const int pmin = seen.off + wa_query(w, rlo), pmax = seen.off + wa_query(w, rlo + 31);      // (rows behind the last one: no harm)
+        if (rlo < rr.hi && rlo + 32 > rr.lo && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
                 s = WaMma<T>::mma(wa_frag_row<T>(qrow, i, 0), kf[i], s);
-                dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), vf[i], dp);
+                if constexpr (VREG) dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), vf[i], dp);
+                else dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), wa_frag_row<T>(vrow, i, 0), dp);
             }
-            const bool all = whole && kmax <= pmin + a.right && (kmin >= pmax - a.left || kmax < a.sinks);
+            const bool all = whole && rlo >= rr.lo && rlo + 32 <= rr.hi && kmax <= pmin + a.right && (kmin >= pmax - a.left || kmax < a.sinks);
             float p[16], ds[16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float4 lse = *reinterpret_cast<const float4*>(st + 8 * j), dl = *reinterpret_cast<const float4*>(st + ROWS + 8 * j);
                 const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
-                const int4 po = *reinterpret_cast<const int4*>(sp + 4 * hl + 8 * j);
-                const int ps[4] = {po.x, po.y, po.z, po.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * j + e;
                     p[r] = wa_exp2(fmaf(s[r], w.c, -ls[e]));
                     ds[r] = p[r] * (dp[r] - de[e]);
-                    if (!all) {
-                        const bool see = kok && key <= ps[e] + a.right && (key >= ps[e] - a.left || key < a.sinks);
+                }
+            }
+            if (!all) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int4 po = *reinterpret_cast<const int4*>(sp + 4 * hl + 8 * j);
+                    const int ps[4] = {po.x, po.y, po.z, po.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * j + e;
+                        const bool see = (uint32_t)(ps[e] - see_from) <= see_n && (uint32_t)(rlo - rr.lo + 4 * hl + 8 * j + e) < (uint32_t)(rr.hi - rr.lo);
                         p[r] = see ? p[r] : 0.f;
                         ds[r] = see ? ds[r] : 0.f;
                     }
@@ -740,12 +781,12 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
                 }
             }
         }
-        if (t + 1 < steps) store((t + 1) & 1);
+        wa_stage_wait();
         __syncthreads();
     }
     // the two halves of the rows: through LDS, dV first
     float* slot = reinterpret_cast<float*>(lds) + kb * (DT * 16 * 64) + lane;
-    static_assert(2 * DT * 16 * 64 * 4 <= 4 * BUF, "the partial results fit the stage buffers");
+    static_assert(KB * DT * 16 * 64 * 4 <= 4 * BUF, "the partial results fit the stage buffers");
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
         wa_f32x16* acc = pass ? dk : dv;
@@ -767,7 +808,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dkv_kernel(WaArgs w)
     if (qs != 0) return;
     if (kt < w.sink_tiles && w.chunks > 0) {                                 // one of the pieces of a tile with first tokens
         const size_t piece = ((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1) + (far ? chunk + 1 : 0);
-        float* part = a.ws + (size_t)a.B * a.Hk * w.rows + (piece * WA_KT + 32 * kb + (lane & 31)) * 2 * DP;
+        float* part = a.ws + wa_delta_floats(w) + (piece * KT + 32 * kb + (lane & 31)) * 2 * DP;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -797,11 +838,11 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(2 * DP) wa_sink_join_kernel(WaArgs w)
 {
     const VpfWindowAttn& a = w.a;
-    const int per = min(w.sink_tiles * WA_KT, a.Lkv), bh = blockIdx.x / per, key = blockIdx.x % per, kt = key / WA_KT, d = threadIdx.x % DP;
+    const int KT = w.key_tile, per = min(w.sink_tiles * KT, a.Lkv), bh = blockIdx.x / per, key = blockIdx.x % per, kt = key / KT, d = threadIdx.x % DP;
     const bool is_v = threadIdx.x >= DP;
-    const float* p = a.ws + (size_t)a.B * a.Hk * w.rows + ((((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1)) * WA_KT + key % WA_KT) * 2 * DP + threadIdx.x;
+    const float* p = a.ws + wa_delta_floats(w) + ((((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1)) * KT + key % KT) * 2 * DP + threadIdx.x;
     float s = 0.f;
-    for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * WA_KT * 2 * DP];
+    for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * KT * 2 * DP];
     if (d >= a.head_dim) return;
     const int b = bh / a.Hk, hk = bh % a.Hk;
     if (is_v) ((T*)a.dv)[b * a.dv_sb + key * a.dv_sl + hk * a.dv_sh + d] = (T)s;
@@ -818,7 +859,7 @@ static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
     w.a = *args;
     VpfWindowAttn& a = w.a;
     if (a.B < 0 || a.Lq < 0 || a.Lkv < 0 || a.Hk < 1 || a.Hq < a.Hk || a.Hq % a.Hk || a.head_dim < 8 || a.head_dim > VPF_WINDOW_MAX_DIM || a.head_dim % 8 ||
-        a.Lkv >= WA_FAR || a.Lq >= WA_FAR || a.sinks < 0 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return VPF_ERR_BADSHAPE;
+        a.Lkv >= WA_FAR || a.Lq >= WA_FAR - a.Lkv || a.sinks < 0 || !(a.scale > 0.f) || !(a.scale < INFINITY)) return VPF_ERR_BADSHAPE;
     if (a.dtype != VPF_T_F16 && a.dtype != VPF_T_BF16) return VPF_ERR_UNSUPPORTED;
     a.left = a.left < 0 || a.left > WA_FAR ? WA_FAR : a.left;
     a.right = a.right < 0 || a.right > WA_FAR ? WA_FAR : a.right;
@@ -863,15 +904,18 @@ static void wa_plan_fwd(WaArgs& w, int& rb)
 }
 static long wa_fwd_ws(const WaArgs& w) { return w.splits > 1 ? (long)w.splits * w.a.B * w.a.Hk * w.rows * (wa_dp(w.a.head_dim) + 2) : 0; }
 
-// The rows behind a sink tile's own window are cut into pieces about as long as the row range of an ordinary tile, where that leaves
-// more than one of them.
+// Key tiles of 128 at head dimension 128 where that leaves a workgroup for each CU (the stages of Q and dO then serve twice the keys), else of 64.
+// The rows behind a sink tile's own window are cut into pieces about as long as the row range of an ordinary tile, where that leaves more than
+// one of them.
 static void wa_plan_bwd(WaArgs& w)
 {
     const VpfWindowAttn& a = w.a;
-    w.ktiles = vpf_cdiv(a.Lkv, WA_KT);
-    w.sink_tiles = vpf_cdiv(a.sinks, WA_KT);
+    w.key_tile = wa_dp(a.head_dim) == 128 && (long)a.B * a.Hk * vpf_cdiv(a.Lkv, 128) >= 256 ? 128 : 64;
+    w.ktiles = vpf_cdiv(a.Lkv, w.key_tile);
+    w.sink_tiles = vpf_cdiv(a.sinks, w.key_tile);
     w.chunks = 0;
-    const long range = ((long)a.left + a.right + WA_KT) * w.g;
+    const long range = ((long)a.left + a.right + w.key_tile) * w.g, all = vpf_cdiv(w.rows, WA_ROWS), cycle = range / WA_ROWS + 2;
+    w.cycle = (int)(cycle < all ? cycle : all > 0 ? all : 1);
     if (w.sink_tiles > 0 && w.rows > 2 * range) {
         long rows = range > 512 ? range : 512;
         w.chunk_rows = (int)((rows + 63) / 64 * 64);
@@ -880,8 +924,7 @@ static void wa_plan_bwd(WaArgs& w)
 }
 static long wa_bwd_ws(const WaArgs& w)
 {
-    const long rows = ((long)w.a.B * w.a.Hk * w.rows + 3) / 4 * 4;
-    return rows + (w.chunks ? (long)w.a.B * w.a.Hk * w.sink_tiles * (w.chunks + 1) * WA_KT * 2 * wa_dp(w.a.head_dim) : 0);
+    return (long)wa_delta_floats(w) + (w.chunks ? (long)w.a.B * w.a.Hk * w.sink_tiles * (w.chunks + 1) * w.key_tile * 2 * wa_dp(w.a.head_dim) : 0);
 }
 
 // more than 64 KB of LDS has to be asked for, once per kernel and device
@@ -895,7 +938,7 @@ template <typename K> static int wa_lds(K kernel, size_t bytes, VpfPerDevice& do
 
 template <typename T, int DP, int RB, int KS, int SUBK> static int wa_launch_fwd(const WaArgs& w, hipStream_t st)
 {
-    constexpr size_t lds = 4 * SUBK * KS * WaTile<DP>::PITCH + 2 * SUBK * KS;
+    constexpr size_t lds = 4 * SUBK * KS * WaTile<DP>::PITCH + SUBK * KS / 4;
     static VpfPerDevice done;
     if (const int rc = wa_lds(wa_fwd_kernel<T, DP, RB, KS, SUBK>, lds, done)) return rc;
     const long grid = (long)w.a.B * w.a.Hk * w.tiles * w.splits;
@@ -915,7 +958,7 @@ template <typename T, int DP> static int wa_fwd(const WaArgs& w, int rb, hipStre
 template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaArgs& w, hipStream_t st)
 {
     constexpr int STAGE = (KS == 1 ? 64 : 32) * KS;
-    constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + 2 * STAGE;
+    constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + STAGE / 4;
     static VpfPerDevice done;
     if (const int rc = wa_lds(wa_dq_kernel<T, DP, RB, KS>, lds, done)) return rc;
     hipLaunchKernelGGL((wa_dq_kernel<T, DP, RB, KS>), dim3((unsigned)((long)w.a.B * w.a.Hk * w.tiles)), dim3(WA_THREADS), lds, st, w);
@@ -934,14 +977,19 @@ template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
         if (rc) return rc;
     }
     if (w.a.Lkv == 0) return VPF_OK;
-    constexpr size_t lds = 4 * 64 * WaTile<DP>::PITCH + 6 * 64 * 4;
-    static VpfPerDevice done;
-    if (const int rc = wa_lds(wa_dkv_kernel<T, DP>, lds, done)) return rc;
     const long grid = bh * (w.ktiles + (long)w.sink_tiles * w.chunks);
     if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
-    hipLaunchKernelGGL((wa_dkv_kernel<T, DP>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
+    auto launch = [&](auto kernel, int kb, VpfPerDevice& done) -> int {
+        const size_t lds = 4 * WA_ROWS * WaTile<DP>::PITCH + (DP <= 96 ? 0 : 32 * kb * WaTile<DP>::PITCH) + 6 * WA_ROWS * 4;
+        if (const int rc = wa_lds(kernel, lds, done)) return rc;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(128 * kb), lds, st, w);
+        return VPF_OK;
+    };
+    static VpfPerDevice done2, done4;
+    if constexpr (DP == 128) { if (w.key_tile == 128) { if (const int rc = launch(wa_dkv_kernel<T, DP, 4>, 4, done4)) return rc; } }
+    if (w.key_tile == 64) { if (const int rc = launch(wa_dkv_kernel<T, DP, 2>, 2, done2)) return rc; }
     if (w.chunks) {
-        const int per = w.sink_tiles * WA_KT < w.a.Lkv ? w.sink_tiles * WA_KT : w.a.Lkv;
+        const int per = w.sink_tiles * w.key_tile < w.a.Lkv ? w.sink_tiles * w.key_tile : w.a.Lkv;
         hipLaunchKernelGGL((wa_sink_join_kernel<T, DP>), dim3((unsigned)(bh * per)), dim3(2 * DP), 0, st, w);
     }
     VPF_CHECK_LAUNCH();

@@ -382,7 +382,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     Lkv, g = k.shape[1], Hq // k.shape[2]
     if dh % 8 or not 8 <= dh <= 128:
         raise L.VpfError(f"window_attention: head_dim is a multiple of 8 up to 128 (got {dh})")
-    if Lkv >= 1 << 30 or Lq * g * g >= 1 << 31:
+    if Lq + Lkv >= 1 << 30 or Lq * g * g >= 1 << 31:
         raise L.VpfError(f"window_attention: Lq {Lq}, Lkv {Lkv}, {g} heads per key head: beyond the kernels' index range")
     left, right = window
     for side in (left, right):
