@@ -24,6 +24,16 @@ def test_structs_match_the_library():
         assert L.lib().vpf_abi_sizeof(which) == ctypes.sizeof(cls), cls.__name__
 
 
+def test_packed_argument_structs_have_the_c_layout():
+    """L.packer builds what ctypes builds, field for field."""
+    for cls in (L.Rotary, L.GatedNorm, L.WindowAttn):
+        values = [float(i) / 8 if t is L.F else 3 + 7 * i for i, (_, t) in enumerate(cls._fields_)]
+        raw = L.packer(cls).pack(*values)
+        assert len(raw) == ctypes.sizeof(cls)
+        back = cls.from_buffer_copy(raw)
+        assert [getattr(back, n) for n, _ in cls._fields_] == values, cls.__name__
+
+
 def test_rotary_refusals():
     plan = O.RotaryAxes((8, 8), 32)
     q, k, pos = torch.zeros(2, 5, 4, 32), torch.zeros(2, 5, 2, 32), torch.zeros(5, 2)

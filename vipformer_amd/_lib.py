@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -262,6 +263,45 @@ class WindowAttn(ctypes.Structure):
                 ("q", VP), ("k", VP), ("v", VP), ("pad", VP), ("lens", VP), ("out", VP), ("lse", VP), ("out_lo", VP),
                 ("dout", VP), ("dq", VP), ("dk", VP), ("dv", VP), ("ws", VP), ("ws_floats", L_)] + \
                [(f"{t}_{s}", L_) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("sb", "sl", "sh")]
+
+
+def packer(cls):
+    """``cls`` (a ctypes.Structure of the scalar types above) as one struct.Struct: building the argument struct field by field costs a small
+    operator more host time than its launch.  Values in field order, null pointers as 0; the bytes go to the entry point as they are."""
+    return struct.Struct("@" + "".join(_PACK[t] for _, t in cls._fields_) + "0l")      # native sizes and alignment, padded like the C struct
+
+
+_PACK = {VP: "P", I: "i", F: "f", L_: "l", U32: "I"}
+
+
+def launch(name: str, packed: bytes, device) -> None:
+    """An entry point that takes one argument struct, as bytes, on torch's current stream of ``device`` (made current if it is not)."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes, fn.restype = SIGS[name], I
+        _bound[name] = fn
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise VpfError(f"{name} failed: {lib().vpf_strerror(rc).decode()} (rc={rc})")
+
+
+def scratch_floats(name: str, packed: bytes, *args) -> int:
+    """What a vpf_*_ws query of the library answers for this argument struct (floats)."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes, fn.restype = [VP] + [I] * len(args), L_
+        _bound[name] = fn
+    n = fn(packed, *args)
+    if n < 0:
+        check(n, name)
+    return n
 
 
 def call_struct(name: str, struct, *extra) -> None:

@@ -11,13 +11,10 @@ Every operator is asynchronous on torch's current stream of the tensors' device,
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
 import math
 from typing import Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import ops
@@ -25,11 +22,7 @@ from . import ops
 F32 = torch.float32
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}                   # VPF_T_*
 _POS = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}       # VPF_POS_*
-
-
-def _on(device):
-    """The library launches on the CURRENT device's stream: make it the tensors'."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_pack_rotary, _pack_norm, _pack_attn = (L.packer(c).pack for c in (L.Rotary, L.GatedNorm, L.WindowAttn))
 
 
 def _same_device(what: str, first: torch.Tensor, *rest) -> None:
@@ -40,17 +33,28 @@ def _same_device(what: str, first: torch.Tensor, *rest) -> None:
 
 
 def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _ptr(t) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _once(what: str) -> None:
+    """The kernels' gradients carry no graph of their own."""
+    if torch.is_grad_enabled():
+        raise L.VpfError(f"{what} is differentiable once (backward was called with create_graph=True)")
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
     """Batch, token and head stride; 0 where the size is 1 (torch leaves any number there)."""
-    s = t.stride()
-    return tuple(s[i] if t.shape[i] > 1 else 0 for i in range(3))
+    sb, sl, sh, _ = t.stride()
+    nb, nl, nh, _ = t.shape
+    return (sb if nb > 1 else 0, sl if nl > 1 else 0, sh if nh > 1 else 0)
 
 
 # --------------------------------------------------------------------------- rotary positions with several axes
@@ -75,7 +79,7 @@ class RotaryAxes:
             raise L.VpfError(f"RotaryAxes: base must be positive and finite (got {base})")
         if layout not in ("half", "pair") or ladder not in ("axis", "joint"):
             raise L.VpfError(f"RotaryAxes: layout is 'half' or 'pair', ladder 'axis' or 'joint' (got {layout!r}, {ladder!r})")
-        self.layout, self.ladder, self.pairs = layout, ladder, P
+        self.layout, self.ladder, self.pairs, self.layout_code = layout, ladder, P, int(layout == "pair")
         self._tables = {}
 
     def frequencies(self) -> torch.Tensor:
@@ -92,46 +96,47 @@ class RotaryAxes:
         return t
 
 
-def _rotary_call(plan, pos, tensors, outs, inverse):
-    q, k = (tensors + (None,))[:2]
-    oq, ok = (outs + (None,))[:2]
-    B, Lt, Hq, dh = q.shape
-    freq, axis = plan.tables(q.device)
-    zero = (0, 0, 0)
-    s = L.Rotary(B, Lt, Hq, 0 if k is None else k.shape[2], dh, plan.pairs, len(plan.sections), int(plan.layout == "pair"), _TYPE[q.dtype],
-                 _POS[pos.dtype], int(inverse), 0, _ptr(q), _ptr(k), _ptr(oq), _ptr(ok), *_strides(q), *(zero if k is None else _strides(k)),
-                 *_strides(oq), *(zero if k is None else _strides(ok)), _ptr(pos),
-                 pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, _ptr(freq), _ptr(axis))
-    with _on(q.device):
-        L.call_struct("vpf_rotary_axes", s)
+_NONE3 = (0, 0, 0)
 
 
 def _rotary_ready(t):
     """The kernel takes any strides with a contiguous, pair-aligned last dimension; everything else is copied."""
-    if t.stride(3) != 1 or any(s % 2 for s in _strides(t)) or t.data_ptr() % (2 * t.element_size()):
+    sb, sl, sh = _strides(t)
+    if t.stride(3) != 1 or (sb | sl | sh) & 1 or t.data_ptr() % (2 * t.element_size()):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _rotary_run(plan, pos, tensors, inverse):
-    tensors = tuple(_rotary_ready(t) for t in tensors)
-    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors)
-    _rotary_call(plan, pos, tensors, outs, inverse)
-    return outs
+def _rotary_run(plan, pos, q, k, inverse):
+    q = _rotary_ready(q)
+    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = None
+    if k is not None:
+        k = _rotary_ready(k)
+        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    B, Lt, Hq, dh = q.shape
+    freq, axis = plan.tables(q.device)
+    L.launch("vpf_rotary_axes", _pack_rotary(
+        B, Lt, Hq, 0 if k is None else k.shape[2], dh, plan.pairs, len(plan.sections), plan.layout_code, _TYPE[q.dtype], _POS[pos.dtype], inverse, 0,
+        q.data_ptr(), _ptr(k), oq.data_ptr(), _ptr(ok), *_strides(q), *(_NONE3 if k is None else _strides(k)),
+        *_strides(oq), *(_NONE3 if k is None else _strides(ok)), pos.data_ptr(), pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0,
+        freq.data_ptr(), axis.data_ptr()), q.device)
+    return oq, ok
 
 
 class RotaryAxesFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, plan, pos, *tensors):
+    def forward(ctx, plan, pos, q, k):
         ctx.plan = plan
         ctx.save_for_backward(pos)
-        return _rotary_run(plan, pos, tensors, False)
+        oq, ok = _rotary_run(plan, pos, q, k, 0)
+        return oq if k is None else (oq, ok)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
+    def backward(ctx, gq, gk=None):
+        _once("rotary_axes")
         (pos,) = ctx.saved_tensors
-        return (None, None) + _rotary_run(ctx.plan, pos, grads, True)
+        return (None, None) + _rotary_run(ctx.plan, pos, gq, gk, 1)
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryAxes):
@@ -156,31 +161,25 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     if positions.requires_grad:
         raise L.VpfError("rotary_axes: no gradient with respect to the positions (detach them)")
     _same_device("rotary_axes", q, k, positions)
-    tensors = (q,) if k is None else (q, k)
     pos = positions.contiguous()
-    outs = RotaryAxesFn.apply(plan, pos, *tensors) if _wants_grad(*tensors) else _rotary_run(plan, pos, tensors, False)
+    if _wants_grad(q, k):
+        return RotaryAxesFn.apply(plan, pos, q, k)
+    outs = _rotary_run(plan, pos, q, k, 0)
     return outs[0] if k is None else outs
 
 
 # --------------------------------------------------------------------------- norms around a block, its gate and residual scale
-def _norm_struct(cfg, x, y, gate, params):
-    """The arguments both directions share.  cfg: (kind, gate_mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre)."""
+def _norm_forward(cfg, x, y, gate, params, keep):
+    """cfg: (kind, gate_mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre)."""
     kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = cfg
     D = x.shape[-1]
-    s = L.GatedNorm(x.numel() // D, gate_rows, D, kind, _TYPE[x.dtype], _TYPE[y.dtype], mode, has_post, has_pre, 0, alpha, beta, eps_post, eps_pre,
-                    _ptr(x), _ptr(y), _ptr(gate))
-    s.w_post, s.b_post, s.w_pre, s.b_pre = (_ptr(p) for p in params)
-    return s
-
-
-def _norm_forward(cfg, x, y, gate, params, keep):
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty(y.shape, dtype=y.dtype, device=y.device) if cfg[4] else None
-    stats = torch.empty(4, x.numel() // x.shape[-1], dtype=F32, device=x.device) if keep else None
-    s = _norm_struct(cfg, x, y, gate, params)
-    s.h, s.n, s.stats = _ptr(h), _ptr(n), _ptr(stats)
-    with _on(x.device):
-        L.call_struct("vpf_gated_norm_fwd", s)
+    rows = x.numel() // D
+    h = torch.empty_like(x)
+    n = torch.empty_like(y) if has_pre else None
+    stats = torch.empty(4 * rows, dtype=F32, device=x.device) if keep else None
+    L.launch("vpf_gated_norm_fwd", _pack_norm(
+        rows, gate_rows, D, kind, _TYPE[x.dtype], _TYPE[y.dtype], mode, has_post, has_pre, 0, alpha, beta, eps_post, eps_pre, x.data_ptr(), y.data_ptr(),
+        _ptr(gate), *map(_ptr, params), h.data_ptr(), _ptr(n), _ptr(stats), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), x.device)
     return h, n, stats
 
 
@@ -195,30 +194,34 @@ class GatedNormFn(torch.autograd.Function):
         return (h, n) if n is not None else h
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dn=None):
+        _once("gated_norm_residual")
         x, y, gate, stats, *params = ctx.saved_tensors
         need = ctx.needs_input_grad
+        kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = ctx.cfg
         dev, D = x.device, x.shape[-1]
         dh = dh.contiguous()
         dn = None if dn is None else dn.contiguous()
         dx = torch.empty_like(x) if need[1] else None
         dy = torch.empty_like(y) if need[2] else None
         dgate = torch.empty_like(gate) if need[3] else None
-        s = _norm_struct(ctx.cfg, x, y, gate, params)
-        flat = torch.empty(4, D, dtype=F32, device=dev)
-        grads = [flat[i].view_as(p) if p is not None and need[4 + i] else None for i, p in enumerate(params)]
-        s.stats, s.dh, s.dn, s.dx, s.dy, s.dgate = (_ptr(t) for t in (stats, dh, dn, dx, dy, dgate))
-        s.dw_post, s.db_post, s.dw_pre, s.db_pre = (_ptr(g) for g in grads)
-        floats = L.lib().vpf_gated_norm_ws
-        floats.restype = L.L_
-        ws = torch.empty(max(int(floats(ctypes.byref(s))), 4), dtype=F32, device=dev)
-        s.ws, s.ws_floats = _ptr(ws), ws.numel()
-        with _on(dev):
-            L.call_struct("vpf_gated_norm_bwd", s)
+        flat = grads = None
+        if True in need[4:]:
+            flat = torch.empty(4, D, dtype=F32, device=dev)
+            grads = [g if n else None for g, n in zip(flat.unbind(0), need[4:])]
+        else:
+            grads = [None] * 4
+        args = [x.numel() // D, gate_rows, D, kind, _TYPE[x.dtype], _TYPE[y.dtype], mode, has_post, has_pre, 0, alpha, beta, eps_post, eps_pre,
+                x.data_ptr(), y.data_ptr(), _ptr(gate), *map(_ptr, params), 0, 0, stats.data_ptr(), dh.data_ptr(), _ptr(dn), _ptr(dx), _ptr(dy), _ptr(dgate),
+                *map(_ptr, grads), 0, 0]
+        floats = L.scratch_floats("vpf_gated_norm_ws", _pack_norm(*args))
+        ws = torch.empty(max(floats, 4), dtype=F32, device=dev)
+        args[-2:] = ws.data_ptr(), ws.numel()
+        L.launch("vpf_gated_norm_bwd", _pack_norm(*args), dev)
         inv = ctx.iscale.inv if ctx.iscale is not None else None
         if inv is not None:
-            flat.mul_(inv)
+            if flat is not None:
+                flat.mul_(inv)
             if dgate is not None and ctx.gate_is_param:
                 dgate.mul_(inv)
         return (None, dx, dy, dgate, *grads)
@@ -291,46 +294,41 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
 def _attn_ready(t: torch.Tensor) -> torch.Tensor:
     """16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8 elements, those of tokens and heads below 2^23;
     everything else is copied."""
-    s = _strides(t)
-    if t.stride(3) != 1 or any(n % 8 for n in s) or max(s[1:]) >= 1 << 23 or t.data_ptr() % 16:
+    sb, sl, sh = _strides(t)
+    if t.stride(3) != 1 or (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or t.data_ptr() & 15:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _attn_struct(cfg, q, k, v, pad, lens, out, lse, lo):
+def _attn_args(cfg, q, k, v, pad, lens, out, lse, lo):
+    """The fields both directions share, in front of the gradients' and behind them."""
     left, right, sinks, scale = cfg
     B, Lq, Hq, dh = q.shape
-    s = L.WindowAttn(B, Lq, k.shape[1], Hq, k.shape[2], dh, left, right, sinks, _TYPE[q.dtype], scale, 0, _ptr(q), _ptr(k), _ptr(v), _ptr(pad),
-                     _ptr(lens), _ptr(out), _ptr(lse), _ptr(lo))
-    for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
-        _attn_strides(s, name, t)
-    return s
+    head = (B, Lq, k.shape[1], Hq, k.shape[2], dh, left, right, sinks, _TYPE[q.dtype], scale, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(pad),
+            _ptr(lens), out.data_ptr(), _ptr(lse), _ptr(lo))
+    return head, _strides(q) + _strides(k) + _strides(v) + _strides(out)
 
 
-def _attn_strides(s, name, t):
-    sb, sl, sh = _strides(t)
-    setattr(s, name + "_sb", sb), setattr(s, name + "_sl", sl), setattr(s, name + "_sh", sh)
-
-
-def _attn_workspace(s, backward, device):
-    fn = L.lib().vpf_window_attn_ws
-    fn.restype = L.L_
-    n = int(fn(ctypes.byref(s), backward))
-    L.check(min(n, 0), "vpf_window_attn_ws")
+def _attn_launch(name, head, tail, backward, device):
+    """Scratch is asked for, allocated and handed over; it stays alive until the launch is issued (the allocator orders its reuse by stream)."""
+    n = L.scratch_floats("vpf_window_attn_ws", _pack_attn(*head, 0, 0, *tail), backward)
     ws = torch.empty(n, dtype=F32, device=device) if n else None
-    s.ws, s.ws_floats = _ptr(ws), n
-    return ws
+    L.launch(name, _pack_attn(*head, _ptr(ws), n, *tail), device)
+
+
+_NO_GRAD_PTRS, _NO_GRAD_STRIDES = (0,) * 4, (0,) * 12
 
 
 def _attn_forward(cfg, q, k, v, pad, lens, keep):
     B, Lq, Hq, dh = q.shape
-    out = torch.empty(B, Lq, Hq, dh, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, k.shape[2], Lq * Hq // k.shape[2], dtype=F32, device=q.device) if keep else None
-    lo = torch.empty(B, Lq, Hq, dh, dtype=q.dtype, device=q.device) if keep else None
-    s = _attn_struct(cfg, q, k, v, pad, lens, out, lse, lo)
-    ws = _attn_workspace(s, 0, q.device)        # noqa: F841  (alive until the launch is issued; the allocator orders its reuse by stream)
-    with _on(q.device):
-        L.call_struct("vpf_window_attn_fwd", s)
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = lo = None
+    if keep:
+        lse = torch.empty(B * Lq * Hq, dtype=F32, device=dev)
+        lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    head, tail = _attn_args(cfg, q, k, v, pad, lens, out, lse, lo)
+    _attn_launch("vpf_window_attn_fwd", head + _NO_GRAD_PTRS, tail + _NO_GRAD_STRIDES, 0, dev)
     return out, lse, lo
 
 
@@ -344,18 +342,15 @@ class WindowAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
+        _once("window_attention")
         q, k, v, out, lse, lo, pad, lens = ctx.saved_tensors
         dout = _attn_ready(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        s = _attn_struct(ctx.cfg, q, k, v, pad, lens, out, lse, lo)
-        s.dout, s.dq, s.dk, s.dv = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv)
-        for name, t in (("do", dout), ("dq", dq), ("dk", dk), ("dv", dv)):
-            _attn_strides(s, name, t)
-        ws = _attn_workspace(s, 1, q.device)    # noqa: F841
-        with _on(q.device):
-            L.call_struct("vpf_window_attn_bwd", s)
+        dev = q.device
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        head, tail = _attn_args(ctx.cfg, q, k, v, pad, lens, out, lse, lo)
+        _attn_launch("vpf_window_attn_bwd", head + (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
+                     tail + _strides(dout) + _strides(dq) + _strides(dk) + _strides(dv), 1, dev)
         return None, dq, dk, dv, None, None
 
 
