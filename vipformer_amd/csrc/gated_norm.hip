@@ -21,17 +21,6 @@ enum { GN_WANT_WPOST = 1, GN_WANT_BPOST = 2, GN_WANT_WPRE = 4, GN_WANT_BPRE = 8,
 
 // this thread's columns of a row: 8 t .. 8 t + 7 (V = 8: D a multiple of 8, 16-byte aligned) or t, t + TPR, .. (V = 1)
 template <int TPR, int V> __device__ __forceinline__ int gn_col(int t, int e) { return V == 8 ? 8 * t + e : t + e * TPR; }
-template <typename T, int TPR, int V> __device__ __forceinline__ void gn_load(float* v, const T* p, int t, int D, float fill = 0.f)
-{
-    if constexpr (V == 8) {
-        if (8 * t < D) { vpf_load<T, 8>(v, p + 8 * t); return; }
-#pragma unroll
-        for (int e = 0; e < GN_E; ++e) v[e] = fill;
-    } else {
-#pragma unroll
-        for (int e = 0; e < GN_E; ++e) { const int c = gn_col<TPR, V>(t, e); v[e] = c < D ? (float)p[c] : fill; }
-    }
-}
 template <typename T, int TPR, int V> __device__ __forceinline__ void gn_store(T* p, const float* v, int t, int D)
 {
     if constexpr (V == 8) { if (8 * t < D) vpf_store<T, 8>(p + 8 * t, v); }
@@ -40,9 +29,24 @@ template <typename T, int TPR, int V> __device__ __forceinline__ void gn_store(T
         for (int e = 0; e < GN_E; ++e) { const int c = gn_col<TPR, V>(t, e); if (c < D) p[c] = (T)v[e]; }
     }
 }
+// a thread's part of a row as it lies in memory: the next row's tensors wait in these registers while this row is worked on.  Columns behind D
+// are fetched from column 0 and read as 0.
+template <typename T, int TPR, int V> struct GnRaw {
+    VpfRaw<T, V> r[GN_E / V];
+    __device__ __forceinline__ void fetch(const T* p, int t, int D)
+    {
+#pragma unroll
+        for (int e = 0; e < GN_E; e += V) { const int c = gn_col<TPR, V>(t, e); r[e / V].load(p + (c < D ? c : 0)); }
+    }
+    __device__ __forceinline__ void get(float* v, int t, int D) const
+    {
+#pragma unroll
+        for (int e = 0; e < GN_E; ++e) { const float x = r[e / V].get(e % V); v[e] = gn_col<TPR, V>(t, e) < D ? x : 0.f; }
+    }
+};
 template <int TPR, int V> __device__ __forceinline__ void gn_param(float* v, const float* p, int t, int D, float none)
 {
-    if (p) gn_load<float, TPR, V>(v, p, t, D);
+    if (p) { GnRaw<float, TPR, V> r; r.fetch(p, t, D); r.get(v, t, D); }
     else {
 #pragma unroll
         for (int e = 0; e < GN_E; ++e) v[e] = none;
@@ -111,18 +115,27 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_fwd_kernel(GnArgs g)
     gn_param<TPR, V>(bn, a.b_pre, t, D, 0.f);
 #pragma unroll
     for (int e = 0; e < GN_E; ++e) gt[e] = 1.f;
+    GnRaw<TX, TPR, V> rx;
+    GnRaw<TY, TPR, V> ry_, rg;
+    auto fetch = [&](long i) {
+        const long r = min(i + grp, r1 - 1);                              // the last rows may be taken twice: every wave meets every barrier
+        rx.fetch((const TX*)a.x + r * D, t, D);
+        ry_.fetch((const TY*)a.y + r * D, t, D);
+        if (a.gate_mode == VPF_GATE_FULL) rg.fetch((const TY*)a.gate + r * D, t, D);
+    };
+    fetch(r0);
     int sample = -1;
     for (long i = r0; i < r1; i += G) {
-        const long r = min(i + grp, r1 - 1);                              // the last rows may be taken twice: every wave meets every barrier
+        const long r = min(i + grp, r1 - 1);
         const bool mine = i + grp < r1;
         float x[GN_E], y[GN_E];
-        gn_load<TX, TPR, V>(x, (const TX*)a.x + r * D, t, D);
-        gn_load<TY, TPR, V>(y, (const TY*)a.y + r * D, t, D);
-        if (a.gate_mode == VPF_GATE_FULL) gn_load<TY, TPR, V>(gt, (const TY*)a.gate + r * D, t, D);
+        rx.get(x, t, D); ry_.get(y, t, D);
+        if (a.gate_mode == VPF_GATE_FULL) rg.get(gt, t, D);
         else if (a.gate_mode == VPF_GATE_ROWS) {
             const int s = (int)((uint32_t)r / (uint32_t)a.gate_rows);
-            if (s != sample) { gn_load<float, TPR, V>(gt, (const float*)a.gate + (long)s * D, t, D); sample = s; }
+            if (s != sample) { gn_param<TPR, V>(gt, (const float*)a.gate + (long)s * D, t, D, 1.f); sample = s; }
         }
+        fetch(i + G < r1 ? i + G : i);                                    // (unconditional: behind a branch its values would be awaited at the join)
         float my = 0.f, ry = 1.f, mh = 0.f, rh = 1.f;
         if (a.has_post) {
             gn_stats<TPR, V>(y, t, D, a.kind, a.eps_post, my, ry, red, buf);
@@ -191,18 +204,30 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
         if (a.gate_mode == VPF_GATE_ROWS) {
             s = (int)((uint32_t)seg / (uint32_t)a.gate_rows);
             end = min(r1, (long)(s + 1) * a.gate_rows);
-            gn_load<float, TPR, V>(gt, (const float*)a.gate + (long)s * D, t, D);
+            gn_param<TPR, V>(gt, (const float*)a.gate + (long)s * D, t, D, 1.f);
         }
+        GnRaw<TX, TPR, V> rdh, rx;
+        GnRaw<TY, TPR, V> rdn, ry_, rg;
+        float s0, s1_, s2_, s3;
+        auto fetch = [&](long i) {
+            const long r = min(i + grp, end - 1);
+            rdh.fetch((const TX*)a.dh + r * D, t, D);
+            if (a.has_pre) rdn.fetch((const TY*)a.dn + r * D, t, D);
+            rx.fetch((const TX*)a.x + r * D, t, D);
+            ry_.fetch((const TY*)a.y + r * D, t, D);
+            if (a.gate_mode == VPF_GATE_FULL) rg.fetch((const TY*)a.gate + r * D, t, D);
+            s0 = a.stats[r]; s1_ = a.stats[a.rows + r]; s2_ = a.stats[2 * a.rows + r]; s3 = a.stats[3 * a.rows + r];
+        };
+        fetch(seg);
         for (long i = seg; i < end; i += G) {
             const long r = min(i + grp, end - 1);
             const bool mine = i + grp < end;
             float x[GN_E], y[GN_E], dh[GN_E], dn[GN_E], u[GN_E];
-            gn_load<TX, TPR, V>(dh, (const TX*)a.dh + r * D, t, D);
-            if (a.has_pre) gn_load<TY, TPR, V>(dn, (const TY*)a.dn + r * D, t, D);
-            gn_load<TX, TPR, V>(x, (const TX*)a.x + r * D, t, D);
-            gn_load<TY, TPR, V>(y, (const TY*)a.y + r * D, t, D);
-            if (a.gate_mode == VPF_GATE_FULL) gn_load<TY, TPR, V>(gt, (const TY*)a.gate + r * D, t, D);
-            const float my = a.stats[r], ry = a.stats[a.rows + r], mh = a.stats[2 * a.rows + r], rh = a.stats[3 * a.rows + r];
+            rdh.get(dh, t, D); rx.get(x, t, D); ry_.get(y, t, D);
+            if (a.has_pre) rdn.get(dn, t, D);
+            if (a.gate_mode == VPF_GATE_FULL) rg.get(gt, t, D);
+            const float my = s0, ry = s1_, mh = s2_, rh = s3;
+            fetch(i + G < end ? i + G : i);                               // (unconditional: behind a branch its values would be awaited at the join)
             const float one = mine ? 1.f : 0.f;
 #pragma unroll
             for (int e = 0; e < GN_E; ++e) {
@@ -322,11 +347,11 @@ static void gn_plan(GnArgs& g, int want_wgs)
     g.nwg = vpf_cdiv(g.a.rows, per);
 }
 // Backward: a workgroup walks at least 4 row groups, so that its partial rows (5 D floats) stay small beside what it reads, and the
-// partials are at most 768 rows (three workgroups per CU).
+// partials are at most 1024 rows (four workgroups per CU).
 static void gn_plan_bwd(GnArgs& g)
 {
     const long want = g.a.rows / (4L * gn_groups(g.a.D)) + 1;
-    gn_plan(g, want < 768 ? (int)want : 768);
+    gn_plan(g, want < 1024 ? (int)want : 1024);
     const VpfGatedNorm& a = g.a;
     g.want = (a.has_post && a.dw_post ? GN_WANT_WPOST : 0) | (a.has_post && a.db_post ? GN_WANT_BPOST : 0) | (a.has_pre && a.dw_pre ? GN_WANT_WPRE : 0) |
              (a.has_pre && a.db_pre ? GN_WANT_BPRE : 0) | (a.gate_mode == VPF_GATE_ROWS && a.dgate ? GN_WANT_GATE : 0);

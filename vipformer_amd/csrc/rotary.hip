@@ -8,15 +8,15 @@
 // one sincospi per angle) while its first q / k loads are in flight; what remains is one read and one write of q and k: HBM bound.
 #include "vpf_elem.h"
 
-#define ROT_THREADS 256
-#define ROT_ITEMS 4             // chunks a thread has in flight: loads of all of them are issued in front of the angle table
-#define ROT_TOKENS 64           // tokens a workgroup takes at most
+#define ROT_BYTES 128           // bytes a thread has in flight
+#define ROT_MAX_THREADS 1024
 
 struct RotArgs {
     VpfRotary a;
     int tok;                    // tokens per workgroup
     int blocks;                 // workgroups per sample
     int rot_chunks, chunks;     // chunks of a head: rotated ones, all of them (the rest is copied)
+    int side;                   // tokens side by side in a workgroup
 };
 
 __device__ __forceinline__ double rot_pos(const VpfRotary& a, size_t i)
@@ -31,76 +31,68 @@ __device__ __forceinline__ double rot_pos(const VpfRotary& a, size_t i)
 
 // A chunk is what one thread rotates at a time: HALF: V channels at c and the V partners at c + P; otherwise: V pairs side by side
 // (2 V channels).  Chunks behind rot_chunks are copied: V (HALF) or 2 V channels each.
+// A thread keeps its head and chunk and walks over tokens, ITEMS of them in flight: the divisions and the pointers are made once.
 template <typename T, int V, bool HALF>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotArgs r)
+__global__ void __launch_bounds__(ROT_MAX_THREADS) rotary_kernel(RotArgs r)
 {
+    constexpr int N = 2 * V * (int)sizeof(T), ITEMS = ROT_BYTES / N < 1 ? 1 : ROT_BYTES / N > 8 ? 8 : ROT_BYTES / N;
     extern __shared__ float2 rot_table[];                       // [tok][P]
     const VpfRotary& a = r.a;
-    const int b = blockIdx.x / r.blocks, t0 = (blockIdx.x % r.blocks) * r.tok;
-    const int nt = min(r.tok, a.L - t0), H = a.Hq + a.Hk;
-    const int per = H * r.chunks, n = nt * per;
-
-    struct Item { const T* src; T* dst; int t, c; };
-    auto locate = [&](int i) {
-        Item it;
-        it.t = i / per;
-        const int rest = i - it.t * per, head = rest / r.chunks;
-        it.c = rest - head * r.chunks;
-        const long tok = t0 + it.t;
-        if (head < a.Hq) {
-            it.src = (const T*)a.q + b * a.q_sb + tok * a.q_sl + head * a.q_sh;
-            it.dst = (T*)a.oq + b * a.oq_sb + tok * a.oq_sl + head * a.oq_sh;
-        } else {
-            const int hk = head - a.Hq;
-            it.src = (const T*)a.k + b * a.k_sb + tok * a.k_sl + hk * a.k_sh;
-            it.dst = (T*)a.ok + b * a.ok_sb + tok * a.ok_sl + hk * a.ok_sh;
-        }
-        return it;
-    };
+    const int b = blockIdx.x / r.blocks, t0 = (blockIdx.x % r.blocks) * r.tok, nt = min(r.tok, a.L - t0);
+    const int H = a.Hq + a.Hk, per = H * r.chunks, sub = (int)threadIdx.x / per;
     bool table = false;
-    for (int base = 0; base < n; base += ROT_THREADS * ROT_ITEMS) {
-        float x[ROT_ITEMS][2 * V];
+    // (one turn of the outer loop unless a token has more chunks than the workgroup threads)
+    for (int base = 0; base < per; base += blockDim.x) {
+        const bool mine = sub < r.side && base + (int)threadIdx.x - sub * per < per;
+        const int item = mine ? base + threadIdx.x - sub * per : 0, head = item / r.chunks, c = item - head * r.chunks;
+        const bool isq = head < a.Hq, turned = c < r.rot_chunks;
+        const int h = isq ? head : head - a.Hq;
+        const long sl = isq ? a.q_sl : a.k_sl, ol = isq ? a.oq_sl : a.ok_sl;
+        const int at = HALF ? (turned ? c * V : 2 * a.P + (c - r.rot_chunks) * V) : c * 2 * V;
+        const T* src = (isq ? (const T*)a.q + b * a.q_sb + h * a.q_sh : (const T*)a.k + b * a.k_sb + h * a.k_sh) + t0 * sl + at;
+        T* dst = (isq ? (T*)a.oq + b * a.oq_sb + h * a.oq_sh : (T*)a.ok + b * a.ok_sb + h * a.ok_sh) + t0 * ol + at;
+        const int partner = turned ? a.P : 0;
+        for (int first = 0; first < nt; first += ITEMS * r.side) {
+            VpfRaw<T, HALF ? V : 2 * V> x[ITEMS], z[HALF ? ITEMS : 1];
 #pragma unroll
-        for (int j = 0; j < ROT_ITEMS; ++j) {
-            const int i = base + j * ROT_THREADS + threadIdx.x;
-            if (i >= n) continue;
-            const Item it = locate(i);
-            if (it.c < r.rot_chunks) {
-                if (HALF) { vpf_load<T, V>(x[j], it.src + it.c * V); vpf_load<T, V>(x[j] + V, it.src + a.P + it.c * V); }
-                else vpf_load<T, 2 * V>(x[j], it.src + it.c * 2 * V);
-            } else if (HALF) vpf_load<T, V>(x[j], it.src + 2 * a.P + (it.c - r.rot_chunks) * V);
-            else vpf_load<T, 2 * V>(x[j], it.src + it.c * 2 * V);
-        }
-        if (!table) {
-            for (int i = threadIdx.x; i < nt * a.P; i += ROT_THREADS) {
-                const int t = i / a.P, p = i - t * a.P;
-                const double turns = rot_pos(a, (size_t)b * a.pos_sb + (size_t)(t0 + t) * a.axes + a.axis[p]) * a.freq[p];
-                float s, c;
-                sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-                rot_table[i] = make_float2(c, a.inverse ? -s : s);
+            for (int j = 0; j < ITEMS; ++j) {                   // (tokens behind the last one: the last one again, dropped below)
+                const T* p = src + min(first + j * r.side + sub, nt - 1) * sl;
+                x[j].load(p);
+                if (HALF) z[j].load(p + partner);
             }
-            __syncthreads();
-            table = true;
-        }
-#pragma unroll
-        for (int j = 0; j < ROT_ITEMS; ++j) {
-            const int i = base + j * ROT_THREADS + threadIdx.x;
-            if (i >= n) continue;
-            const Item it = locate(i);
-            if (it.c < r.rot_chunks) {
-                const float2* cs = rot_table + it.t * a.P + it.c * V;
-                float y[2 * V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float2 w = cs[e];
-                    const float x0 = HALF ? x[j][e] : x[j][2 * e], x1 = HALF ? x[j][V + e] : x[j][2 * e + 1];
-                    y[HALF ? e : 2 * e] = x0 * w.x - x1 * w.y;
-                    y[HALF ? V + e : 2 * e + 1] = x1 * w.x + x0 * w.y;
+            if (!table) {
+                for (int i = threadIdx.x; i < nt * a.P; i += blockDim.x) {
+                    const int t = i / a.P, p = i - t * a.P;
+                    const double turns = rot_pos(a, (size_t)b * a.pos_sb + (size_t)(t0 + t) * a.axes + a.axis[p]) * a.freq[p];
+                    float s, co;
+                    sincospif(2.0f * (float)(turns - rint(turns)), &s, &co);
+                    rot_table[i] = make_float2(co, a.inverse ? -s : s);
                 }
-                if (HALF) { vpf_store<T, V>(it.dst + it.c * V, y); vpf_store<T, V>(it.dst + a.P + it.c * V, y + V); }
-                else vpf_store<T, 2 * V>(it.dst + it.c * 2 * V, y);
-            } else if (HALF) vpf_store<T, V>(it.dst + 2 * a.P + (it.c - r.rot_chunks) * V, x[j]);
-            else vpf_store<T, 2 * V>(it.dst + it.c * 2 * V, x[j]);
+                __syncthreads();
+                table = true;
+            }
+#pragma unroll
+            for (int j = 0; j < ITEMS; ++j) {
+                const int t = first + j * r.side + sub;
+                if (!mine || t >= nt) continue;
+                T* p = dst + t * ol;
+                float y[2 * V];
+                if (turned) {
+                    const float2* cs = rot_table + t * a.P + c * V;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float2 w = cs[e];
+                        const float x0 = HALF ? x[j].get(e) : x[j].get(2 * e), x1 = HALF ? z[j].get(e) : x[j].get(2 * e + 1);
+                        y[HALF ? e : 2 * e] = x0 * w.x - x1 * w.y;
+                        y[HALF ? V + e : 2 * e + 1] = x1 * w.x + x0 * w.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < (HALF ? V : 2 * V); ++e) y[e] = x[j].get(e);
+                }
+                if (!HALF) vpf_store<T, 2 * V>(p, y);
+                else { vpf_store<T, V>(p, y); if (turned) vpf_store<T, V>(p + a.P, y + V); }
+            }
         }
     }
 }
@@ -112,19 +104,22 @@ static int rotary_launch(const VpfRotary& a, hipStream_t st)
     r.a = a;
     r.rot_chunks = a.P / V;
     r.chunks = r.rot_chunks + (a.head_dim - 2 * a.P) / (HALF ? V : 2 * V);
-    // Tokens per workgroup: enough that every thread holds ROT_ITEMS chunks and the angle table is shared by them, but no fewer than
-    // about 1024 workgroups (four per CU) where the call has that many tokens.
-    const long per = (long)(a.Hq + a.Hk) * r.chunks, tokens = (long)a.B * a.L;
-    long tok = (ROT_THREADS * ROT_ITEMS + per - 1) / per;
-    tok = tok < tokens / 1024 + 1 ? tok : tokens / 1024 + 1;
-    tok = tok < ROT_TOKENS ? tok : ROT_TOKENS;
-    const long fits = 65536 / (long)sizeof(float2) / a.P;
+    // A workgroup is as many whole tokens side by side as 256 threads hold (one, with up to 1024 threads, where a token has more chunks).
+    const int per = (a.Hq + a.Hk) * r.chunks;
+    r.side = per <= 256 ? 256 / per : 1;
+    const int threads = vpf_cdiv((long)r.side * per < ROT_MAX_THREADS ? (long)r.side * per : ROT_MAX_THREADS, 64) * 64;
+    // Its tokens: one full set in flight, fewer where the call would not leave about 1024 workgroups (four per CU).
+    constexpr int N = 2 * V * (int)sizeof(T), ITEMS = ROT_BYTES / N < 1 ? 1 : ROT_BYTES / N > 8 ? 8 : ROT_BYTES / N;
+    const long tokens = (long)a.B * a.L, fits = 65536 / (long)sizeof(float2) / a.P;
+    long deep = tokens / (1024L * r.side);
+    deep = deep < 1 ? 1 : deep < ITEMS ? deep : ITEMS;
+    long tok = deep * r.side;
     tok = tok < fits ? tok : fits;
     r.tok = (int)(tok < a.L ? tok : a.L);
     r.blocks = vpf_cdiv(a.L, r.tok);
     const long grid = (long)a.B * r.blocks;
     if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
-    hipLaunchKernelGGL((rotary_kernel<T, V, HALF>), dim3((unsigned)grid), dim3(ROT_THREADS), sizeof(float2) * r.tok * a.P, st, r);
+    hipLaunchKernelGGL((rotary_kernel<T, V, HALF>), dim3((unsigned)grid), dim3(threads), sizeof(float2) * r.tok * a.P, st, r);
     VPF_CHECK_LAUNCH();
     return VPF_OK;
 }

@@ -31,3 +31,26 @@ template <typename T, int N> __device__ __forceinline__ void vpf_store(T* p, con
     for (int i = 0; i < N; ++i) r.e[i] = (T)v[i];
     *reinterpret_cast<VpfPack<T, N>*>(p) = r;
 }
+// The same N elements unconverted, in whole registers: a load whose value is first needed much later (converting it at once would make the
+// wave wait right behind the load; so would a branch around it -- load from a clamped address and drop the value instead).
+template <typename T, int N> struct VpfRaw {
+    static constexpr int BYTES = N * (int)sizeof(T), WORDS = (BYTES + 3) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* p)
+    {
+        if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+        } else if constexpr (BYTES == 8) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+        else if constexpr (BYTES == 4) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        else w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
+    __device__ __forceinline__ float get(int i) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return (float)__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (16 * (i & 1))));
+    }
+};
