@@ -496,3 +496,293 @@ def test_window_attention_is_bitwise_reproducible():
         runs.append([out.detach(), *torch.autograd.grad(out, (q, k, v), dout)])
     for r in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+# ------------------------------------------------------------------------------------------ edges that the three share
+def test_empty_calls_and_zero_gradients():
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    w, gate = torch.ones(16, device="cuda", requires_grad=True), torch.ones(2, 1, 16, device="cuda", requires_grad=True)
+    x = torch.zeros(2, 0, 16, device="cuda", requires_grad=True)
+    h, n = gated_norm_residual(x, x.detach().half(), gate=gate, post=(w, None), pre=(w, None), kind="rms")
+    assert h.shape == n.shape == x.shape
+    dx, dw, dg = torch.autograd.grad((h, n), (x, w, gate), (h.detach(), n.detach()))
+    assert dx.shape == x.shape and float(dw.abs().sum()) == 0.0 and float(dg.abs().sum()) == 0.0
+    q = torch.zeros(0, 5, 2, 16, device="cuda", dtype=torch.float16)
+    assert rotary_axes(q, q, torch.zeros(5, 1, device="cuda"), RotaryAxes((8,), 16))[1].shape == q.shape
+    assert window_attention(q, q, q, (3, 3)).shape == q.shape
+
+
+def test_block_ops_refuse_a_second_derivative():
+    from vipformer_amd import _lib
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    g = gen(1)
+    q = randn(g, 1, 8, 1, 16, dtype=torch.float16).requires_grad_()
+    x = randn(g, 1, 8, 16).requires_grad_()
+    for out, leaf in ((rotary_axes(q, None, torch.zeros(8, 1, device="cuda"), RotaryAxes((8,), 16)), q), (window_attention(q, q, q), q),
+                      (gated_norm_residual(x, x)[0], x)):
+        with pytest.raises(_lib.VpfError, match="differentiable once"):
+            torch.autograd.grad(out.float().sum(), leaf, create_graph=True)
+
+
+def test_block_ops_mixed_devices_and_cpu_tensors_are_refused():
+    from vipformer_amd import _lib
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    q, cpu = torch.zeros(1, 4, 1, 16, device="cuda", dtype=torch.float16), torch.zeros(1, 4, 1, 16, dtype=torch.float16)
+    for call in (lambda: rotary_axes(q, None, torch.zeros(4, 1), RotaryAxes((8,), 16)), lambda: window_attention(q, cpu, cpu),
+                 lambda: window_attention(q, q, q, kv_lens=torch.ones(1, dtype=torch.int32)), lambda: gated_norm_residual(q, q, post=(torch.ones(16), None))):
+        with pytest.raises(_lib.VpfError):
+            call()
+
+
+def block_inputs(g, B=2, L=145, D=256, H=4):
+    c = lambda *s, scale=1.0, dt=torch.float32: randn(g, *s, scale=scale, dtype=dt)
+    P = dict(x=c(B, L, D), a=c(B, L, D, dt=torch.float16), wqkv=c(3 * D, D, scale=D ** -0.5, dt=torch.float16), wo=c(D, D, scale=D ** -0.5, dt=torch.float16),
+             gate=c(D, scale=0.5), w1=1.0 + c(D, scale=0.1), b1=c(D, scale=0.1), w2=1.0 + c(D, scale=0.1), b2=c(D, scale=0.1))
+    grid = torch.stack(torch.meshgrid(torch.arange(12.0), torch.arange(12.0), indexing="ij"), -1).reshape(-1, 2)
+    pos = torch.cat([torch.zeros(1, 2), grid]).cuda()
+    return P, pos
+
+
+def block(P, pos, plan, pad=None):
+    """Projection -> rotary positions -> windowed attention -> projection -> gated norms: the operators as one encoder block uses them."""
+    from vipformer_amd.ops_block import gated_norm_residual, rotary_axes, window_attention
+    B, L, D = P["x"].shape
+    qkv = torch.nn.functional.linear(P["a"], P["wqkv"]).view(B, L, 3, plan.heads, plan.head_dim)
+    q, k = rotary_axes(qkv[:, :, 0], qkv[:, :, 1], pos, plan)
+    o = window_attention(q, k, qkv[:, :, 2], (32, 32), sinks=1, pad_mask=pad)
+    y = torch.nn.functional.linear(o.flatten(2), P["wo"])
+    return gated_norm_residual(P["x"], y, gate=P["gate"], post=(P["w1"], P["b1"]), pre=(P["w2"], P["b2"]), alpha=0.9)
+
+
+def block_plan(H=4, dh=64):
+    from vipformer_amd.ops_block import RotaryAxes
+    plan = RotaryAxes((16, 16), dh, base=100.0)
+    plan.heads = H
+    return plan
+
+
+def test_a_block_of_them_against_64_bits():
+    """The run as it is used, forward and every gradient.  16 roundings to fp16 on the way (6 forward, 10 back), each 2^-11 of its tensor, at most
+    doubled by softmax and norms: 2^-6 of the result's norm."""
+    g = gen(21)
+    P, pos = block_inputs(g)
+    plan = block_plan()
+    pad = torch.zeros(2, 145, dtype=torch.bool, device="cuda")
+    pad[1, 100:] = True
+    for t in P.values():
+        t.requires_grad_()
+    h, n = block(P, pos, plan, pad)
+    dh, dn = randn(g, *h.shape), randn(g, *n.shape, dtype=torch.float16)
+    grads = torch.autograd.grad((h, n), list(P.values()), (dh, dn))
+
+    R = {k: v.detach().double().requires_grad_() for k, v in P.items()}
+    B, L, D = R["x"].shape
+    qkv = (R["a"] @ R["wqkv"].t()).view(B, L, 3, 4, 64)
+    f = plan.frequencies().cuda()
+    ang = torch.cat([pos[:, :1].double() * f[:16], pos[:, 1:].double() * f[16:]], -1)[None, :, None]
+    turn = lambda t: torch.cat([t[..., :32] * ang.cos() - t[..., 32:] * ang.sin(), t[..., 32:] * ang.cos() + t[..., :32] * ang.sin()], -1)
+    q, k, v = (t.transpose(1, 2) for t in (turn(qkv[:, :, 0]), turn(qkv[:, :, 1]), qkv[:, :, 2]))
+    m = seen_mask(B, L, L, (32, 32), 1, pad, None)[:, None]
+    s = (q @ k.transpose(-1, -2) / 8.0).masked_fill(~m, -math.inf)
+    dead = ~m.any(-1, keepdim=True)
+    o = (torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0) @ v).transpose(1, 2).reshape(B, L, D)
+    y = o @ R["wo"].t()
+    ln = lambda z, w, b: torch.nn.functional.layer_norm(z, (D,), w, b, 1e-5)
+    hr = 0.9 * R["x"] + R["gate"] * ln(y, R["w1"], R["b1"])
+    nr = ln(hr, R["w2"], R["b2"])
+    ref = torch.autograd.grad((hr, nr), list(R.values()), (dh.double(), dn.double()))
+    for name, a, b in [("h", h, hr), ("n", n, nr)] + list(zip(P, grads, ref)):
+        rel = float((a.detach().double() - b).norm() / b.detach().norm())
+        assert rel < 2.0 ** -6, (name, rel)
+
+
+def test_gradients_against_differences():
+    """<gradient, d> against (f(x + e d) - f(x - e d)) / 2 e of the operators themselves.  fp32: e = 2^-6, the difference carries e^2 / 6 of the third
+    derivative and 2^-24 / e of each of the summed outputs, below 2^-9 of the sum of their magnitudes."""
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes
+    g = gen(22)
+    plan = RotaryAxes((4, 4), 20)
+    q, dq, pos = randn(g, 2, 9, 3, 20), randn(g, 2, 9, 3, 20), torch.rand(9, 2, generator=g, device="cuda") * 50
+    cq = randn(g, 2, 9, 3, 20)
+    f = lambda t: float((rotary_axes(t, None, pos, plan).double() * cq).sum())
+    q.requires_grad_()
+    (grad,) = torch.autograd.grad(rotary_axes(q, None, pos, plan), q, cq)
+    e = 2.0 ** -6
+    with torch.no_grad():
+        diff = (f(q + e * dq) - f(q - e * dq)) / (2 * e)
+    assert abs(diff - float((grad.double() * dq).sum())) < 2.0 ** -9 * float((cq * dq).abs().sum())
+    for kind in ("layer", "rms"):
+        t = {n: randn(g, *s) for n, s in dict(x=(3, 7, 48), y=(3, 7, 48), gate=(3, 1, 48), w1=(48,), b1=(48,), w2=(48,), b2=(48,)).items()}
+        ch, cn = randn(g, 3, 7, 48), randn(g, 3, 7, 48)
+        run = lambda t: gated_norm_residual(t["x"], t["y"], gate=t["gate"], post=(t["w1"], t["b1"]), pre=(t["w2"], t["b2"]), kind=kind, alpha=0.9, beta=0.75)
+        f = lambda t: sum(float((a.double() * c).sum()) for a, c in zip(run(t), (ch, cn)))
+        leaves = {n: v.clone().requires_grad_() for n, v in t.items()}
+        grads = dict(zip(t, torch.autograd.grad(run(leaves), list(leaves.values()), (ch, cn))))
+        for name in t:
+            d = randn(g, *t[name].shape)
+            e = 2.0 ** -8
+            diff = (f({**t, name: t[name] + e * d}) - f({**t, name: t[name] - e * d})) / (2 * e)
+            assert abs(diff - float((grads[name].double() * d).sum())) < 2.0 ** -9 * float((grads[name] * d).abs().sum() + ch.abs().sum()), (kind, name)
+
+
+def test_captured_block_follows_its_inputs_over_replays():
+    """Forward and backward of the block in one captured graph: replays with new inputs, eager work and synchronisations in between, bit for bit."""
+    g = gen(23)
+    P, pos = block_inputs(g)
+    plan = block_plan()
+    for t in P.values():
+        t.requires_grad_()
+    dh, dn = randn(g, 2, 145, 256), randn(g, 2, 145, 256, dtype=torch.float16)
+
+    def step():
+        h, n = block(P, pos, plan)
+        return [h.detach(), n.detach(), *torch.autograd.grad((h, n), list(P.values()), (dh, dn))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        with torch.no_grad():
+            P["a"].copy_(randn(g, *P["a"].shape, dtype=torch.float16))
+            P["x"].copy_(randn(g, *P["x"].shape))
+        graph.replay()
+        got = [t.clone() for t in outs]
+        torch.cuda.synchronize()
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), i
+
+
+def test_captured_decode_follows_lengths_and_cache():
+    """Single tokens over a preallocated cache in a captured graph: lengths and cache advance on the device between replays."""
+    from vipformer_amd.ops_block import window_attention
+    g = gen(24)
+    B, cap, Hq, Hk, dh = 3, 9000, 8, 2, 128
+    q = randn(g, B, 1, Hq, dh, dtype=torch.bfloat16)
+    kc, vc = (torch.full((B, cap, Hk, dh), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    lens = torch.tensor([5000, 4097, 100], dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lens.tolist()):
+        kc[b, :n], vc[b, :n] = randn(g, n, Hk, dh, dtype=torch.bfloat16), randn(g, n, Hk, dh, dtype=torch.bfloat16)
+    run = lambda: window_attention(q, kc, vc, (4095, 0), sinks=4, kv_lens=lens)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(4):
+        at = lens.long()
+        for b in range(B):
+            kc[b, at[b]], vc[b, at[b]] = randn(g, Hk, dh, dtype=torch.bfloat16), randn(g, Hk, dh, dtype=torch.bfloat16)
+        q.copy_(randn(g, B, 1, Hq, dh, dtype=torch.bfloat16))
+        lens += 1
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, run())
+        m = seen_mask(B, 1, cap, (4095, 0), 4, None, lens)
+        attention_close(got, *attention_ref(q, kc, vc, m, dh ** -0.5)["out"], "decode")
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams, each with its own inputs, many calls in flight: every result is the one a lone call gives."""
+    from vipformer_amd.ops_block import gated_norm_residual, window_attention
+    g = gen(25)
+    sets = []
+    for _ in range(2):
+        q, k, v = (randn(g, 1, 2000, h, 64, dtype=torch.bfloat16).requires_grad_() for h in (4, 2, 2))
+        x, w = randn(g, 1, 2000, 256).requires_grad_(), randn(g, 256).requires_grad_()
+        sets.append((q, k, v, x, w, randn(g, 1, 2000, 256), randn(g, 1, 1, 4, 64, dtype=torch.bfloat16), randn(g, 1, 20000, 2, 64, dtype=torch.bfloat16)))
+
+    def work(s):
+        q, k, v, x, w, dh, qs, kv = s
+        out = window_attention(q, k, v, (50, 0), sinks=3)
+        h, _ = gated_norm_residual(x, out.flatten(2), gate=w, post=(w, None), kind="rms")
+        return [out.detach(), h.detach(), *torch.autograd.grad(h, (q, k, v, x, w), dh), window_attention(qs, kv, kv, (9999, 0))]
+
+    alone = [work(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(work(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+
+
+def test_expanded_gradients_and_sums():
+    """Gradients that arrive with strides of 0 (a plain .sum()) and through views."""
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    g = gen(26)
+    q = randn(g, 2, 40, 4, 64, dtype=torch.float16).requires_grad_()
+    out = window_attention(q, q, q, (9, 9))
+    (a,) = torch.autograd.grad(out.sum(), q)
+    m = seen_mask(2, 40, 40, (9, 9), 0, None, None)
+    ref = attention_ref(q, q, q, m, 0.125, torch.ones_like(q))
+    # three gradients of one tensor, added in fp16: two more roundings, each half a step of a partial sum
+    extra = sum(ref[n][0].abs() for n in ("dq", "dk", "dv"))
+    d = (a.double() - sum(ref[n][0] for n in ("dq", "dk", "dv"))).abs()
+    assert float((d - 2.0 ** -11 * (3 * extra + 8 * sum(ref[n][1] for n in ("dq", "dk", "dv"))) - 1e-5).max()) <= 0.0
+    plan, pos = RotaryAxes((32,), 64), torch.arange(40, device="cuda")[:, None]
+    (b,) = torch.autograd.grad(rotary_axes(q, None, pos, plan).sum(), q)
+    r, size = rotary_ref(torch.ones_like(q), pos, plan, -1.0)
+    close(b, r, ROT * size, "rotary")
+    x = randn(g, 2, 40, 64).requires_grad_()
+    h, n = gated_norm_residual(x, x.detach(), pre=(None, None))
+    (c,) = torch.autograd.grad(h.sum() + n.transpose(0, 1).sum(), x)
+    one = torch.ones_like(x)
+    ref = norm_ref(x, x.detach(), None, None, (None, None), "layer", 1.0, 1.0, 1e-5, one, one)
+    close(c, ref["dx"][0], BWD_N * ref["dx"][1], "norm")
+
+
+def test_rotary_in_place_through_the_c_abi():
+    """oq = q, ok = k: the same bits as with outputs of their own."""
+    from vipformer_amd import _lib as L, ops_block as O
+    g = gen(27)
+    for layout in ("half", "pair"):
+        plan = O.RotaryAxes((10, 10), 48, layout=layout)
+        q, k, pos = randn(g, 2, 300, 6, 48, dtype=torch.bfloat16), randn(g, 2, 300, 2, 48, dtype=torch.bfloat16), torch.rand(300, 2, generator=g, device="cuda") * 9
+        oq, ok = O.rotary_axes(q, k, pos, plan)
+        freq, axis = plan.tables(q.device)
+        s = O._strides(q) + O._strides(k)
+        L.launch("vpf_rotary_axes", O._pack_rotary(2, 300, 6, 2, 48, 20, 2, plan.layout_code, 2, 0, 0, 0, q.data_ptr(), k.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                                   *s, *s, pos.data_ptr(), 0, freq.data_ptr(), axis.data_ptr()), q.device)
+        assert torch.equal(q, oq) and torch.equal(k, ok)
+
+
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^32 bytes (and elements): a cache of 2.1 million tokens, as many tokens to rotate and to norm."""
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    g = gen(28)
+    n, dt = (1 << 21) + 5, torch.bfloat16
+    k, v = (torch.empty(1, n, 8, 128, dtype=dt, device="cuda") for _ in range(2))
+    tail = slice(n - 3100, n)
+    for t in (k, v):
+        t.fill_(float("nan"))
+        t[:, tail], t[:, :4] = randn(g, 1, 3100, 8, 128, dtype=dt), randn(g, 1, 4, 8, 128, dtype=dt)
+    q = randn(g, 1, 2, 16, 128, dtype=dt)
+    out = window_attention(q, k, v, (3000, 0), sinks=4)
+    cat = lambda t: torch.cat([t[:, :4], t[:, tail]], 1)
+    p = torch.arange(2)[:, None] + 3102
+    j = torch.arange(3104)[None]
+    m = ((j <= p) & ((j >= p - 3000) | (j < 4)))[None].cuda()
+    attention_close(out, *attention_ref(q, cat(k), cat(v), m, 128 ** -0.5)["out"], "cache")
+    k[:, :-16] = 0.5
+    plan, pos = RotaryAxes((64,), 128), torch.arange(n, device="cuda", dtype=torch.int32)[:, None]
+    r = rotary_axes(k, None, pos, plan)
+    ref, size = rotary_ref(k[:, -16:], pos[-16:], plan)
+    close(r[:, -16:], ref, ROT * size, "rotary")
+    del r, v
+    x = k.view(n, 1024)
+    h, nn = gated_norm_residual(x, x, pre=(None, None), kind="rms")
+    ref = norm_ref(x[-16:], x[-16:], None, None, (None, None), "rms", 1.0, 1.0, 1e-5, x[-16:], x[-16:])
+    close(h[-16:], ref["h"][0], FWD_N * ref["h"][1], "h")
+    close(nn[-16:], ref["n"][0], FWD_N * ref["n"][1], "n")

@@ -7,7 +7,9 @@ LayerNorm and residual pieces of ops.py:
 
 Heads are a dimension of their own ([B, L, heads, head_dim], any strides whose last dimension is contiguous: slices of one projection's
 output go in as they are).  fp16 and bf16 are chosen by the tensors, per call; the library's build-time operand type does not matter here.
-Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once, and may be captured into a HIP graph.
+Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once, and may be captured into a HIP graph once
+it has run there (a RotaryAxes makes its tables at its first use on a device).  As everywhere in torch, a backward pass is captured only while no
+eager graph of the same leaves is alive (train.GraphedStep).
 """
 from __future__ import annotations
 
@@ -200,6 +202,8 @@ class GatedNormFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = ctx.cfg
         dev, D = x.device, x.shape[-1]
+        if x.numel() == 0:
+            return (None, *(torch.zeros_like(t) if t is not None and n else None for t, n in zip((x, y, gate, *params), need[1:])))
         dh = dh.contiguous()
         dn = None if dn is None else dn.contiguous()
         dx = torch.empty_like(x) if need[1] else None
