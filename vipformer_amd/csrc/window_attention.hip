@@ -338,14 +338,13 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 #pragma unroll
                 for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s[kb]);
             }
-            if (pad || !wa_all(w, span, x0, SUBK, wmin, wmax)) {
 #pragma unroll
-                for (int kb = 0; kb < NB; ++kb) {
+            for (int kb = 0; kb < NB; ++kb)
+                if (pad || !wa_all(w, span, x0 + 32 * kb, 32, wmin, wmax)) {
                     uint32_t see = wa_visible(span, x0 + 32 * kb, pos + a.right, pos - a.left, a.sinks);
                     if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + kb];
                     wa_hide(s[kb], see, hl);
                 }
-            }
             float mx = s[0][0];
 #pragma unroll
             for (int kb = 0; kb < NB; ++kb)
@@ -736,7 +735,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
         const int* sp = reinterpret_cast<const int*>(stats + (t & 1) * 3 * ROWS + 2 * ROWS + 32 * qs);
         const int rlo = block(t) + 32 * qs;
         const int pmin = seen.off + wa_query(w, rlo), pmax = seen.off + wa_query(w, rlo + 31);      // (rows behind the last one: no harm)
-        if (rlo < rr.hi && rlo + 32 > rr.lo && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
+        if (rlo < rr.hi && rlo + 32 > rr.lo && !(far && kmin >= a.sinks) && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
@@ -806,9 +805,9 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
         }
     }
     if (qs != 0) return;
-    if (kt < w.sink_tiles && w.chunks > 0) {                                 // one of the pieces of a tile with first tokens
-        const size_t piece = ((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1) + (far ? chunk + 1 : 0);
-        float* part = a.ws + wa_delta_floats(w) + (piece * KT + 32 * kb + (lane & 31)) * 2 * DP;
+    if (w.chunks > 0 && key < a.sinks) {                                     // a first token: one of the pieces of its sum
+        const size_t piece = (size_t)bh * (w.chunks + 1) + (far ? chunk + 1 : 0);
+        float* part = a.ws + wa_delta_floats(w) + (piece * a.sinks + key) * 2 * DP;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -819,6 +818,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
             }
         return;
     }
+    if (far) return;
     if (key >= a.Lkv) return;
     T* okp = (T*)a.dk + b * a.dk_sb + key * a.dk_sl + hk * a.dk_sh;
     T* ovp = (T*)a.dv + b * a.dv_sb + key * a.dv_sl + hk * a.dv_sh;
@@ -833,16 +833,17 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
         }
 }
 
-// pieces of the key tiles with first tokens -> dk, dv: one workgroup per key and (sample, key head)
+// pieces of the first tokens' sums -> dk, dv: one workgroup per first token and (sample, key head)
 template <typename T, int DP>
 __global__ void __launch_bounds__(2 * DP) wa_sink_join_kernel(WaArgs w)
 {
     const VpfWindowAttn& a = w.a;
-    const int KT = w.key_tile, per = min(w.sink_tiles * KT, a.Lkv), bh = blockIdx.x / per, key = blockIdx.x % per, kt = key / KT, d = threadIdx.x % DP;
+    const int bh = blockIdx.x / a.sinks, key = blockIdx.x % a.sinks, d = threadIdx.x % DP;
     const bool is_v = threadIdx.x >= DP;
-    const float* p = a.ws + wa_delta_floats(w) + ((((size_t)bh * w.sink_tiles + kt) * (w.chunks + 1)) * KT + key % KT) * 2 * DP + threadIdx.x;
+    const float* p = a.ws + wa_delta_floats(w) + ((size_t)bh * (w.chunks + 1) * a.sinks + key) * 2 * DP + threadIdx.x;
     float s = 0.f;
-    for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * KT * 2 * DP];
+#pragma unroll 4
+    for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * a.sinks * 2 * DP];
     if (d >= a.head_dim) return;
     const int b = bh / a.Hk, hk = bh % a.Hk;
     if (is_v) ((T*)a.dv)[b * a.dv_sb + key * a.dv_sl + hk * a.dv_sh + d] = (T)s;
@@ -924,7 +925,7 @@ static void wa_plan_bwd(WaArgs& w)
 }
 static long wa_bwd_ws(const WaArgs& w)
 {
-    return (long)wa_delta_floats(w) + (w.chunks ? (long)w.a.B * w.a.Hk * w.sink_tiles * (w.chunks + 1) * w.key_tile * 2 * wa_dp(w.a.head_dim) : 0);
+    return (long)wa_delta_floats(w) + (w.chunks ? (long)w.a.B * w.a.Hk * (w.chunks + 1) * w.a.sinks * 2 * wa_dp(w.a.head_dim) : 0);
 }
 
 // more than 64 KB of LDS has to be asked for, once per kernel and device
@@ -989,8 +990,7 @@ template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
     if constexpr (DP == 128) { if (w.key_tile == 128) { if (const int rc = launch(wa_dkv_kernel<T, DP, 4>, 4, done4)) return rc; } }
     if (w.key_tile == 64) { if (const int rc = launch(wa_dkv_kernel<T, DP, 2>, 2, done2)) return rc; }
     if (w.chunks) {
-        const int per = w.sink_tiles * w.key_tile < w.a.Lkv ? w.sink_tiles * w.key_tile : w.a.Lkv;
-        hipLaunchKernelGGL((wa_sink_join_kernel<T, DP>), dim3((unsigned)(bh * per)), dim3(2 * DP), 0, st, w);
+        hipLaunchKernelGGL((wa_sink_join_kernel<T, DP>), dim3((unsigned)(bh * w.a.sinks)), dim3(2 * DP), 0, st, w);
     }
     VPF_CHECK_LAUNCH();
     return VPF_OK;
