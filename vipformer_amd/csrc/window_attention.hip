@@ -182,7 +182,8 @@ __device__ __forceinline__ void wa_dma_any(const void* p, uint32_t lds_byte)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds_byte), "v"(p) : "memory", "m0");
 }
 #pragma clang diagnostic pop
-__device__ __forceinline__ void wa_stage_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// waits for this wave's loads but the N youngest (they retire in order)
+template <int N> __device__ __forceinline__ void wa_stage_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 template <int DP, int ROWS, int NW = 4> struct WaStage {
     static constexpr int PITCH = WaTile<DP>::PITCH, ALL = NW * 1024, PER = ROWS * PITCH / ALL, STEP = ALL / PITCH;      // wave instructions of one tile per wave
     static_assert(ROWS * PITCH % ALL == 0 && STEP % 16 == 0, "a stage is whole instructions of all waves, whole periods of the swizzle apart");
@@ -254,14 +255,17 @@ __device__ __forceinline__ void wa_hide(wa_f32x16& s, uint32_t visible, int hl)
 }
 
 // ------------------------------------------------------------------ forward
-// Workgroup = 4 waves = RB blocks of 32 rows x KS parts of a stage's keys (SUBK each); K and V are double-buffered in LDS, the loads of the
-// next stage are in flight during the products of this one.  splits > 1: the stages of a row tile are divided over workgroups, whose
+// Workgroup = 4 waves = RB groups of RW blocks of 32 rows x KS parts of a stage's keys (SUBK each); K and V are double-buffered in LDS, the loads of
+// the next stage are in flight during the products of this one.  At RW = 1 every fragment of K and V that comes from LDS serves one matrix
+// instruction, which keeps the LDS as busy as the matrix cores; at RW = 2 it serves two.  The priority is up around the products, so that the two
+// waves of a SIMD fall out of step and one's softmax runs beside the other's products (4 - 5 %).  splits > 1: the stages of a row tile are divided over workgroups, whose
 // (maximum, sum, unnormalised output) wa_join_kernel joins.
-template <typename T, int DP, int RB, int KS, int SUBK>
+template <typename T, int DP, int RB, int RW, int KS, int SUBK>
 __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
-    constexpr int STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
+    constexpr int STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, KG = RW == 1 ? NB : 1, BUF = STAGE * Tile::PITCH, WR = 32 * RW;
+    constexpr bool DEEP = KS == 4;                                           // few rows: the loads are what takes time
     extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][K, V][STAGE rows], pads
     const VpfWindowAttn& a = w.a;
     uint32_t* const pads = reinterpret_cast<uint32_t*>(lds + 4 * BUF);     // [2][STAGE / 32]: a bit for every key that is not padding
@@ -270,115 +274,156 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     wa_item(w, bh, tile, split);
     const int b = bh / a.Hk, hk = bh % a.Hk;
     const WaSeen seen = wa_seen(w, b);
-    const int r0 = tile * 32 * RB, rend = min(r0 + 32 * RB, w.rows);
+    const int r0 = tile * WR * RB, rend = min(r0 + WR * RB, w.rows);
     const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1));
     const int stages = (span.total + STAGE - 1) / STAGE, t0 = (int)((long)stages * split / w.splits), t1 = (int)((long)stages * (split + 1) / w.splits);
 
-    // this lane's row
-    const int row = r0 + rb * 32 + (lane & 31), rq = min(row, w.rows - 1), qi = wa_query(w, rq);
-    const int pos = seen.off + qi, wlast = min(r0 + rb * 32 + 31, w.rows - 1);
-    const bool live = r0 + rb * 32 < w.rows;
-    const int wmin = seen.off + wa_query(w, min(r0 + rb * 32, w.rows - 1)), wmax = seen.off + wa_query(w, wlast);
-    typename WaMma<T>::v8 qf[KST];
-    {
+    // this lane's rows: one of each of the wave's RW blocks
+    const int wrow = r0 + rb * WR;
+    const bool live = wrow < w.rows;
+    const int wmin = seen.off + wa_query(w, min(wrow, w.rows - 1)), wmax = seen.off + wa_query(w, min(wrow + WR - 1, w.rows - 1));
+    auto row_of = [&](int j) { return wrow + 32 * j + (lane & 31); };
+    int pos[RW];
+    typename WaMma<T>::v8 qf[RW][KST];
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+        const int rq = min(row_of(j), w.rows - 1), qi = wa_query(w, rq);
+        pos[j] = seen.off + qi;
         const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + (hk * w.g + (rq - qi * w.g)) * a.q_sh;
 #pragma unroll
         for (int s = 0; s < KST; ++s) {
             const int d = 16 * s + 8 * hl;
             uint4 u = make_uint4(0, 0, 0, 0);
             if (d < a.head_dim) u = *reinterpret_cast<const uint4*>(qp + d);
-            qf[s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
+            qf[j][s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
         }
     }
     const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
     const char* vp = (const char*)((const T*)a.v + b * a.v_sb + hk * a.v_sh);
     const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
 
-    wa_f32x16 o[DT];
+    wa_f32x16 o[RW][DT];
+    float m[RW], l[RW];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = wa_zero16();
-    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < RW; ++j) {
+        m[j] = -INFINITY; l[j] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[j][dt] = wa_zero16();
+    }
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
-    bool kept = false;
     auto load = [&](int t) {
         const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
         const long kst = a.k_sl * (long)sizeof(T), vst = a.v_sl * (long)sizeof(T);
         if (pad || x0 < span.first) {
             auto key = [&](int r) { return (long)(x0 + r < span.first ? x0 + r : x0 + r + span.shift); };
+            if (pad) {
+                const uint64_t kept = __ballot((int)threadIdx.x <= last && !pad[key(min((int)threadIdx.x, last))]);      // threads 64 i ..: entries 64 i ..
+                if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[(t & 1) * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(kept >> (32 * lane));
+            }
             // a key that nobody here sees must not reach the product with V: 0 * NaN is NaN
             stage.rows_of(kp, kst, last, key, nullptr, at);
             stage.rows_of(vp, vst, last, key, pad, at + BUF);
-            if (pad) kept = (int)threadIdx.x <= last && !pad[key(threadIdx.x)];
         } else {
             stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
             stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
         }
     };
-    auto store = [&](int buf) {
-        if (pad) {
-            const uint64_t bits = __ballot(kept);                            // threads 64 i .. hold entries 64 i .. of the stage
-            if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[buf * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(bits >> (32 * lane));
-        }
-        wa_stage_wait();
-    };
-    if (t0 < t1) { load(t0); store(t0 & 1); }
-    __syncthreads();
+    if (t0 < t1) load(t0);
+    if (DEEP && t0 + 1 < t1) load(t0 + 1);
+    if (!DEEP) { wa_stage_wait<0>(); __syncthreads(); }
     for (int t = t0; t < t1; ++t) {
-        if (t + 1 < t1) load(t + 1);
+        if (DEEP) {                                                          // two stages in flight; this one's loads are the older ones
+            if (t + 1 < t1) wa_stage_wait<2 * WaStage<DP, STAGE>::PER>();
+            else wa_stage_wait<0>();
+            __syncthreads();
+        } else if (t + 1 < t1) load(t + 1);
         const int x0 = t * STAGE + ks * SUBK;
         const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), vcol = wa_opaque(col_base + sk + BUF);
-        if (live && !wa_none(w, span, x0, SUBK, wmin, wmax)) {
-            wa_f32x16 s[NB];
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) {
-                s[kb] = wa_zero16();
+        for (int k0 = 0; k0 < NB; k0 += KG) {
+            const int xg = x0 + 32 * k0;
+            if (!live || wa_none(w, span, xg, 32 * KG, wmin, wmax)) continue;
+            wa_f32x16 s[RW][KG];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int i = 0; i < KST; ++i) s[kb] = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s[kb]);
-            }
+            for (int kb = 0; kb < KG; ++kb) {
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb)
-                if (pad || !wa_all(w, span, x0 + 32 * kb, 32, wmin, wmax)) {
-                    uint32_t see = wa_visible(span, x0 + 32 * kb, pos + a.right, pos - a.left, a.sinks);
-                    if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + kb];
-                    wa_hide(s[kb], see, hl);
+                for (int j = 0; j < RW; ++j) s[j][kb] = wa_zero16();
+#pragma unroll
+                for (int i = 0; i < KST; ++i) {
+                    const typename WaMma<T>::v8 kf = wa_frag_row<T>(krow, i, 32 * (k0 + kb) * Tile::PITCH);
+#pragma unroll
+                    for (int j = 0; j < RW; ++j) s[j][kb] = WaMma<T>::mma(kf, qf[j][i], s[j][kb]);
                 }
-            float mx = s[0][0];
+            }
+            __builtin_amdgcn_s_setprio(0);
+            if (pad || !wa_all(w, span, xg, 32 * KG, wmin, wmax)) {
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb)
+                for (int j = 0; j < RW; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-            mx = wa_half_max(mx) * w.c;
+                    for (int kb = 0; kb < KG; ++kb) {
+                        uint32_t see = wa_visible(span, xg + 32 * kb, pos[j] + a.right, pos[j] - a.left, a.sinks);
+                        if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + k0 + kb];
+                        wa_hide(s[j][kb], see, hl);
+                    }
+            }
+            float mx[RW];
+            bool grown = false;
+#pragma unroll
+            for (int j = 0; j < RW; ++j) {
+                mx[j] = s[j][0][0];
+#pragma unroll
+                for (int kb = 0; kb < KG; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mx[j] = fmaxf(mx[j], s[j][kb][r]);
+                mx[j] = wa_half_max(mx[j]) * w.c;
+                grown = grown || mx[j] > m[j] + 8.f;
+            }
             // The running maximum only has to keep exp2 in range: it moves when a row has outgrown it by 2^8 (weights up to 256 fit every type)
-            if (__any(mx > m + 8.f)) {
-                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : wa_exp2(m - mn);
-                m = mn;
-                l *= f;
+            if (__any(grown)) {
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+                for (int j = 0; j < RW; ++j) {
+                    const float mn = fmaxf(m[j], mx[j]), f = m[j] == -INFINITY ? 0.f : wa_exp2(m[j] - mn);
+                    m[j] = mn;
+                    l[j] *= f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[dt][r] *= f;
-            }
-            const float base = m == -INFINITY ? 0.f : m;                     // a row that has seen nothing yet: every weight is exp2(-inf)
+                    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb) {
-                float p[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { p[r] = wa_exp2(fmaf(s[kb][r], w.c, -base)); l += p[r]; }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(vcol, dt, (32 * kb + 16 * i) * Tile::PITCH), pf, o[dt]);
+                        for (int r = 0; r < 16; ++r) o[j][dt][r] *= f;
                 }
             }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int kb = 0; kb < KG; ++kb) {
+                typename WaMma<T>::v8 pf[RW][2];
+#pragma unroll
+                for (int j = 0; j < RW; ++j) {
+                    const float base = m[j] == -INFINITY ? 0.f : m[j];       // a row that has seen nothing yet: every weight is exp2(-inf)
+                    float p[16];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) { p[r] = wa_exp2(fmaf(s[j][kb][r], w.c, -base)); l[j] += p[r]; }
+                    pf[j][0] = wa_pack8<T>(p); pf[j][1] = wa_pack8<T>(p + 8);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const typename WaMma<T>::v8 vf = wa_frag_col<T, DP>(vcol, dt, (32 * (k0 + kb) + 16 * i) * Tile::PITCH);
+#pragma unroll
+                        for (int j = 0; j < RW; ++j) o[j][dt] = WaMma<T>::mma(vf, pf[j][i], o[j][dt]);
+                    }
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
-        if (t + 1 < t1) store((t + 1) & 1);
-        __syncthreads();
+        if (!DEEP) { wa_stage_wait<0>(); __syncthreads(); }
+        else if (t + 2 < t1) { __syncthreads(); load(t + 2); }
     }
-    if (KS > 1) {                                                            // join the key parts through LDS (the stages are done with)
+    if (DEEP) __syncthreads();
+    static_assert(KS == 1 || RW == 1, "parts of the keys are joined for one row block");
+    if constexpr (KS > 1) {                                                            // join the key parts through LDS (the stages are done with)
         float* slots = reinterpret_cast<float*>(lds);
         constexpr int SLOT = (DT * 16 + 2) * 64;
         static_assert((KS / 2) * RB * SLOT * 4 <= 4 * BUF, "the partial results fit the stage buffers");
@@ -389,26 +434,31 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) slot[(dt * 16 + r) * 64] = o[dt][r];
-                slot[DT * 16 * 64] = m; slot[(DT * 16 + 1) * 64] = l;
+                    for (int r = 0; r < 16; ++r) slot[(dt * 16 + r) * 64] = o[0][dt][r];
+                slot[DT * 16 * 64] = m[0]; slot[(DT * 16 + 1) * 64] = l[0];
             }
             __syncthreads();
             if (ks < step) {
                 const float* slot = slots + (ks * RB + rb) * SLOT + lane;
-                const float m2 = slot[DT * 16 * 64], mn = fmaxf(m, m2);
-                const float f1 = m == -INFINITY ? 0.f : wa_exp2(m - mn), f2 = m2 == -INFINITY ? 0.f : wa_exp2(m2 - mn);
-                l = l * f1 + slot[(DT * 16 + 1) * 64] * f2;
-                m = mn;
+                const float m2 = slot[DT * 16 * 64], mn = fmaxf(m[0], m2);
+                const float f1 = m[0] == -INFINITY ? 0.f : wa_exp2(m[0] - mn), f2 = m2 == -INFINITY ? 0.f : wa_exp2(m2 - mn);
+                l[0] = l[0] * f1 + slot[(DT * 16 + 1) * 64] * f2;
+                m[0] = mn;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * f1 + slot[(dt * 16 + r) * 64] * f2;
+                    for (int r = 0; r < 16; ++r) o[0][dt][r] = o[0][dt][r] * f1 + slot[(dt * 16 + r) * 64] * f2;
             }
             if (step > 1) __syncthreads();
         }
     }
-    if (ks != 0 || row >= w.rows) return;
-    l = wa_half_sum(l);
+    if (ks != 0) return;
+#pragma unroll
+    for (int jr = 0; jr < RW; ++jr) {
+    const int row = row_of(jr);
+    if (row >= w.rows) return;
+    const int qi = wa_query(w, row);
+    const float lr = wa_half_sum(l[jr]), mr = m[jr];
     if (w.splits > 1) {
         const size_t at = ((size_t)split * a.B * a.Hk + bh) * w.rows + row;
         float* part = a.ws + at * DP;
@@ -416,18 +466,18 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(part + 32 * dt + 8 * j + 4 * hl) = make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
-        if (hl == 0) reinterpret_cast<float2*>(a.ws + (size_t)w.splits * a.B * a.Hk * w.rows * DP)[at] = make_float2(m, l);
-        return;
+                *reinterpret_cast<float4*>(part + 32 * dt + 8 * j + 4 * hl) = make_float4(o[jr][dt][4 * j], o[jr][dt][4 * j + 1], o[jr][dt][4 * j + 2], o[jr][dt][4 * j + 3]);
+        if (hl == 0) reinterpret_cast<float2*>(a.ws + (size_t)w.splits * a.B * a.Hk * w.rows * DP)[at] = make_float2(mr, lr);
+        continue;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* op = (T*)a.out + b * a.o_sb + qi * a.o_sl + (hk * w.g + (rq - qi * w.g)) * a.o_sh;
+    const float inv = lr == 0.f ? 0.f : 1.f / lr;
+    T* op = (T*)a.out + b * a.o_sb + qi * a.o_sl + (hk * w.g + (row - qi * w.g)) * a.o_sh;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int d = 32 * dt + 8 * j + 4 * hl;
-            const float v[4] = {o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv, o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv};
+            const float v[4] = {o[jr][dt][4 * j] * inv, o[jr][dt][4 * j + 1] * inv, o[jr][dt][4 * j + 2] * inv, o[jr][dt][4 * j + 3] * inv};
             if (d < a.head_dim) {
                 vpf_store<T, 4>(op + d, v);
                 if (a.out_lo) {
@@ -436,7 +486,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
                 }
             }
         }
-    if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = l == 0.f ? INFINITY : m + log2f(l);
+    if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = lr == 0.f ? INFINITY : mr + log2f(lr);
+    }
 }
 
 // parts of the keys -> output: one wave per row.  Lane i holds maximum and sum of part i (splits <= 64); the channels' loads of 4 parts are in
@@ -532,30 +583,25 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
-    bool kept = false;
     auto load = [&](int t) {
         const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
         const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
         const long kst = a.k_sl * (long)sizeof(T), vst = a.v_sl * (long)sizeof(T);
         if (pad || x0 < span.first) {
             auto key = [&](int r) { return (long)(x0 + r < span.first ? x0 + r : x0 + r + span.shift); };
+            if (pad) {
+                const uint64_t kept = __ballot((int)threadIdx.x <= last && !pad[key(min((int)threadIdx.x, last))]);      // threads 64 i ..: entries 64 i ..
+                if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[(t & 1) * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(kept >> (32 * lane));
+            }
             // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
             stage.rows_of(kp, kst, last, key, pad, at);
             stage.rows_of(vp, vst, last, key, nullptr, at + BUF);
-            if (pad) kept = (int)threadIdx.x <= last && !pad[key(threadIdx.x)];
         } else {
             stage.rows(kp + (x0 + span.shift) * kst, (uint32_t)kst, last, at);
             stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
         }
     };
-    auto store = [&](int buf) {
-        if (pad) {
-            const uint64_t bits = __ballot(kept);                            // threads 64 i .. hold entries 64 i .. of the stage
-            if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[buf * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(bits >> (32 * lane));
-        }
-        wa_stage_wait();
-    };
-    if (stages > 0) { load(0); store(0); }
+    if (stages > 0) { load(0); wa_stage_wait<0>(); }
     __syncthreads();
     for (int t = 0; t < stages; ++t) {
         if (t + 1 < stages) load(t + 1);
@@ -565,12 +611,14 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
         for (int kb = 0; kb < NB; ++kb) {
             const int xb = x0 + 32 * kb;
             if (!live || wa_none(w, span, xb, 32, wmin, wmax)) continue;
+            __builtin_amdgcn_s_setprio(1);
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
                 s = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH), qf[i], s);
                 dp = WaMma<T>::mma(wa_frag_row<T>(krow, i, 32 * kb * Tile::PITCH + BUF), gf[i], dp);
             }
+            __builtin_amdgcn_s_setprio(0);
             const bool all = !pad && wa_all(w, span, xb, 32, wmin, wmax);
             if (!all) {
                 uint32_t see = wa_visible(span, xb, pos + a.right, pos - a.left, a.sinks);
@@ -591,7 +639,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
                 for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(kcol, dt, (32 * kb + 16 * i) * Tile::PITCH), df, dq[dt]);
             }
         }
-        if (t + 1 < stages) store((t + 1) & 1);
+        wa_stage_wait<0>();
         __syncthreads();
     }
     if (KS > 1) {
@@ -725,7 +773,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
     int top = b_hi - 1;
     { const int c = (top + 1) / w.cycle * w.cycle - 1; if (c >= b_lo) top = c; }
     auto block = [&](int t) { const int i = top - t; return (i < b_lo ? i + steps : i) * ROWS; };
-    if (steps > 0) { load(block(0), 0); wa_stage_wait(); }
+    if (steps > 0) { load(block(0), 0); wa_stage_wait<0>(); }
     __syncthreads();
     for (int t = 0; t < steps; ++t) {
         if (t + 1 < steps) load(block(t + 1), (t + 1) & 1);
@@ -736,6 +784,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
         const int rlo = block(t) + 32 * qs;
         const int pmin = seen.off + wa_query(w, rlo), pmax = seen.off + wa_query(w, rlo + 31);      // (rows behind the last one: no harm)
         if (rlo < rr.hi && rlo + 32 > rr.lo && !(far && kmin >= a.sinks) && pmax >= kmin - a.right && (pmin <= kmax + a.left || kmin < a.sinks)) {
+            __builtin_amdgcn_s_setprio(1);
             wa_f32x16 s = wa_zero16(), dp = wa_zero16();
 #pragma unroll
             for (int i = 0; i < KST; ++i) {
@@ -743,6 +792,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
                 if constexpr (VREG) dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), vf[i], dp);
                 else dp = WaMma<T>::mma(wa_frag_row<T>(qrow, i, BUF), wa_frag_row<T>(vrow, i, 0), dp);
             }
+            __builtin_amdgcn_s_setprio(0);
             const bool all = whole && rlo >= rr.lo && rlo + 32 <= rr.hi && kmax <= pmin + a.right && (kmin >= pmax - a.left || kmax < a.sinks);
             float p[16], ds[16];
 #pragma unroll
@@ -780,7 +830,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
                 }
             }
         }
-        wa_stage_wait();
+        wa_stage_wait<0>();
         __syncthreads();
     }
     // the two halves of the rows: through LDS, dV first
@@ -851,6 +901,7 @@ __global__ void __launch_bounds__(2 * DP) wa_sink_join_kernel(WaArgs w)
 }
 
 // ------------------------------------------------------------------ host
+static long wa_min(long a, long b) { return a < b ? a : b; }
 static int wa_dp(int dh) { return dh <= 32 ? 32 : dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 
 static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
@@ -892,6 +943,11 @@ static int wa_runs(const WaArgs& w) { return (long)w.a.B * w.a.Hk < 8 && ((long)
 static void wa_plan_fwd(WaArgs& w, int& rb)
 {
     rb = wa_row_blocks(w);
+    // Two row blocks a wave (256 rows a workgroup) from head dimension 72 on, where the walk over the keys is long beside the queries of a tile
+    // (bf16, left window + causal; one / two blocks, us: dim 128, 4 heads a key, window 256 181 / 182, 512 245 / 241, 1024 383 / 368, 4096 1220 / 1137;
+    // dim 96, 1 head, 4096 278 / 246; dim 64, 1 head, 4096 173 / 186, which the exponentials bound, not the LDS).
+    const long seen = wa_min((long)w.a.left + w.a.right + 1, (long)w.a.Lkv);
+    if (rb == 4 && w.a.head_dim > 64 && seen * w.g >= 16 * 256 && (long)w.a.B * w.a.Hk * vpf_cdiv(w.rows, 256) >= 256) rb = 8;
     w.tiles = vpf_cdiv(w.rows, 32 * rb);
     w.splits = 1;
     const long wgs = (long)w.a.B * w.a.Hk * w.tiles;
@@ -937,23 +993,24 @@ template <typename K> static int wa_lds(K kernel, size_t bytes, VpfPerDevice& do
     return VPF_OK;
 }
 
-template <typename T, int DP, int RB, int KS, int SUBK> static int wa_launch_fwd(const WaArgs& w, hipStream_t st)
+template <typename T, int DP, int RB, int RW, int KS, int SUBK> static int wa_launch_fwd(const WaArgs& w, hipStream_t st)
 {
     constexpr size_t lds = 4 * SUBK * KS * WaTile<DP>::PITCH + SUBK * KS / 4;
     static VpfPerDevice done;
-    if (const int rc = wa_lds(wa_fwd_kernel<T, DP, RB, KS, SUBK>, lds, done)) return rc;
+    if (const int rc = wa_lds(wa_fwd_kernel<T, DP, RB, RW, KS, SUBK>, lds, done)) return rc;
     const long grid = (long)w.a.B * w.a.Hk * w.tiles * w.splits;
     if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
-    hipLaunchKernelGGL((wa_fwd_kernel<T, DP, RB, KS, SUBK>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
+    hipLaunchKernelGGL((wa_fwd_kernel<T, DP, RB, RW, KS, SUBK>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
     if (w.splits > 1) hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3(vpf_cdiv((long)w.a.B * w.a.Hk * w.rows, 4)), dim3(WA_THREADS), 0, st, w);
     VPF_CHECK_LAUNCH();
     return VPF_OK;
 }
 template <typename T, int DP> static int wa_fwd(const WaArgs& w, int rb, hipStream_t st)
 {
-    if (rb == 4) return wa_launch_fwd<T, DP, 4, 1, 64>(w, st);
-    if (rb == 2) return wa_launch_fwd<T, DP, 2, 2, 32>(w, st);
-    return wa_launch_fwd<T, DP, 1, 4, 32>(w, st);
+    if constexpr (DP > 64) { if (rb == 8) return wa_launch_fwd<T, DP, 4, 2, 1, 64>(w, st); }
+    if (rb == 4) return wa_launch_fwd<T, DP, 4, 1, 1, 64>(w, st);
+    if (rb == 2) return wa_launch_fwd<T, DP, 2, 1, 2, 32>(w, st);
+    return wa_launch_fwd<T, DP, 1, 1, 4, 32>(w, st);
 }
 
 template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaArgs& w, hipStream_t st)
