@@ -278,38 +278,9 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     const WaSpan span = wa_span(w, seen, seen.off + wa_query(w, r0), seen.off + wa_query(w, rend - 1));
     const int stages = (span.total + STAGE - 1) / STAGE, t0 = (int)((long)stages * split / w.splits), t1 = (int)((long)stages * (split + 1) / w.splits);
 
-    // this lane's rows: one of each of the wave's RW blocks
-    const int wrow = r0 + rb * WR;
-    const bool live = wrow < w.rows;
-    const int wmin = seen.off + wa_query(w, min(wrow, w.rows - 1)), wmax = seen.off + wa_query(w, min(wrow + WR - 1, w.rows - 1));
-    auto row_of = [&](int j) { return wrow + 32 * j + (lane & 31); };
-    int pos[RW];
-    typename WaMma<T>::v8 qf[RW][KST];
-#pragma unroll
-    for (int j = 0; j < RW; ++j) {
-        const int rq = min(row_of(j), w.rows - 1), qi = wa_query(w, rq);
-        pos[j] = seen.off + qi;
-        const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + (hk * w.g + (rq - qi * w.g)) * a.q_sh;
-#pragma unroll
-        for (int s = 0; s < KST; ++s) {
-            const int d = 16 * s + 8 * hl;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (d < a.head_dim) u = *reinterpret_cast<const uint4*>(qp + d);
-            qf[j][s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
-        }
-    }
     const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
     const char* vp = (const char*)((const T*)a.v + b * a.v_sb + hk * a.v_sh);
     const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
-
-    wa_f32x16 o[RW][DT];
-    float m[RW], l[RW];
-#pragma unroll
-    for (int j = 0; j < RW; ++j) {
-        m[j] = -INFINITY; l[j] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[j][dt] = wa_zero16();
-    }
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
@@ -333,6 +304,35 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
     };
     if (t0 < t1) load(t0);
     if (DEEP && t0 + 1 < t1) load(t0 + 1);
+    // this lane's rows: one of each of the wave's RW blocks
+    const int wrow = r0 + rb * WR;
+    const bool live = wrow < w.rows;
+    const int wmin = seen.off + wa_query(w, min(wrow, w.rows - 1)), wmax = seen.off + wa_query(w, min(wrow + WR - 1, w.rows - 1));
+    auto row_of = [&](int j) { return wrow + 32 * j + (lane & 31); };
+    int pos[RW];
+    typename WaMma<T>::v8 qf[RW][KST];
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+        const int rq = min(row_of(j), w.rows - 1), qi = wa_query(w, rq);
+        pos[j] = seen.off + qi;
+        const T* qp = (const T*)a.q + b * a.q_sb + qi * a.q_sl + (hk * w.g + (rq - qi * w.g)) * a.q_sh;
+#pragma unroll
+        for (int s = 0; s < KST; ++s) {
+            const int d = 16 * s + 8 * hl;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (d < a.head_dim) u = *reinterpret_cast<const uint4*>(qp + d);
+            qf[j][s] = __builtin_bit_cast(typename WaMma<T>::v8, u);
+        }
+    }
+    wa_f32x16 o[RW][DT];
+    float m[RW], l[RW];
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+        m[j] = -INFINITY; l[j] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[j][dt] = wa_zero16();
+    }
+
     if (!DEEP) { wa_stage_wait<0>(); __syncthreads(); }
     for (int t = t0; t < t1; ++t) {
         if (DEEP) {                                                          // two stages in flight; this one's loads are the older ones
@@ -807,16 +807,24 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
                 }
             }
             if (!all) {
+                const bool cut = rlo < rr.lo || rlo + 32 > rr.hi;            // (uniform) rows outside the range: another workgroup's, or none
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int4 po = *reinterpret_cast<const int4*>(sp + 4 * hl + 8 * j);
                     const int ps[4] = {po.x, po.y, po.z, po.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * j + e;
-                        const bool see = (uint32_t)(ps[e] - see_from) <= see_n && (uint32_t)(rlo - rr.lo + 4 * hl + 8 * j + e) < (uint32_t)(rr.hi - rr.lo);
-                        p[r] = see ? p[r] : 0.f;
-                        ds[r] = see ? ds[r] : 0.f;
+                        const bool see = (uint32_t)(ps[e] - see_from) <= see_n;
+                        p[4 * j + e] = see ? p[4 * j + e] : 0.f;
+                        ds[4 * j + e] = see ? ds[4 * j + e] : 0.f;
+                    }
+                }
+                if (cut) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const bool in = (uint32_t)(rlo - rr.lo + 4 * hl + 8 * (r >> 2) + (r & 3)) < (uint32_t)(rr.hi - rr.lo);
+                        p[r] = in ? p[r] : 0.f;
+                        ds[r] = in ? ds[r] : 0.f;
                     }
                 }
             }
