@@ -525,10 +525,13 @@ __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
 }
 
 // ------------------------------------------------------------------ backward: queries
-// dS = P (dP - delta), dP = dO V^T, delta = rowsum(dO . O);  dQ = scale dS K.  The walk over the keys is the forward kernel's; delta is
-// kept for the kernel of the keys.  dS is rounded to the tensors' type for its product, as P is.  delta takes O as forward had it before
-// rounding (out + out_lo): with the rounded O its error alone is as large as dS's own rounding (error of dq against 64 bits 1.6 instead of 1.4
-// times the output's rounding).
+// dS = P (dP - delta), dP = dO V^T, delta = sum of P dP = rowsum(dO . O);  dQ = scale dS K.  The walk over the keys is the forward kernel's.  dS is
+// rounded to the tensors' type for its product, as P is.
+// delta comes in three qualities.  rowsum(dO . O) is there before the walk, with O as forward had it before rounding (out + out_lo; with the
+// rounded O the error of dq against 64 bits was 1.6 instead of 1.4 times the output's own rounding); what is left in it is the rounding of
+// forward's weights, 1 / sqrt(keys) of dS's own rounding.  Where rows see few keys (WA_FEW) the walk is therefore made twice, first for
+// the sum of P dP in fp32.  That sum is also what a single walk leaves behind for the kernel of the keys.
+#define WA_FEW 64
 template <typename T, int DP, int RB, int KS>
 __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 {
@@ -537,6 +540,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const VpfWindowAttn& a = w.a;
     uint32_t* const pads = reinterpret_cast<uint32_t*>(lds + 4 * BUF);     // [2][STAGE / 32]: a bit for every key that is not padding
+    float* const sums = reinterpret_cast<float*>(pads + 2 * (STAGE / 32));  // [KS][RB][32]: the key parts' sums of P dP
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), hl = lane >> 5, rb = wave % RB, ks = wave / RB;
     int bh, tile, split;
     wa_item(w, bh, tile, split);
@@ -571,7 +575,6 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * ((float)of[i] + (float)ol[i]);
         }
         delta = wa_half_sum(delta);
-        if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
     }
     const float lse = a.lse[(size_t)bh * w.rows + rq];
     const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
@@ -583,15 +586,15 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 
     const WaStage<DP, STAGE> stage(a.head_dim);
     const uint32_t tiles_at = wa_lds_byte(lds), row_base = wa_row_base<DP>(), col_base = wa_col_base<DP>();
-    auto load = [&](int t) {
+    auto load = [&](int t, int buf) {
         const int x0 = t * STAGE, last = min(STAGE, span.total - x0) - 1;
-        const uint32_t at = tiles_at + (t & 1) * 2 * BUF;
+        const uint32_t at = tiles_at + buf * 2 * BUF;
         const long kst = a.k_sl * (long)sizeof(T), vst = a.v_sl * (long)sizeof(T);
         if (pad || x0 < span.first) {
             auto key = [&](int r) { return (long)(x0 + r < span.first ? x0 + r : x0 + r + span.shift); };
             if (pad) {
                 const uint64_t kept = __ballot((int)threadIdx.x <= last && !pad[key(min((int)threadIdx.x, last))]);      // threads 64 i ..: entries 64 i ..
-                if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[(t & 1) * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(kept >> (32 * lane));
+                if (lane < 2 && wave * 2 + lane < STAGE / 32) pads[buf * (STAGE / 32) + wave * 2 + lane] = (uint32_t)(kept >> (32 * lane));
             }
             // a key that nobody here sees must not reach the product with K: 0 * NaN is NaN
             stage.rows_of(kp, kst, last, key, pad, at);
@@ -601,12 +604,30 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             stage.rows(vp + (x0 + span.shift) * vst, (uint32_t)vst, last, at + BUF);
         }
     };
-    if (stages > 0) { load(0); wa_stage_wait<0>(); }
+    // the fewest keys a row here can see (padding aside): at one of the ends of the tile's positions
+    auto keys_of = [&](int p) { const int lo = max(0, p - a.left); return min(p + a.right, seen.n - 1) + 1 - lo + min(a.sinks, lo); };
+    const bool twice = min(keys_of(seen.off + wa_query(w, r0)), keys_of(seen.off + wa_query(w, rend - 1))) <= WA_FEW;
+    const int steps = twice ? 2 * stages : stages;
+    float pdp = 0.f;
+    auto joined = [&](float v) {                                             // over the lane pair and the key parts
+        v = wa_half_sum(v);
+        if constexpr (KS > 1) {
+            if (hl == 0) sums[(ks * RB + rb) * 32 + lane] = v;
+            __syncthreads();
+            v = 0.f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) v += sums[(i * RB + rb) * 32 + (lane & 31)];
+        }
+        return v;
+    };
+    if (stages > 0) { load(0, 0); wa_stage_wait<0>(); }
     __syncthreads();
-    for (int t = 0; t < stages; ++t) {
-        if (t + 1 < stages) load(t + 1);
+    for (int step = 0; step < steps; ++step) {
+        const int t = step < stages ? step : step - stages, next = t + 1 < stages ? t + 1 : 0;
+        const bool first = twice && step < stages;                           // the walk for delta alone
+        if (step + 1 < steps) load(next, (step + 1) & 1);
         const int x0 = t * STAGE + ks * SUBK;
-        const uint32_t sk = tiles_at + (t & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), kcol = wa_opaque(col_base + sk);
+        const uint32_t sk = tiles_at + (step & 1) * 2 * BUF + ks * SUBK * Tile::PITCH, krow = wa_opaque(row_base + sk), kcol = wa_opaque(col_base + sk);
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
             const int xb = x0 + 32 * kb;
@@ -622,16 +643,19 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             const bool all = !pad && wa_all(w, span, xb, 32, wmin, wmax);
             if (!all) {
                 uint32_t see = wa_visible(span, xb, pos + a.right, pos - a.left, a.sinks);
-                if (pad) see &= pads[(t & 1) * (STAGE / 32) + ks * NB + kb];
+                if (pad) see &= pads[(step & 1) * (STAGE / 32) + ks * NB + kb];
                 wa_hide(s, see, hl);
             }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const float p = wa_exp2(fmaf(s[r], w.c, -lse));
-                ds[r] = p * (dp[r] - delta);
-                if (!all) ds[r] = s[r] == -INFINITY ? 0.f : ds[r];           // what a hidden key holds stays out
+                float x = p * dp[r];
+                if (!all) x = s[r] == -INFINITY ? 0.f : x;                   // what a hidden key holds stays out
+                pdp += x;
+                ds[r] = fmaf(-p, delta, x);
             }
+            if (first) continue;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const typename WaMma<T>::v8 df = wa_pack8<T>(ds + 8 * i);
@@ -639,9 +663,12 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
                 for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(kcol, dt, (32 * kb + 16 * i) * Tile::PITCH), df, dq[dt]);
             }
         }
+        if (first && step + 1 == stages) { delta = joined(pdp); pdp = 0.f; }
         wa_stage_wait<0>();
         __syncthreads();
     }
+    if (!twice) delta = joined(pdp);
+    if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
     if (KS > 1) {
         float* slots = reinterpret_cast<float*>(lds);
         constexpr int SLOT = DT * 16 * 64;
@@ -1024,7 +1051,7 @@ template <typename T, int DP> static int wa_fwd(const WaArgs& w, int rb, hipStre
 template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaArgs& w, hipStream_t st)
 {
     constexpr int STAGE = (KS == 1 ? 64 : 32) * KS;
-    constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + STAGE / 4;
+    constexpr size_t lds = 4 * STAGE * WaTile<DP>::PITCH + STAGE / 4 + KS * RB * 32 * 4;
     static VpfPerDevice done;
     if (const int rc = wa_lds(wa_dq_kernel<T, DP, RB, KS>, lds, done)) return rc;
     hipLaunchKernelGGL((wa_dq_kernel<T, DP, RB, KS>), dim3((unsigned)((long)w.a.B * w.a.Hk * w.tiles)), dim3(WA_THREADS), lds, st, w);
