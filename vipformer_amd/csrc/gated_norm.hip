@@ -30,7 +30,7 @@ template <typename T, int TPR, int V> __device__ __forceinline__ void gn_store(T
     }
 }
 // a thread's part of a row as it lies in memory: the next row's tensors wait in these registers while this row is worked on.  Columns behind D
-// are fetched from column 0 and read as 0.
+// are fetched from column 0; they read as 0 (V = 1) or the thread's share of every row sum is dropped (V = 8: whole threads are behind D).
 template <typename T, int TPR, int V> struct GnRaw {
     VpfRaw<T, V> r[GN_E / V];
     __device__ __forceinline__ void fetch(const T* p, int t, int D)
@@ -41,7 +41,7 @@ template <typename T, int TPR, int V> struct GnRaw {
     __device__ __forceinline__ void get(float* v, int t, int D) const
     {
 #pragma unroll
-        for (int e = 0; e < GN_E; ++e) { const float x = r[e / V].get(e % V); v[e] = gn_col<TPR, V>(t, e) < D ? x : 0.f; }
+        for (int e = 0; e < GN_E; ++e) { const float x = r[e / V].get(e % V); v[e] = V == 8 || gn_col<TPR, V>(t, e) < D ? x : 0.f; }
     }
 };
 template <int TPR, int V> __device__ __forceinline__ void gn_param(float* v, const float* p, int t, int D, float none)
@@ -83,18 +83,20 @@ template <int TPR> __device__ __forceinline__ void gn_sum2(float& a, float& b, f
 template <int TPR, int V>
 __device__ __forceinline__ void gn_stats(const float* v, int t, int D, int rms, float eps, float& mean, float& rstd, float2 (*red)[16], int& buf)
 {
-    const float inv = 1.f / (float)D;
+    const float inv = 1.f / (float)D, live = V == 8 && 8 * t >= D ? 0.f : 1.f;
     float s = 0.f, q = 0.f;
     mean = 0.f;
     if (!rms) {
 #pragma unroll
-        for (int e = 0; e < GN_E; ++e) s += v[e];                         // (columns behind D hold 0)
+        for (int e = 0; e < GN_E; ++e) s += v[e];
+        s *= live;
         gn_sum2<TPR>(s, q, red, buf);
         mean = s * inv;
     }
     q = 0.f; s = 0.f;
 #pragma unroll
-    for (int e = 0; e < GN_E; ++e) { const float d = gn_col<TPR, V>(t, e) < D ? v[e] - mean : 0.f; q += d * d; }
+    for (int e = 0; e < GN_E; ++e) { const float d = V == 8 || gn_col<TPR, V>(t, e) < D ? v[e] - mean : 0.f; q = fmaf(d, d, q); }
+    q *= live;
     gn_sum2<TPR>(q, s, red, buf);
     rstd = rsqrtf(q * inv + eps);
 }
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_fwd_kernel(GnArgs g)
 #pragma unroll
         for (int e = 0; e < GN_E; ++e) {
             x[e] = a.alpha * x[e] + a.beta * gt[e] * y[e];
-            if (gn_col<TPR, V>(t, e) >= D) x[e] = 0.f;
+            if (V == 1 && gn_col<TPR, V>(t, e) >= D) x[e] = 0.f;
         }
         if (mine) gn_store<TX, TPR, V>((TX*)a.h + r * D, x, t, D);
         if (a.has_pre) {
@@ -191,7 +193,8 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
     const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR, D = a.D;
     const long r0 = (long)blockIdx.x * g.rows_per_wg, r1 = min(a.rows, r0 + g.rows_per_wg);
     const float inv = 1.f / (float)D, plain = a.kind == 0 ? 1.f : 0.f;    // RMS has no mean to take out
-    float wp[GN_E], bp[GN_E], wn[GN_E], gt[GN_E], awp[GN_E], abp[GN_E], awn[GN_E], abn[GN_E], ag[GN_E];
+    const float live = V == 8 && 8 * t >= D ? 0.f : 1.f;
+    float wp[GN_E], bp[GN_E], wn[GN_E], gt[GN_E], bg[GN_E], awp[GN_E], abp[GN_E], awn[GN_E], abn[GN_E], ag[GN_E];
     gn_param<TPR, V>(wp, a.has_post ? a.w_post : nullptr, t, D, 1.f);
     gn_param<TPR, V>(bp, a.has_post ? a.b_post : nullptr, t, D, 0.f);
     gn_param<TPR, V>(wn, a.w_pre, t, D, 1.f);
@@ -226,28 +229,40 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
             rdh.get(dh, t, D); rx.get(x, t, D); ry_.get(y, t, D);
             if (a.has_pre) rdn.get(dn, t, D);
             if (a.gate_mode == VPF_GATE_FULL) rg.get(gt, t, D);
-            const float my = s0, ry = s1_, mh = s2_, rh = s3;
+            const float ry = s1_, cy = -s0 * s1_, rh = s3, ch = -s2_ * s3;
             fetch(i + G < end ? i + G : i);                               // (unconditional: behind a branch its values would be awaited at the join)
-            const float one = mine ? 1.f : 0.f;
+            if (G > 1 && !mine) {                                         // a row taken twice: its gradients count once
+#pragma unroll
+                for (int e = 0; e < GN_E; ++e) dh[e] = dn[e] = 0.f;
+            }
+            if (a.gate_mode == VPF_GATE_FULL || i == seg) {
+#pragma unroll
+                for (int e = 0; e < GN_E; ++e) bg[e] = a.beta * gt[e];
+            }
 #pragma unroll
             for (int e = 0; e < GN_E; ++e) {
-                y[e] = (y[e] - my) * ry;                                  // no post norm: mean 0, rstd 1
-                u[e] = y[e] * wp[e] + bp[e];
+                y[e] = fmaf(y[e], ry, cy);                                // no post norm: mean 0, rstd 1
+                u[e] = fmaf(y[e], wp[e], bp[e]);
             }
             if (a.has_pre) {
                 float s1 = 0.f, s2 = 0.f;
 #pragma unroll
                 for (int e = 0; e < GN_E; ++e) {
-                    x[e] = (a.alpha * x[e] + a.beta * gt[e] * u[e] - mh) * rh;
-                    if (gn_col<TPR, V>(t, e) >= D) x[e] = 0.f;
-                    awn[e] += one * dn[e] * x[e]; abn[e] += one * dn[e];
-                    dn[e] *= wn[e];
-                    s1 += dn[e]; s2 += dn[e] * x[e];
+                    x[e] = fmaf(fmaf(a.alpha, x[e], bg[e] * u[e]), rh, ch);
+                    if (V == 1 && gn_col<TPR, V>(t, e) >= D) x[e] = 0.f;
+                    awn[e] = fmaf(dn[e], x[e], awn[e]);
                 }
+                if (g.want & GN_WANT_BPRE) {
+#pragma unroll
+                    for (int e = 0; e < GN_E; ++e) abn[e] += dn[e];
+                }
+#pragma unroll
+                for (int e = 0; e < GN_E; ++e) { dn[e] *= wn[e]; s1 += dn[e]; s2 = fmaf(dn[e], x[e], s2); }
+                s1 *= live; s2 *= live;
                 gn_sum2<TPR>(s1, s2, red, buf);
                 s1 *= inv * plain; s2 *= inv;
 #pragma unroll
-                for (int e = 0; e < GN_E; ++e) dh[e] += rh * (dn[e] - s1 - x[e] * s2);
+                for (int e = 0; e < GN_E; ++e) dh[e] = fmaf(rh, fmaf(-x[e], s2, dn[e] - s1), dh[e]);
             }
             if (a.dx && mine) {
 #pragma unroll
@@ -260,28 +275,35 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
                     for (int e = 0; e < GN_E; ++e) x[e] = a.beta * dh[e] * u[e];
                     gn_store<TY, TPR, V>((TY*)a.dgate + r * D, x, t, D);
                 }
-            } else {
+            } else if (g.want & GN_WANT_GATE) {
 #pragma unroll
-                for (int e = 0; e < GN_E; ++e) ag[e] += one * a.beta * dh[e] * u[e];
+                for (int e = 0; e < GN_E; ++e) ag[e] = fmaf(dh[e], u[e], ag[e]);      // (times beta when it is written)
             }
             float f1 = 0.f, f2 = 0.f;
 #pragma unroll
             for (int e = 0; e < GN_E; ++e) {
-                if (gn_col<TPR, V>(t, e) >= D) dh[e] = 0.f;
-                dh[e] *= a.beta * gt[e];
-                awp[e] += one * dh[e] * y[e]; abp[e] += one * dh[e];
-                dh[e] *= wp[e];
-                f1 += dh[e]; f2 += dh[e] * y[e];
+                if (V == 1 && gn_col<TPR, V>(t, e) >= D) dh[e] = 0.f;
+                dh[e] *= bg[e];
+                awp[e] = fmaf(dh[e], y[e], awp[e]);
             }
+            if (g.want & GN_WANT_BPOST) {
+#pragma unroll
+                for (int e = 0; e < GN_E; ++e) abp[e] += dh[e];
+            }
+#pragma unroll
+            for (int e = 0; e < GN_E; ++e) { dh[e] *= wp[e]; f1 += dh[e]; f2 = fmaf(dh[e], y[e], f2); }
             if (a.has_post) {
+                f1 *= live; f2 *= live;
                 gn_sum2<TPR>(f1, f2, red, buf);
                 f1 *= inv * plain; f2 *= inv;
 #pragma unroll
-                for (int e = 0; e < GN_E; ++e) dh[e] = ry * (dh[e] - f1 - y[e] * f2);
+                for (int e = 0; e < GN_E; ++e) dh[e] = ry * fmaf(-y[e], f2, dh[e] - f1);
             }
             if (a.dy && mine) gn_store<TY, TPR, V>((TY*)a.dy + r * D, dh, t, D);
         }
         if (g.want & GN_WANT_GATE) {
+#pragma unroll
+            for (int e = 0; e < GN_E; ++e) ag[e] *= a.beta;
             gn_partial<TPR, V>(ag, wsg + ((long)blockIdx.x + s) * D, t, grp, D, cols);
 #pragma unroll
             for (int e = 0; e < GN_E; ++e) ag[e] = 0.f;
@@ -347,11 +369,12 @@ static void gn_plan(GnArgs& g, int want_wgs)
     g.nwg = vpf_cdiv(g.a.rows, per);
 }
 // Backward: a workgroup walks at least 4 row groups, so that its partial rows (5 D floats) stay small beside what it reads, and the
-// partials are at most 1024 rows (four workgroups per CU).
+// partials are at most 512 rows (two workgroups per CU, the next row of each in flight).  Measured on 32768 x 2048 in bf16, kernel + fold:
+// 512 177 + 6 us, 768 215 + 10, 1024 177 + 14, 1536 189 + 19.
 static void gn_plan_bwd(GnArgs& g)
 {
     const long want = g.a.rows / (4L * gn_groups(g.a.D)) + 1;
-    gn_plan(g, want < 1024 ? (int)want : 1024);
+    gn_plan(g, want < 512 ? (int)want : 512);
     const VpfGatedNorm& a = g.a;
     g.want = (a.has_post && a.dw_post ? GN_WANT_WPOST : 0) | (a.has_post && a.db_post ? GN_WANT_BPOST : 0) | (a.has_pre && a.dw_pre ? GN_WANT_WPRE : 0) |
              (a.has_pre && a.db_pre ? GN_WANT_BPRE : 0) | (a.gate_mode == VPF_GATE_ROWS && a.dgate ? GN_WANT_GATE : 0);
