@@ -261,6 +261,30 @@ def test_gated_norm_many_samples_and_ranks(shape):
     norm_case(shape, "layer", "sample", "f32", "fp16", True, True)
 
 
+@pytest.mark.parametrize("L", [1, 2, 7, 31, 33])
+def test_gated_norm_gates_of_few_rows(L):
+    """Gate rows that serve fewer rows than a workgroup holds (their gradient goes through scratch row by row), in both paths of the row kernels."""
+    norm_case((301, L, 64), "layer", "sample", "f32", "fp16", True, True)
+    norm_case((40, L, 257), "rms", "sample", "bf16", "bf16", True, True)
+    norm_case((5, L, 2048), "layer", "sample", "f32", "f32", False, True)
+
+
+def test_gated_norm_more_samples_than_a_grid():
+    """300 000 gate rows of 1 000 channels: the fold of their gradients walks over more items than a launch has workgroups."""
+    from vipformer_amd.ops_block import gated_norm_residual
+    g = gen(14)
+    B, D = 300000, 1000
+    x, y = randn(g, B, 1, D).requires_grad_(), randn(g, B, 1, D, dtype=torch.float16)
+    gate = randn(g, B, 1, D).requires_grad_()
+    h, _ = gated_norm_residual(x, y, gate=gate, post=(None, None), kind="rms")
+    dh = randn(g, B, 1, D)
+    (dg,) = torch.autograd.grad(h, gate, dh)
+    rows = torch.randint(0, B, (500,), generator=g, device="cuda")
+    rows[0], rows[1] = 0, B - 1
+    ref = norm_ref(x[rows], y[rows], gate[rows], (None, None), None, "rms", 1.0, 1.0, 1e-5, dh[rows], None)
+    close(dg[rows], ref["dgate"][0], BWD_N * ref["dgate"][1], "dgate")
+
+
 def test_gated_norm_modules_identity_and_unused_outputs():
     from vipformer_amd.ops_block import gated_norm_residual
     g = gen(11)
@@ -427,6 +451,12 @@ def test_window_attention_every_workgroup_shape(dh, dtype):
         pad = torch.arange(L, device="cuda")[None, :] >= torch.randint(1, L + 1, (B, 1), generator=g, device="cuda")
         attention_case(B, L, L, Hq, Hk, dh, (33, 21), 2, dtype)
         attention_case(B, L, L, Hq, Hk, dh, (40, 0), 3, dtype, pad=pad)
+
+
+@pytest.mark.parametrize("L,Hq,Hk,dh,window,sinks", [(3000, 2, 1, 64, (0, 0), 600), (2500, 1, 1, 32, (3, 0), 100), (3000, 4, 1, 128, (10, 10), 130)])
+def test_window_attention_many_first_tokens(L, Hq, Hk, dh, window, sinks):
+    """First tokens over several key tiles: with pieces of their far rows, and (more than 8 tiles) without."""
+    attention_case(1, L, L, Hq, Hk, dh, window, sinks, "bf16")
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])

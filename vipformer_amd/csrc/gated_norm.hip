@@ -16,7 +16,8 @@
 
 template <int TPR> struct GnGeom { static constexpr int NT = TPR <= 256 ? 256 : TPR, G = NT / TPR, W = (TPR + 63) / 64; };
 
-struct GnArgs { VpfGatedNorm a; int rows_per_wg, nwg, want; };
+// `single`: a gate row serves so few rows that its gradient goes row by row to scratch and is summed from there
+struct GnArgs { VpfGatedNorm a; int rows_per_wg, nwg, want, single; };
 enum { GN_WANT_WPOST = 1, GN_WANT_BPOST = 2, GN_WANT_WPRE = 4, GN_WANT_BPRE = 8, GN_WANT_GATE = 16 };
 
 // this thread's columns of a row: 8 t .. 8 t + 7 (V = 8: D a multiple of 8, 16-byte aligned) or t, t + TPR, .. (V = 1)
@@ -181,7 +182,7 @@ __device__ __forceinline__ void gn_partial(const float* acc, float* dst, int t, 
 }
 
 // ws: [4][nwg][D] partials of dw_post, db_post, dw_pre, db_pre, then [nwg + samples][D] of the gate: workgroup w's rows of sample s go to
-// row w + s (unique: along consecutive rows at least one of the two rises from one (w, s) to the next)
+// row w + s (unique: along consecutive rows at least one of the two rises from one (w, s) to the next).  g.single: [rows][D] of the gate instead.
 template <typename TX, typename TY, int TPR, int V>
 __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
 {
@@ -204,13 +205,14 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
     for (long seg = r0; seg < r1;) {
         long end = r1;
         int s = 0;
-        if (a.gate_mode == VPF_GATE_ROWS) {
+        if (a.gate_mode == VPF_GATE_ROWS && !g.single) {
             s = (int)((uint32_t)seg / (uint32_t)a.gate_rows);
             end = min(r1, (long)(s + 1) * a.gate_rows);
             gn_param<TPR, V>(gt, (const float*)a.gate + (long)s * D, t, D, 1.f);
         }
         GnRaw<TX, TPR, V> rdh, rx;
         GnRaw<TY, TPR, V> rdn, ry_, rg;
+        GnRaw<float, TPR, V> rgs;
         float s0, s1_, s2_, s3;
         auto fetch = [&](long i) {
             const long r = min(i + grp, end - 1);
@@ -219,6 +221,7 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
             rx.fetch((const TX*)a.x + r * D, t, D);
             ry_.fetch((const TY*)a.y + r * D, t, D);
             if (a.gate_mode == VPF_GATE_FULL) rg.fetch((const TY*)a.gate + r * D, t, D);
+            if (g.single) rgs.fetch((const float*)a.gate + (long)((uint32_t)r / (uint32_t)a.gate_rows) * D, t, D);
             s0 = a.stats[r]; s1_ = a.stats[a.rows + r]; s2_ = a.stats[2 * a.rows + r]; s3 = a.stats[3 * a.rows + r];
         };
         fetch(seg);
@@ -229,13 +232,14 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
             rdh.get(dh, t, D); rx.get(x, t, D); ry_.get(y, t, D);
             if (a.has_pre) rdn.get(dn, t, D);
             if (a.gate_mode == VPF_GATE_FULL) rg.get(gt, t, D);
+            if (g.single) rgs.get(gt, t, D);
             const float ry = s1_, cy = -s0 * s1_, rh = s3, ch = -s2_ * s3;
             fetch(i + G < end ? i + G : i);                               // (unconditional: behind a branch its values would be awaited at the join)
             if (G > 1 && !mine) {                                         // a row taken twice: its gradients count once
 #pragma unroll
                 for (int e = 0; e < GN_E; ++e) dh[e] = dn[e] = 0.f;
             }
-            if (a.gate_mode == VPF_GATE_FULL || i == seg) {
+            if (a.gate_mode == VPF_GATE_FULL || g.single || i == seg) {
 #pragma unroll
                 for (int e = 0; e < GN_E; ++e) bg[e] = a.beta * gt[e];
             }
@@ -275,6 +279,12 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
                     for (int e = 0; e < GN_E; ++e) x[e] = a.beta * dh[e] * u[e];
                     gn_store<TY, TPR, V>((TY*)a.dgate + r * D, x, t, D);
                 }
+            } else if (g.single) {
+                if ((g.want & GN_WANT_GATE) && mine) {
+#pragma unroll
+                    for (int e = 0; e < GN_E; ++e) x[e] = a.beta * dh[e] * u[e];
+                    gn_store<float, TPR, V>(wsg + r * D, x, t, D);
+                }
             } else if (g.want & GN_WANT_GATE) {
 #pragma unroll
                 for (int e = 0; e < GN_E; ++e) ag[e] = fmaf(dh[e], u[e], ag[e]);      // (times beta when it is written)
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
             }
             if (a.dy && mine) gn_store<TY, TPR, V>((TY*)a.dy + r * D, dh, t, D);
         }
-        if (g.want & GN_WANT_GATE) {
+        if ((g.want & GN_WANT_GATE) && !g.single) {
 #pragma unroll
             for (int e = 0; e < GN_E; ++e) ag[e] *= a.beta;
             gn_partial<TPR, V>(ag, wsg + ((long)blockIdx.x + s) * D, t, grp, D, cols);
@@ -319,41 +329,47 @@ __global__ void __launch_bounds__(GnGeom<TPR>::NT) gn_bwd_kernel(GnArgs g)
 
 // Partial rows -> sums: workgroup = 64 columns of one result (the four parameters, then the gate of every sample), 16 slices of the partial
 // rows in parallel, joined in LDS in a fixed order.
-__global__ void __launch_bounds__(64 * GN_FOLD_SLICES) gn_fold_kernel(GnArgs g, int col_blocks)
+__global__ void __launch_bounds__(64 * GN_FOLD_SLICES) gn_fold_kernel(GnArgs g, int col_blocks, long items)
 {
     __shared__ float part[GN_FOLD_SLICES][64];
     const VpfGatedNorm& a = g.a;
-    const int k = blockIdx.x / col_blocks, lane = threadIdx.x & 63, c = (blockIdx.x % col_blocks) * 64 + lane, sl = threadIdx.x >> 6;
-    if (k < 4 && !(g.want & (1 << k))) return;
-    const float* src;
-    long n;
-    if (k < 4) { src = a.ws + (long)k * g.nwg * a.D; n = g.nwg; }
-    else {
-        const long s = k - 4, w0 = s * a.gate_rows / g.rows_per_wg, w1 = ((s + 1) * a.gate_rows - 1) / g.rows_per_wg;
-        src = a.ws + (4L * g.nwg + w0 + s) * a.D; n = w1 - w0 + 1;
-    }
-    const long per = (n + GN_FOLD_SLICES - 1) / GN_FOLD_SLICES, b = min(n, sl * per), e = min(n, b + per);
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    if (c < a.D) {
-        long i = b;
-        for (; i + 3 < e; i += 4) {
-            s0 += src[i * a.D + c]; s1 += src[(i + 1) * a.D + c]; s2 += src[(i + 2) * a.D + c]; s3 += src[(i + 3) * a.D + c];
+    const int lane = threadIdx.x & 63, sl = threadIdx.x >> 6;
+    for (long item = blockIdx.x; item < items; item += gridDim.x) {
+        const long k = item / col_blocks;
+        const int c = (int)(item % col_blocks) * 64 + lane;
+        if (k < 4 && !(g.want & (1 << k))) continue;
+        const float* src;
+        long n;
+        if (k < 4) { src = a.ws + k * g.nwg * a.D; n = g.nwg; }
+        else if (g.single) { src = a.ws + (4L * g.nwg + (k - 4) * a.gate_rows) * a.D; n = a.gate_rows; }
+        else {
+            const long s = k - 4, w0 = s * a.gate_rows / g.rows_per_wg, w1 = ((s + 1) * a.gate_rows - 1) / g.rows_per_wg;
+            src = a.ws + (4L * g.nwg + w0 + s) * a.D; n = w1 - w0 + 1;
         }
-        for (; i < e; ++i) s0 += src[i * a.D + c];
-    }
-    part[sl][lane] = (s0 + s1) + (s2 + s3);
-    __syncthreads();
-    if (sl == 0 && c < a.D) {
-        float s = 0.f;
+        const long per = (n + GN_FOLD_SLICES - 1) / GN_FOLD_SLICES, b = min(n, sl * per), e = min(n, b + per);
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        if (c < a.D) {
+            long i = b;
+            for (; i + 3 < e; i += 4) {
+                s0 += src[i * a.D + c]; s1 += src[(i + 1) * a.D + c]; s2 += src[(i + 2) * a.D + c]; s3 += src[(i + 3) * a.D + c];
+            }
+            for (; i < e; ++i) s0 += src[i * a.D + c];
+        }
+        part[sl][lane] = (s0 + s1) + (s2 + s3);
+        __syncthreads();
+        if (sl == 0 && c < a.D) {
+            float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < GN_FOLD_SLICES; ++j) s += part[j][lane];
-        switch (k) {
-            case 0: a.dw_post[c] = s; break;
-            case 1: a.db_post[c] = s; break;
-            case 2: a.dw_pre[c] = s; break;
-            case 3: a.db_pre[c] = s; break;
-            default: ((float*)a.dgate)[(long)(k - 4) * a.D + c] = s;
+            for (int j = 0; j < GN_FOLD_SLICES; ++j) s += part[j][lane];
+            switch (k) {
+                case 0: a.dw_post[c] = s; break;
+                case 1: a.db_post[c] = s; break;
+                case 2: a.dw_pre[c] = s; break;
+                case 3: a.db_pre[c] = s; break;
+                default: ((float*)a.dgate)[(k - 4) * a.D + c] = s;
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -378,8 +394,12 @@ static void gn_plan_bwd(GnArgs& g)
     const VpfGatedNorm& a = g.a;
     g.want = (a.has_post && a.dw_post ? GN_WANT_WPOST : 0) | (a.has_post && a.db_post ? GN_WANT_BPOST : 0) | (a.has_pre && a.dw_pre ? GN_WANT_WPRE : 0) |
              (a.has_pre && a.db_pre ? GN_WANT_BPRE : 0) | (a.gate_mode == VPF_GATE_ROWS && a.dgate ? GN_WANT_GATE : 0);
+    // a gate row that serves fewer rows than two walks of a workgroup's row groups: segments of its own would leave most groups idle
+    g.single = a.gate_mode == VPF_GATE_ROWS && a.gate_rows < 2 * gn_groups(a.D);
 }
 static long gn_samples(const VpfGatedNorm& a) { return a.gate_mode == VPF_GATE_ROWS ? a.rows / a.gate_rows : 0; }
+
+static long gn_ws_floats(const GnArgs& g) { return (4L * g.nwg + (g.single ? g.a.rows : g.nwg + gn_samples(g.a))) * g.a.D; }
 
 static int gn_check(const VpfGatedNorm& a)
 {
@@ -435,7 +455,7 @@ extern "C" int vpf_gated_norm_fwd(const VpfGatedNorm* args, void* stream)
 {
     (void)hipGetLastError();
     if (!args) return VPF_ERR_NULL;
-    GnArgs g = {*args, 0, 0, 0};
+    GnArgs g = {*args, 0, 0, 0, 0};
     const VpfGatedNorm& a = g.a;
     if (const int rc = gn_check(a)) return rc;
     if (a.rows == 0) return VPF_OK;
@@ -447,31 +467,30 @@ extern "C" int vpf_gated_norm_fwd(const VpfGatedNorm* args, void* stream)
 extern "C" long vpf_gated_norm_ws(const VpfGatedNorm* args)
 {
     if (!args) return VPF_ERR_NULL;
-    GnArgs g = {*args, 0, 0, 0};
+    GnArgs g = {*args, 0, 0, 0, 0};
     if (const int rc = gn_check(g.a)) return rc;
     if (g.a.rows == 0) return 0;
     gn_plan_bwd(g);
-    return (5L * g.nwg + gn_samples(g.a)) * g.a.D;
+    return gn_ws_floats(g);
 }
 
 extern "C" int vpf_gated_norm_bwd(const VpfGatedNorm* args, void* stream)
 {
     (void)hipGetLastError();
     if (!args) return VPF_ERR_NULL;
-    GnArgs g = {*args, 0, 0, 0};
+    GnArgs g = {*args, 0, 0, 0, 0};
     const VpfGatedNorm& a = g.a;
     if (const int rc = gn_check(a)) return rc;
     if (a.rows == 0) return VPF_OK;
     if (!a.x || !a.y || !a.dh || !a.stats || (a.has_pre && !a.dn) || (a.gate_mode != VPF_GATE_NONE && !a.gate) || !a.ws) return VPF_ERR_NULL;
     gn_plan_bwd(g);
     const long samples = gn_samples(a);
-    if (a.ws_floats < (5L * g.nwg + samples) * a.D) return VPF_ERR_BADSHAPE;
+    if (a.ws_floats < gn_ws_floats(g)) return VPF_ERR_BADSHAPE;
     if (const int rc = gn_pick<true>(g, (hipStream_t)stream)) return rc;
     if (!g.want) return VPF_OK;
     const int cb = vpf_cdiv(a.D, 64);
-    const long grid = cb * (4 + (g.want & GN_WANT_GATE ? samples : 0));
-    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
-    hipLaunchKernelGGL(gn_fold_kernel, dim3((unsigned)grid), dim3(64 * GN_FOLD_SLICES), 0, (hipStream_t)stream, g, cb);
+    const long items = cb * (4 + (g.want & GN_WANT_GATE ? samples : 0));
+    hipLaunchKernelGGL(gn_fold_kernel, dim3((unsigned)(items < 65536 ? items : 65536)), dim3(64 * GN_FOLD_SLICES), 0, (hipStream_t)stream, g, cb, items);
     VPF_CHECK_LAUNCH();
     return VPF_OK;
 }

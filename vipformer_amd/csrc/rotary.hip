@@ -118,7 +118,7 @@ static int rotary_launch(const VpfRotary& a, hipStream_t st)
     r.tok = (int)(tok < a.L ? tok : a.L);
     r.blocks = vpf_cdiv(a.L, r.tok);
     const long grid = (long)a.B * r.blocks;
-    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
+    if (grid * threads >= 1L << 32) return VPF_ERR_BADSHAPE;          // (a launch counts its threads in 32 bits)
     hipLaunchKernelGGL((rotary_kernel<T, V, HALF>), dim3((unsigned)grid), dim3(threads), sizeof(float2) * r.tok * a.P, st, r);
     VPF_CHECK_LAUNCH();
     return VPF_OK;

@@ -23,6 +23,7 @@ typedef __attribute__((ext_vector_type(8))) short wa_s16x8;
 typedef __attribute__((ext_vector_type(16))) float wa_f32x16;
 #define WA_LOG2E 1.4426950408889634f
 #define WA_THREADS 256
+#define WA_MAX_GRID (1L << 23)          // workgroups of up to 512 threads: a launch counts its threads in 32 bits
 #define WA_FAR (1 << 30)                // an open side of the window; positions and lengths stay below it
 
 template <typename T> struct WaMma;
@@ -998,7 +999,7 @@ static long wa_fwd_ws(const WaArgs& w) { return w.splits > 1 ? (long)w.splits * 
 
 // Key tiles of 128 at head dimension 128 where that leaves a workgroup for each CU (the stages of Q and dO then serve twice the keys), else of 64.
 // The rows behind a sink tile's own window are cut into pieces about as long as the row range of an ordinary tile, where that leaves more than
-// one of them.
+// one of them: at most 32 pieces (they are fp32 scratch), none where the first tokens fill more than 8 tiles (enough workgroups by themselves).
 static void wa_plan_bwd(WaArgs& w)
 {
     const VpfWindowAttn& a = w.a;
@@ -1008,8 +1009,9 @@ static void wa_plan_bwd(WaArgs& w)
     w.chunks = 0;
     const long range = ((long)a.left + a.right + w.key_tile) * w.g, all = vpf_cdiv(w.rows, WA_ROWS), cycle = range / WA_ROWS + 2;
     w.cycle = (int)(cycle < all ? cycle : all > 0 ? all : 1);
-    if (w.sink_tiles > 0 && w.rows > 2 * range) {
+    if (w.sink_tiles > 0 && w.sink_tiles <= 8 && w.rows > 2 * range) {
         long rows = range > 512 ? range : 512;
+        rows = rows > w.rows / 32 ? rows : w.rows / 32;
         w.chunk_rows = (int)((rows + 63) / 64 * 64);
         w.chunks = vpf_cdiv(w.rows, w.chunk_rows);
     }
@@ -1034,7 +1036,7 @@ template <typename T, int DP, int RB, int RW, int KS, int SUBK> static int wa_la
     static VpfPerDevice done;
     if (const int rc = wa_lds(wa_fwd_kernel<T, DP, RB, RW, KS, SUBK>, lds, done)) return rc;
     const long grid = (long)w.a.B * w.a.Hk * w.tiles * w.splits;
-    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
+    if (grid >= WA_MAX_GRID) return VPF_ERR_BADSHAPE;
     hipLaunchKernelGGL((wa_fwd_kernel<T, DP, RB, RW, KS, SUBK>), dim3((unsigned)grid), dim3(WA_THREADS), lds, st, w);
     if (w.splits > 1) hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3(vpf_cdiv((long)w.a.B * w.a.Hk * w.rows, 4)), dim3(WA_THREADS), 0, st, w);
     VPF_CHECK_LAUNCH();
@@ -1061,17 +1063,17 @@ template <typename T, int DP, int RB, int KS> static int wa_launch_dq(const WaAr
 template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
 {
     const long bh = (long)w.a.B * w.a.Hk;
+    const int rb = wa_row_blocks(w);
+    w.tiles = vpf_cdiv(w.rows, 32 * rb);
+    w.splits = 1;
+    w.runs = wa_runs(w);
+    const long grid = bh * (w.ktiles + (long)w.sink_tiles * w.chunks);
+    if (grid >= WA_MAX_GRID || bh * w.tiles >= WA_MAX_GRID || bh * w.a.sinks >= WA_MAX_GRID) return VPF_ERR_BADSHAPE;      // in front of every launch
     if (w.rows > 0) {
-        const int rb = wa_row_blocks(w);
-        w.tiles = vpf_cdiv(w.rows, 32 * rb);
-        w.splits = 1;
-        w.runs = wa_runs(w);
         const int rc = rb == 4 ? wa_launch_dq<T, DP, 4, 1>(w, st) : rb == 2 ? wa_launch_dq<T, DP, 2, 2>(w, st) : wa_launch_dq<T, DP, 1, 4>(w, st);
         if (rc) return rc;
     }
     if (w.a.Lkv == 0) return VPF_OK;
-    const long grid = bh * (w.ktiles + (long)w.sink_tiles * w.chunks);
-    if (grid > 0x7fffffffL) return VPF_ERR_BADSHAPE;
     auto launch = [&](auto kernel, int kb, VpfPerDevice& done) -> int {
         const size_t lds = 4 * WA_ROWS * WaTile<DP>::PITCH + (DP <= 96 ? 0 : 32 * kb * WaTile<DP>::PITCH) + 6 * WA_ROWS * 4;
         if (const int rc = wa_lds(kernel, lds, done)) return rc;

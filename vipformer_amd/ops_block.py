@@ -28,10 +28,13 @@ _pack_rotary, _pack_norm, _pack_attn = (L.packer(c).pack for c in (L.Rotary, L.G
 
 
 def _same_device(what: str, first: torch.Tensor, *rest) -> None:
-    L.need_cuda(first, *rest)
+    dev = first.device
+    if dev.type != "cuda":
+        L.need_cuda(first)
     for t in rest:
-        if t is not None and t.device != first.device:
-            raise L.VpfError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != dev:
+            L.need_cuda(t)
+            raise L.VpfError(f"{what}: tensors on {dev} and {t.device}")
 
 
 def _wants_grad(*ts) -> bool:
@@ -271,10 +274,10 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
     mode, gate_rows = 0, 1
     if gate is not None:
         per_sample = x.dim() >= 2 and gate.dim() == x.dim() and tuple(gate.shape) == (x.shape[0],) + (1,) * (x.dim() - 2) + (D,)
-        if tuple(gate.shape) == (D,):
-            mode, gate_rows = 1, max(rows, 1)
-        elif gate.shape == x.shape and gate.dtype == y.dtype:
+        if gate.shape == x.shape and gate.dtype == y.dtype:
             mode = 2
+        elif tuple(gate.shape) == (D,):
+            mode, gate_rows = 1, max(rows, 1)
         elif per_sample:
             mode, gate_rows = 1, max(rows // max(x.shape[0], 1), 1)
         else:
@@ -368,7 +371,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     With n keys in use the last query stands at the last of them: query i at position n - Lq + i.  n is Lkv, or kv_lens[b] (int32 / int64 [B],
     on the device, read by the kernels: a captured graph follows it): a preallocated cache that is filled to different lengths.
     pad_mask: bool [B, Lkv], True = this key is padding (as the ``pad_mask`` of the framework's encoders); it moves no positions.
-    Keys that no query sees may hold anything.  A query that sees nothing gets zeros (and passes no gradient).
+    Keys that no query sees may hold anything, also NaN; a value that is not finite in a key that some query sees reaches the queries around it, as
+    0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros, and its (finite) gradient reaches nothing.
     Key heads are shared by heads / key heads consecutive query heads.  head_dim: a multiple of 8 up to 128; scale defaults to head_dim ** -0.5.
     Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v.  There is no dropout on the weights here."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] < 1 or \
