@@ -622,7 +622,8 @@ def test_a_block_of_them_against_64_bits():
     nr = ln(hr, R["w2"], R["b2"])
     ref = torch.autograd.grad((hr, nr), list(R.values()), (dh.double(), dn.double()))
     for name, a, b in [("h", h, hr), ("n", n, nr)] + list(zip(P, grads, ref)):
-        rel = float((a.detach().double() - b).norm() / b.detach().norm())
+        a, b = a.detach().double(), b.detach()
+        rel = float((a - b).norm() / b.norm())
         assert rel < 2.0 ** -6, (name, rel)
 
 

@@ -105,27 +105,28 @@ _NONE3 = (0, 0, 0)
 
 
 def _rotary_ready(t):
-    """The kernel takes any strides with a contiguous, pair-aligned last dimension; everything else is copied."""
-    sb, sl, sh = _strides(t)
-    if t.stride(3) != 1 or (sb | sl | sh) & 1 or t.data_ptr() % (2 * t.element_size()):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    """(tensor, strides).  The kernel takes any strides with a contiguous, pair-aligned last dimension; everything else is copied."""
+    st = sb, sl, sh = _strides(t)
+    if (sb | sl | sh) & 1 or t.stride(3) != 1 or t.data_ptr() % (2 * t.element_size()):
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _strides(t)
+    return t, st
 
 
 def _rotary_run(plan, pos, q, k, inverse):
-    q = _rotary_ready(q)
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = None
+    q, sq = _rotary_ready(q)
+    B, Lt, Hq, dh = shape = q.shape
+    dt, dev = q.dtype, q.device
+    oq = torch.empty(shape, dtype=dt, device=dev)
+    ok, Hk, kp, okp, sk, sok = None, 0, 0, 0, _NONE3, _NONE3
     if k is not None:
-        k = _rotary_ready(k)
-        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    B, Lt, Hq, dh = q.shape
-    freq, axis = plan.tables(q.device)
+        k, sk = _rotary_ready(k)
+        ok = torch.empty(k.shape, dtype=dt, device=dev)
+        Hk, kp, okp, sok = k.shape[2], k.data_ptr(), ok.data_ptr(), _strides(ok)
+    freq, axis = plan.tables(dev)
     L.launch("vpf_rotary_axes", _pack_rotary(
-        B, Lt, Hq, 0 if k is None else k.shape[2], dh, plan.pairs, len(plan.sections), plan.layout_code, _TYPE[q.dtype], _POS[pos.dtype], inverse, 0,
-        q.data_ptr(), _ptr(k), oq.data_ptr(), _ptr(ok), *_strides(q), *(_NONE3 if k is None else _strides(k)),
-        *_strides(oq), *(_NONE3 if k is None else _strides(ok)), pos.data_ptr(), pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0,
-        freq.data_ptr(), axis.data_ptr()), q.device)
+        B, Lt, Hq, Hk, dh, plan.pairs, len(plan.sections), plan.layout_code, _TYPE[dt], _POS[pos.dtype], inverse, 0, q.data_ptr(), kp, oq.data_ptr(), okp,
+        *sq, *sk, *_strides(oq), *sok, pos.data_ptr(), pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, freq.data_ptr(), axis.data_ptr()), dev)
     return oq, ok
 
 
@@ -150,15 +151,17 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     positions: [L, axes] or [B, L, axes] (or [1, L, axes]), integers or fp32 / fp64 coordinates; no gradient reaches them.  Angles are
     formed in fp64, so positions far into a stream keep their fraction of a turn.  fp32, fp16 and bf16, rounded once.
     Returns new contiguous tensors (q, k), or q alone where k is None."""
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+    qs = q.shape
+    ks = qs if k is None else k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks[0] != qs[0] or ks[1] != qs[1] or ks[3] != qs[3]:
         raise L.VpfError(f"rotary_axes: q [B, L, heads, head_dim] and k of the same B, L and head_dim (got {tuple(q.shape)}, "
                          f"{None if k is None else tuple(k.shape)})")
-    if q.shape[3] != plan.head_dim:
-        raise L.VpfError(f"rotary_axes: head_dim {q.shape[3]}, the plan was built for {plan.head_dim}")
+    if qs[3] != plan.head_dim:
+        raise L.VpfError(f"rotary_axes: head_dim {qs[3]}, the plan was built for {plan.head_dim}")
     if q.dtype not in _TYPE or (k is not None and k.dtype != q.dtype):
         raise L.VpfError(f"rotary_axes: q and k of one type out of fp32, fp16, bf16 (got {q.dtype}, {None if k is None else k.dtype})")
-    if positions.dim() not in (2, 3) or positions.shape[-2:] != (q.shape[1], len(plan.sections)) or \
-            (positions.dim() == 3 and positions.shape[0] not in (1, q.shape[0])):
+    ps = positions.shape
+    if len(ps) not in (2, 3) or ps[-1] != len(plan.sections) or ps[-2] != qs[1] or (len(ps) == 3 and ps[0] != 1 and ps[0] != qs[0]):
         raise L.VpfError(f"rotary_axes: positions [L, axes] or [B, L, axes] = [({q.shape[0]},) {q.shape[1]}, {len(plan.sections)}] "
                          f"(got {tuple(positions.shape)})")
     if positions.dtype not in _POS:
@@ -234,10 +237,11 @@ class GatedNormFn(torch.autograd.Function):
         return (None, dx, dy, dgate, *grads)
 
 
+_NO_PARAMS = (None, None)
+
+
 def _norm_params(what, wb, kind, eps, x):
     """(weight, bias) of one norm, each fp32 [D] or None, and its epsilon."""
-    if wb is None:
-        return (None, None), eps
     if isinstance(wb, torch.nn.Module):
         want = {"layer": torch.nn.LayerNorm, "rms": torch.nn.RMSNorm}[kind]
         if not isinstance(wb, want) or tuple(wb.normalized_shape) != (x.shape[-1],):
@@ -247,7 +251,7 @@ def _norm_params(what, wb, kind, eps, x):
     if len(wb) != 2:
         raise L.VpfError(f"gated_norm_residual: {what} is a norm module or (weight, bias)")
     for p in wb:
-        if p is not None and (p.dtype != F32 or tuple(p.shape) != (x.shape[-1],)):
+        if p is not None and (p.dtype is not F32 or p.dim() != 1 or p.shape[0] != x.shape[-1]):
             raise L.VpfError(f"gated_norm_residual: {what}: fp32 parameters of shape ({x.shape[-1]},) (got {p.dtype}, {tuple(p.shape)})")
     return tuple(None if p is None else p.contiguous() for p in wb), eps
 
@@ -261,31 +265,32 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
     post / pre: (weight, bias) with fp32 [D] tensors or None entries, a LayerNorm / RMSNorm module, or None for no norm there.
     kind: "layer" or "rms" (biased variance, ``eps`` inside the root) for both norms; a module brings its own eps.
     gate: None, fp32 [D], one fp32 row of D per sample (x [B, ..., D]: gate [B, 1, .., D]), or one of x's shape and y's type."""
-    if x.dim() < 1 or x.shape != y.shape or not 1 <= x.shape[-1] <= 8192:
+    shape = x.shape
+    if len(shape) < 1 or shape != y.shape or not 1 <= shape[-1] <= 8192:
         raise L.VpfError(f"gated_norm_residual: x and y of one shape [..., D], 1 <= D <= 8192 (got {tuple(x.shape)}, {tuple(y.shape)})")
     if x.dtype not in _TYPE or y.dtype not in _TYPE or (x.dtype != F32 and x.dtype != y.dtype):
         raise L.VpfError(f"gated_norm_residual: x is fp32, or x and y are both fp16 or both bf16 (got {x.dtype}, {y.dtype})")
     if kind not in ("layer", "rms"):
         raise L.VpfError(f"gated_norm_residual: kind is 'layer' or 'rms' (got {kind!r})")
-    D = x.shape[-1]
+    D = shape[-1]
     rows = x.numel() // D
     if rows >= 1 << 31:
         raise L.VpfError(f"gated_norm_residual: {rows} rows; at most 2^31 - 1")
     mode, gate_rows = 0, 1
     if gate is not None:
-        per_sample = x.dim() >= 2 and gate.dim() == x.dim() and tuple(gate.shape) == (x.shape[0],) + (1,) * (x.dim() - 2) + (D,)
-        if gate.shape == x.shape and gate.dtype == y.dtype:
+        gs = gate.shape
+        if gs == shape and gate.dtype == y.dtype:
             mode = 2
-        elif tuple(gate.shape) == (D,):
+        elif len(gs) == 1 and gs[0] == D:
             mode, gate_rows = 1, max(rows, 1)
-        elif per_sample:
-            mode, gate_rows = 1, max(rows // max(x.shape[0], 1), 1)
+        elif len(shape) >= 2 and tuple(gs) == (shape[0],) + (1,) * (len(shape) - 2) + (D,):
+            mode, gate_rows = 1, max(rows // max(shape[0], 1), 1)
         else:
             raise L.VpfError(f"gated_norm_residual: gate [D], one row per sample or x's shape in y's type (got {tuple(gate.shape)}, {gate.dtype})")
         if mode == 1 and gate.dtype != F32:
             raise L.VpfError(f"gated_norm_residual: a gate that is shared by rows is fp32 (got {gate.dtype})")
-    wb_post, eps_post = _norm_params("post", post, kind, eps, x)
-    wb_pre, eps_pre = _norm_params("pre", pre, kind, eps, x)
+    wb_post, eps_post = (_NO_PARAMS, eps) if post is None else _norm_params("post", post, kind, eps, x)
+    wb_pre, eps_pre = (_NO_PARAMS, eps) if pre is None else _norm_params("pre", pre, kind, eps, x)
     params = wb_post + wb_pre
     _same_device("gated_norm_residual", x, y, gate, *params)
     cfg = (int(kind == "rms"), mode, gate_rows, int(post is not None), int(pre is not None), float(alpha), float(beta), float(eps_post),
@@ -298,53 +303,52 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
 
 
 # --------------------------------------------------------------------------- attention inside a sliding window
-def _attn_ready(t: torch.Tensor) -> torch.Tensor:
-    """16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8 elements, those of tokens and heads below 2^23;
-    everything else is copied."""
-    sb, sl, sh = _strides(t)
-    if t.stride(3) != 1 or (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or t.data_ptr() & 15:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+def _attn_ready(t: torch.Tensor):
+    """(tensor, its batch, token and head stride).  16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8
+    elements, those of tokens and heads below 2^23; everything else is copied."""
+    st = sb, sl, sh = _strides(t)
+    if (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or t.stride(3) != 1 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _strides(t)
+    return t, st
 
 
-def _attn_args(cfg, q, k, v, pad, lens, out, lse, lo):
-    """The fields both directions share, in front of the gradients' and behind them."""
+def _attn_launch(name, cfg, q, k, v, out, pad, lens, lse, lo, grads, strides, backward):
+    """cfg: (left, right, sinks, scale); grads: (dout, dq, dk, dv); strides: of q, k, v, out, dout, dq, dk, dv in one tuple.  Scratch is asked for,
+    allocated and handed over; it stays alive until the launch is issued (the allocator orders its reuse by stream)."""
     left, right, sinks, scale = cfg
     B, Lq, Hq, dh = q.shape
-    head = (B, Lq, k.shape[1], Hq, k.shape[2], dh, left, right, sinks, _TYPE[q.dtype], scale, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(pad),
-            _ptr(lens), out.data_ptr(), _ptr(lse), _ptr(lo))
-    return head, _strides(q) + _strides(k) + _strides(v) + _strides(out)
-
-
-def _attn_launch(name, head, tail, backward, device):
-    """Scratch is asked for, allocated and handed over; it stays alive until the launch is issued (the allocator orders its reuse by stream)."""
-    n = L.scratch_floats("vpf_window_attn_ws", _pack_attn(*head, 0, 0, *tail), backward)
-    ws = torch.empty(n, dtype=F32, device=device) if n else None
-    L.launch(name, _pack_attn(*head, _ptr(ws), n, *tail), device)
-
-
-_NO_GRAD_PTRS, _NO_GRAD_STRIDES = (0,) * 4, (0,) * 12
-
-
-def _attn_forward(cfg, q, k, v, pad, lens, keep):
-    B, Lq, Hq, dh = q.shape
+    _, Lkv, Hk, _ = k.shape
     dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    head = (B, Lq, Lkv, Hq, Hk, dh, left, right, sinks, _TYPE[q.dtype], scale, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(pad), _ptr(lens),
+            out.data_ptr(), _ptr(lse), _ptr(lo), *grads)
+    packed = _pack_attn(*head, 0, 0, *strides)
+    n = L.scratch_floats("vpf_window_attn_ws", packed, backward)
+    if n:
+        ws = torch.empty(n, dtype=F32, device=dev)
+        packed = _pack_attn(*head, ws.data_ptr(), n, *strides)
+    L.launch(name, packed, dev)
+
+
+_NO_GRADS, _NO_STRIDES = (0,) * 4, (0,) * 12
+
+
+def _attn_forward(cfg, q, k, v, pad, lens, strides, keep):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = lo = None
     if keep:
-        lse = torch.empty(B * Lq * Hq, dtype=F32, device=dev)
-        lo = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    head, tail = _attn_args(cfg, q, k, v, pad, lens, out, lse, lo)
-    _attn_launch("vpf_window_attn_fwd", head + _NO_GRAD_PTRS, tail + _NO_GRAD_STRIDES, 0, dev)
+        lse = torch.empty(q.numel() // q.shape[3], dtype=F32, device=q.device)
+        lo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _attn_launch("vpf_window_attn_fwd", cfg, q, k, v, out, pad, lens, lse, lo, _NO_GRADS, strides + _strides(out) + _NO_STRIDES, 0)
     return out, lse, lo
 
 
 class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, q, k, v, pad, lens):
-        q, k, v = _attn_ready(q), _attn_ready(k), _attn_ready(v)
-        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, True)
-        ctx.cfg = cfg
+        (q, sq), (k, sk), (v, sv) = _attn_ready(q), _attn_ready(k), _attn_ready(v)
+        ctx.cfg, ctx.strides = cfg, sq + sk + sv
+        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, ctx.strides, True)
         ctx.save_for_backward(q, k, v, out, lse, lo, pad, lens)
         return out
 
@@ -352,12 +356,11 @@ class WindowAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         _once("window_attention")
         q, k, v, out, lse, lo, pad, lens = ctx.saved_tensors
-        dout = _attn_ready(dout)
-        dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        head, tail = _attn_args(ctx.cfg, q, k, v, pad, lens, out, lse, lo)
-        _attn_launch("vpf_window_attn_bwd", head + (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
-                     tail + _strides(dout) + _strides(dq) + _strides(dk) + _strides(dv), 1, dev)
+        dout, sd = _attn_ready(dout)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        so, sk = _strides(out), _strides(dk)
+        _attn_launch("vpf_window_attn_bwd", ctx.cfg, q, k, v, out, pad, lens, lse, lo, (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
+                     ctx.strides + so + sd + so + sk + sk, 1)
         return None, dq, dk, dv, None, None
 
 
@@ -375,14 +378,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros, and its (finite) gradient reaches nothing.
     Key heads are shared by heads / key heads consecutive query heads.  head_dim: a multiple of 8 up to 128; scale defaults to head_dim ** -0.5.
     Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v.  There is no dropout on the weights here."""
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[2] < 1 or \
-            q.shape[2] < 1 or q.shape[2] % k.shape[2]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or ks[0] != qs[0] or ks[3] != qs[3] or ks[2] < 1 or qs[2] < 1 or qs[2] % ks[2]:
         raise L.VpfError(f"window_attention: q [B, Lq, heads, head_dim], k and v [B, Lkv, key heads, head_dim], key heads dividing heads (got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)})")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt = q.dtype
+    if (dt is not torch.bfloat16 and dt is not torch.float16) or k.dtype is not dt or v.dtype is not dt:
         raise L.VpfError(f"window_attention: q, k and v all fp16 or all bf16 (got {q.dtype}, {k.dtype}, {v.dtype})")
-    B, Lq, Hq, dh = q.shape
-    Lkv, g = k.shape[1], Hq // k.shape[2]
+    B, Lq, Hq, dh = qs
+    Lkv, g = ks[1], Hq // ks[2]
     if dh % 8 or not 8 <= dh <= 128:
         raise L.VpfError(f"window_attention: head_dim is a multiple of 8 up to 128 (got {dh})")
     if Lq + Lkv >= 1 << 30 or Lq * g * g >= 1 << 31:
@@ -406,5 +410,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     pad = None if pad_mask is None else pad_mask.contiguous().view(torch.uint8)
     lens = None if kv_lens is None else kv_lens.to(torch.int32).contiguous()
     if not _wants_grad(q, k, v):
-        return _attn_forward(cfg, _attn_ready(q), _attn_ready(k), _attn_ready(v), pad, lens, False)[0]
+        (q, sq), (k, sk), (v, sv) = _attn_ready(q), _attn_ready(k), _attn_ready(v)
+        return _attn_forward(cfg, q, k, v, pad, lens, sq + sk + sv, False)[0]
     return WindowAttentionFn.apply(cfg, q, k, v, pad, lens)
