@@ -7,7 +7,7 @@
  * replaces one such composition; the comment above it names the reference lines
  * (relative to the reference repo root) it stands in for.  The Python mirror of
  * the reference interface (vipformer_amd/model/pointcloud/{utils,partseg,classifier}.py)
- * is the only caller; INTEGRATION.md shows the ctypes binding.
+ * and vipformer_amd/ops_block.py are the only callers; INTEGRATION.md shows the ctypes binding.
  *
  * Conventions
  *   - every pointer is a DEVICE pointer unless named host_*; the caller (torch)
