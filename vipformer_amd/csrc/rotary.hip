@@ -8,7 +8,7 @@
 // one sincospi per angle) while its first q / k loads are in flight; what remains is one read and one write of q and k: HBM bound.
 #include "vpf_elem.h"
 
-#define ROT_BYTES 128           // bytes a thread has in flight
+#define ROT_BYTES 64            // bytes a thread has in flight (32, 64, 128, 256: 43, 45, 48, 51 us with 2 x 16 bytes an access, 71, 64, 67, 67 with 16)
 #define ROT_MAX_THREADS 1024
 
 struct RotArgs {
