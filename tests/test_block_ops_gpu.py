@@ -453,6 +453,13 @@ def test_window_attention_every_workgroup_shape(dh, dtype):
         attention_case(B, L, L, Hq, Hk, dh, (40, 0), 3, dtype, pad=pad)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,L,Hq,Hk,dh", [(64, 130, 8, 2, 128), (43, 140, 9, 3, 128), (64, 160, 16, 2, 120), (1, 4100, 32, 8, 128)])
+def test_window_attention_wide_key_tiles_of_shared_heads(B, L, Hq, Hk, dh, dtype):
+    """Gradients over 128-key tiles where the query heads of a key head divide a row block and where they do not."""
+    attention_case(B, L, L, Hq, Hk, dh, (33, 21), 2, dtype)
+
+
 @pytest.mark.parametrize("L,Hq,Hk,dh,window,sinks", [(3000, 2, 1, 64, (0, 0), 600), (2500, 1, 1, 32, (3, 0), 100), (3000, 4, 1, 128, (10, 10), 130)])
 def test_window_attention_many_first_tokens(L, Hq, Hk, dh, window, sinks):
     """First tokens over several key tiles: with pieces of their far rows, and (more than 8 tiles) without."""
