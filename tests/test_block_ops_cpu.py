@@ -164,6 +164,9 @@ def test_window_attention_c_abi_refusals():
     assert fwd(ctypes.byref(make(**{**full, "q": 8})), None) == -2                # not 16-byte aligned
     assert fwd(ctypes.byref(make(**full, k_sl=12)), None) == -2                   # a row stride that is no multiple of 8
     assert bwd(ctypes.byref(make(**full, dv_sh=4)), None) == -2
+    heads = dict(B=1, Hq=1024, Hk=1, ws_floats=1 << 30)                           # 1024 heads of one key head over 2^30 elements
+    for far in (dict(q_sh=1 << 20), dict(do_sh=1 << 20)):
+        assert bwd(ctypes.byref(make(**full, **heads, **far)), None) == -2
     need = ws(ctypes.byref(make()), 1)
     assert need >= 2 * 2 * 10 and ws(ctypes.byref(make(Hk=0)), 1) == -1
     assert bwd(ctypes.byref(make(**full, ws_floats=need - 1)), None) == -1        # refused before anything is launched
@@ -171,3 +174,9 @@ def test_window_attention_c_abi_refusals():
     need = ws(ctypes.byref(make(**step)), 0)
     assert need > 0 and fwd(ctypes.byref(make(**{**step, **full}, ws_floats=need - 1)), None) == -1
     assert fwd(ctypes.byref(make(**{**step, **full, "ws": 0})), None) == -5
+
+
+def test_window_attention_copies_heads_that_lie_too_far_apart():
+    t = torch.empty_strided((1, 3, 1024, 8), (1 << 30, 8, 1 << 20, 1), dtype=torch.float16, device="meta")
+    assert O._attn_ready(t)[1] == (0, 8, 1 << 20) and O._attn_ready(t, 511)[1] == (0, 8, 1 << 20)
+    assert O._attn_ready(t, 512)[1] == O._attn_ready(t, 1024)[1] == (0, 8 * 1024, 8)

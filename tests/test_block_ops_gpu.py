@@ -508,6 +508,22 @@ def test_window_attention_strides_views_scale_and_alignment():
             attention_close(got, *ref[name], name)
 
 
+def test_window_attention_query_heads_far_apart():
+    """512 heads of one key head over 4 GiB: the gradient's kernels have 32-bit offsets inside a stage."""
+    from vipformer_amd.ops_block import window_attention
+    g = gen(11)
+    near, (k, v) = randn(g, 1, 3, 512, 8, dtype=torch.bfloat16), (randn(g, 1, 70, 1, 8, dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    far, dout = (torch.empty(512 << 22, dtype=torch.bfloat16, device="cuda").as_strided((1, 3, 512, 8), (1 << 31, 8, 1 << 22, 1)) for _ in range(2))
+    far.copy_(near)
+    dout.copy_(randn(g, 1, 3, 512, 8, dtype=torch.bfloat16))
+    runs = []
+    for q, d in ((near, dout.contiguous()), (far.detach(), dout)):
+        q.requires_grad_()
+        out = window_attention(q, k, v, (20, 0))
+        runs.append((out.detach(), *torch.autograd.grad(out, (q, k, v), d)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
 def test_window_attention_large_scores_and_growing_maxima():
     """Scores from -300 to 300 whose maximum rises along the keys (the running maximum moves many times) and falls."""
     from vipformer_amd.ops_block import window_attention

@@ -986,7 +986,8 @@ static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
     w.c = a.scale * WA_LOG2E;
     return VPF_OK;
 }
-// 16-byte rows; the offsets inside a stage (up to 128 keys, up to 64 + g rows of queries and heads) are 32-bit byte offsets
+// 16-byte rows; the offsets inside a stage are 32-bit byte offsets: 127 keys' strides below 2^31, and in the dK / dV kernel a row's query
+// (at most 63 of them, 32 where heads share a key head) and head: 2 (2^28 + 2^29) bytes with the heads of a key head below 2^29 elements
 static bool wa_aligned(const void* p, long sb, long sl, long sh)
 {
     return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < VPF_WINDOW_MAX_STRIDE && sh >= 0 && sh < VPF_WINDOW_MAX_STRIDE;
@@ -1163,6 +1164,7 @@ extern "C" int vpf_window_attn_bwd(const VpfWindowAttn* args, void* stream)
         {a.out, a.o_sb, a.o_sl, a.o_sh}, {a.dout, a.do_sb, a.do_sl, a.do_sh}, {a.dq, a.dq_sb, a.dq_sl, a.dq_sh}, {a.dk, a.dk_sb, a.dk_sl, a.dk_sh},
         {a.dv, a.dv_sb, a.dv_sl, a.dv_sh}, {a.out_lo, 0, 0, 0}, {a.ws, 0, 0, 0}};
     for (const auto& x : t) if (!wa_aligned(x.p, x.sb, x.sl, x.sh)) return VPF_ERR_BADALIGN;
+    if (w.g * a.q_sh >= VPF_WINDOW_MAX_HEADS || w.g * a.do_sh >= VPF_WINDOW_MAX_HEADS) return VPF_ERR_BADALIGN;
     wa_plan_bwd(w);
     if (a.ws_floats < wa_bwd_ws(w)) return VPF_ERR_BADSHAPE;
     WA_PICK(wa_bwd, w, (hipStream_t)stream)

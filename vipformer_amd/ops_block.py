@@ -303,11 +303,12 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
 
 
 # --------------------------------------------------------------------------- attention inside a sliding window
-def _attn_ready(t: torch.Tensor):
+def _attn_ready(t: torch.Tensor, shared: int = 0):
     """(tensor, its batch, token and head stride).  16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8
-    elements, those of tokens and heads below 2^23; everything else is copied."""
+    elements, those of tokens and heads below 2^23 and, for a backward pass over ``shared`` heads of a key head, those heads together below
+    2^29; everything else is copied."""
     st = sb, sl, sh = _strides(t)
-    if (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or t.stride(3) != 1 or t.data_ptr() & 15:
+    if (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or shared * sh >= 1 << 29 or t.stride(3) != 1 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         st = _strides(t)
     return t, st
@@ -346,7 +347,7 @@ def _attn_forward(cfg, q, k, v, pad, lens, strides, keep):
 class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, q, k, v, pad, lens):
-        (q, sq), (k, sk), (v, sv) = _attn_ready(q), _attn_ready(k), _attn_ready(v)
+        (q, sq), (k, sk), (v, sv) = _attn_ready(q, q.shape[2] // k.shape[2]), _attn_ready(k), _attn_ready(v)
         ctx.cfg, ctx.strides = cfg, sq + sk + sv
         out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, ctx.strides, True)
         ctx.save_for_backward(q, k, v, out, lse, lo, pad, lens)
@@ -356,7 +357,7 @@ class WindowAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         _once("window_attention")
         q, k, v, out, lse, lo, pad, lens = ctx.saved_tensors
-        dout, sd = _attn_ready(dout)
+        dout, sd = _attn_ready(dout, q.shape[2] // k.shape[2])
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         so, sk = _strides(out), _strides(dk)
         _attn_launch("vpf_window_attn_bwd", ctx.cfg, q, k, v, out, pad, lens, lse, lo, (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
