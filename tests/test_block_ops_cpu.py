@@ -180,3 +180,80 @@ def test_window_attention_copies_heads_that_lie_too_far_apart():
     t = torch.empty_strided((1, 3, 1024, 8), (1 << 30, 8, 1 << 20, 1), dtype=torch.float16, device="meta")
     assert O._attn_ready(t)[1] == (0, 8, 1 << 20) and O._attn_ready(t, 511)[1] == (0, 8, 1 << 20)
     assert O._attn_ready(t, 512)[1] == O._attn_ready(t, 1024)[1] == (0, 8 * 1024, 8)
+
+
+class _Records:
+    """Stands in for the library on the CPU: keeps every argument struct that would be launched; outputs stay unwritten."""
+
+    def __init__(self, monkeypatch):
+        self.calls = []
+        monkeypatch.setattr(O, "_same_device", lambda *a: None)
+        monkeypatch.setattr(L, "launch", lambda name, packed, dev: self.calls.append((name, packed)))
+        monkeypatch.setattr(L, "scratch_floats", lambda *a: 4)
+
+    def last(self, name, cls):
+        assert self.calls[-1][0] == name
+        return cls.from_buffer_copy(self.calls[-1][1])
+
+
+def _packs_elsewhere(kept):
+    """Saved-tensor hooks that bring every tensor back as a copy: contiguous ones (as an offload to the host does) at addresses that are not
+    16-byte aligned, and dimensions in another order in memory."""
+    def plain(t):
+        out = torch.empty(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape).copy_(t)
+        kept.append(out)
+        return out
+
+    def turned(t):
+        order = list(range(t.dim()))[::-1]
+        out = torch.empty([t.shape[i] for i in order], dtype=t.dtype).permute(order).copy_(t)
+        kept.append(out)
+        return out
+    return [(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t), (lambda t: t, plain), (lambda t: t, turned)]
+
+
+def test_window_attention_backward_takes_tensors_as_hooks_bring_them_back(monkeypatch):
+    """Packed q / k / v slices under saved-tensor hooks: the gradient's launch gets strides of the tensors that it is handed."""
+    rec, kept = _Records(monkeypatch), []
+    B, Lq, H, dh = 2, 16, 6, 64
+    for pack, unpack in _packs_elsewhere(kept):
+        qkv = torch.zeros(B, Lq, 3, H, dh, dtype=torch.float16, requires_grad=True)
+        pad, lens = torch.zeros(B, Lq, dtype=torch.bool), torch.full((B,), Lq, dtype=torch.int32)
+        alive = []
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: alive.append(unpack(t)) or alive[-1]):
+            out = O.window_attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], (5, 0), sinks=1, pad_mask=pad, kv_lens=lens)
+            out.backward(torch.zeros_like(out))
+        a = rec.last("vpf_window_attn_bwd", L.WindowAttn)
+        dense = (Lq * H * dh, H * dh, dh)
+        for n in ("q", "k", "v", "o", "do", "dq", "dk", "dv"):
+            assert tuple(getattr(a, f"{n}_{s}") for s in ("sb", "sl", "sh")) == dense, n
+        for n in ("q", "k", "v", "out", "out_lo", "dout"):
+            assert getattr(a, n) % 16 == 0, n
+        assert qkv.grad.shape == qkv.shape
+
+
+def test_rotary_and_gated_norm_backward_take_tensors_as_hooks_bring_them_back(monkeypatch):
+    rec, kept = _Records(monkeypatch), []
+    seen = {}
+    run = O._rotary_run
+    monkeypatch.setattr(O, "_rotary_run", lambda plan, pos, q, k, inverse: seen.update(pos=pos) or run(plan, pos, q, k, inverse))
+    for pack, unpack in _packs_elsewhere(kept):
+        hooks = torch.autograd.graph.saved_tensors_hooks(pack, unpack)
+        q, plan, pos = torch.zeros(2, 5, 4, 32, requires_grad=True), O.RotaryAxes((8, 8), 32), torch.rand(2, 5, 2)
+        with hooks:
+            O.rotary_axes(q, None, pos, plan).sum().backward()
+        assert rec.last("vpf_rotary_axes", L.Rotary).inverse == 1
+        assert seen["pos"].is_contiguous() and torch.equal(seen["pos"], pos)
+        x, w = torch.randn(3, 5, 32, requires_grad=True), torch.randn(32, requires_grad=True)
+        gate = torch.randn(3, 1, 32, requires_grad=True)
+        dense = []
+        ready = O._dense
+        monkeypatch.setattr(O, "_dense", lambda t: dense.append(ready(t)) or dense[-1])
+        with hooks:
+            h, n = O.gated_norm_residual(x, x.detach() + 1, gate=gate, post=(w, None), pre=(w, w))
+            torch.autograd.grad((h, n), (x, gate, w), (h.detach(), n.detach()))
+        monkeypatch.setattr(O, "_dense", ready)
+        a = rec.last("vpf_gated_norm_bwd", L.GatedNorm)
+        assert len(dense) == 8 and [a.x, a.y, a.gate, a.stats, a.w_post, a.b_post, a.w_pre, a.b_pre] == [t if t is None else t.data_ptr() for t in dense]
+        assert all(t is None or t.is_contiguous() for t in dense)
+        assert torch.equal(dense[0], x) and torch.equal(dense[2], gate)

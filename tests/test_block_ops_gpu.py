@@ -840,3 +840,24 @@ def test_offsets_beyond_32_bits():
     ref = norm_ref(x[-16:], x[-16:], None, None, (None, None), "rms", 1.0, 1.0, 1e-5, x[-16:], x[-16:])
     close(h[-16:], ref["h"][0], FWD_N * ref["h"][1], "h")
     close(nn[-16:], ref["n"][0], FWD_N * ref["n"][1], "n")
+
+
+# ------------------------------------------------------------------------------------------ under torch's own machinery
+@pytest.mark.parametrize("pinned", [False, True])
+def test_gradients_of_tensors_that_were_offloaded(pinned):
+    """Saved tensors that travel to the host and back: packed q / k / v slices return contiguous."""
+    from vipformer_amd.ops_block import RotaryAxes, gated_norm_residual, rotary_axes, window_attention
+    g = gen(21)
+    plan, pos = RotaryAxes((16, 16), 64), torch.randint(0, 50, (90, 2), generator=g, device="cuda")
+    qkv, w = randn(g, 2, 90, 3, 6, 64, dtype=torch.bfloat16).requires_grad_(), randn(g, 64).requires_grad_()
+    dout = randn(g, 2, 90, 6, 64, dtype=torch.bfloat16)
+
+    def grads():
+        q, k, v = qkv.unbind(2)
+        out = window_attention(q, k, v, (9, 0), sinks=1) + window_attention(*rotary_axes(q, k, pos, plan), v, (20, 4))
+        h, n = gated_norm_residual(out, v, post=(w, None), pre=(w, None), kind="rms")
+        return torch.autograd.grad((h, n), (qkv, w), (dout, dout))
+    plain = grads()
+    with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
+        moved = grads()
+    assert all(torch.equal(a, b) for a, b in zip(plain, moved))

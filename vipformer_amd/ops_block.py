@@ -55,6 +55,11 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _dense(t):
+    """A saved tensor that was contiguous.  (What a saved-tensor hook brings back has its values and shape; strides and address are its own.)"""
+    return None if t is None else t.contiguous()
+
+
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
     """Batch, token and head stride; 0 where the size is 1 (torch leaves any number there)."""
     sb, sl, sh, _ = t.stride()
@@ -142,7 +147,7 @@ class RotaryAxesFn(torch.autograd.Function):
     def backward(ctx, gq, gk=None):
         _once("rotary_axes")
         (pos,) = ctx.saved_tensors
-        return (None, None) + _rotary_run(ctx.plan, pos, gq, gk, 1)
+        return (None, None) + _rotary_run(ctx.plan, pos.contiguous(), gq, gk, 1)
 
 
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryAxes):
@@ -204,7 +209,7 @@ class GatedNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dh, dn=None):
         _once("gated_norm_residual")
-        x, y, gate, stats, *params = ctx.saved_tensors
+        x, y, gate, stats, *params = map(_dense, ctx.saved_tensors)
         need = ctx.needs_input_grad
         kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = ctx.cfg
         dev, D = x.device, x.shape[-1]
@@ -348,20 +353,23 @@ class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, q, k, v, pad, lens):
         (q, sq), (k, sk), (v, sv) = _attn_ready(q, q.shape[2] // k.shape[2]), _attn_ready(k), _attn_ready(v)
-        ctx.cfg, ctx.strides = cfg, sq + sk + sv
-        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, ctx.strides, True)
+        ctx.cfg = cfg
+        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, sq + sk + sv, True)
         ctx.save_for_backward(q, k, v, out, lse, lo, pad, lens)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _once("window_attention")
-        q, k, v, out, lse, lo, pad, lens = ctx.saved_tensors
-        dout, sd = _attn_ready(dout, q.shape[2] // k.shape[2])
+        q, k, v, *rest = ctx.saved_tensors
+        out, lse, lo, pad, lens = map(_dense, rest)
+        lo = lo.clone() if lo.data_ptr() & 15 else lo
+        g = q.shape[2] // k.shape[2]
+        (q, sq), (k, sk), (v, sv), (out, so), (dout, sd) = _attn_ready(q, g), _attn_ready(k), _attn_ready(v), _attn_ready(out), _attn_ready(dout, g)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        so, sk = _strides(out), _strides(dk)
+        sdq, sdk = _strides(dq), _strides(dk)
         _attn_launch("vpf_window_attn_bwd", ctx.cfg, q, k, v, out, pad, lens, lse, lo, (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
-                     ctx.strides + so + sd + so + sk + sk, 1)
+                     sq + sk + sv + so + sd + sdq + sdk + sdk, 1)
         return None, dq, dk, dv, None, None
 
 
