@@ -257,3 +257,27 @@ def test_rotary_and_gated_norm_backward_take_tensors_as_hooks_bring_them_back(mo
         assert len(dense) == 8 and [a.x, a.y, a.gate, a.stats, a.w_post, a.b_post, a.w_pre, a.b_pre] == [t if t is None else t.data_ptr() for t in dense]
         assert all(t is None or t.is_contiguous() for t in dense)
         assert torch.equal(dense[0], x) and torch.equal(dense[2], gate)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A tangent that would be dropped raises as it does for every Function without a forward-mode rule, also where no gradient is recorded."""
+    from torch.autograd import forward_ad
+    rec = _Records(monkeypatch)
+    q, x, w, pos = torch.zeros(1, 4, 2, 32, dtype=torch.float16), torch.ones(2, 3, 32), torch.ones(32), torch.zeros(4, 2)
+    plan = O.RotaryAxes((8, 8), 32)
+    calls = {
+        "rotary q": lambda d: O.rotary_axes(d(q), q, pos, plan), "rotary k": lambda d: O.rotary_axes(q, d(q), pos, plan),
+        "rotary positions": lambda d: O.rotary_axes(q, q, d(pos), plan),
+        "attention q": lambda d: O.window_attention(d(q), q, q), "attention k": lambda d: O.window_attention(q, d(q), q),
+        "attention v": lambda d: O.window_attention(q, q, d(q)),
+        "norm x": lambda d: O.gated_norm_residual(d(x), x), "norm y": lambda d: O.gated_norm_residual(x, d(x), pre=(None, None)),
+        "norm gate": lambda d: O.gated_norm_residual(x, x, gate=d(w)), "norm weight": lambda d: O.gated_norm_residual(x, x, post=(d(w), None)),
+    }
+    for name, call in calls.items():
+        for context in (torch.enable_grad, torch.no_grad):
+            with forward_ad.dual_level(), context():
+                with pytest.raises(NotImplementedError, match="forward mode"):
+                    call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+                n = len(rec.calls)
+                call(lambda t: t)                                              # no tangent among the inputs: as ever
+                assert len(rec.calls) == n + 1, name

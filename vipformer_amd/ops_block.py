@@ -7,7 +7,7 @@ LayerNorm and residual pieces of ops.py:
 
 Heads are a dimension of their own ([B, L, heads, head_dim], any strides whose last dimension is contiguous: slices of one projection's
 output go in as they are).  fp16 and bf16 are chosen by the tensors, per call; the library's build-time operand type does not matter here.
-Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once, and may be captured into a HIP graph once
+Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once (backward mode), and may be captured into a HIP graph once
 it has run there (a RotaryAxes makes its tables at its first use on a device).  As everywhere in torch, a backward pass is captured only while no
 eager graph of the same leaves is alive (train.GraphedStep).
 """
@@ -17,6 +17,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import ops
@@ -38,6 +39,10 @@ def _same_device(what: str, first: torch.Tensor, *rest) -> None:
 
 
 def _wants_grad(*ts) -> bool:
+    """Does the call go through its autograd Function?  A tensor with a tangent need not require a gradient: while a forward-mode level is open the
+    Function decides (it has no forward-mode rule, so torch raises where one is needed)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
