@@ -281,3 +281,17 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
                 n = len(rec.calls)
                 call(lambda t: t)                                              # no tangent among the inputs: as ever
                 assert len(rec.calls) == n + 1, name
+
+
+@pytest.mark.parametrize("x,y", [(torch.float32, torch.float16), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)])
+def test_modules_without_an_epsilon_get_the_one_of_fp32(monkeypatch, x, y):
+    """torch.nn.RMSNorm's default; its own outputs in 16 bits bear out that it is fp32's."""
+    rec, rms = _Records(monkeypatch), torch.nn.RMSNorm(32, elementwise_affine=False)
+    O.gated_norm_residual(torch.zeros(2, 32, dtype=x), torch.zeros(2, 32, dtype=y), post=rms, pre=rms, kind="rms")
+    a = rec.last("vpf_gated_norm_fwd", L.GatedNorm)
+    eps = torch.finfo(torch.float32).eps
+    assert a.eps_post == a.eps_pre == eps
+    z = (torch.randn(8, 32) * 0.01).to(y)
+    ref = z.double() * torch.rsqrt((z.double() ** 2).mean(-1, keepdim=True) + eps)
+    # half a step of the output and 32 fp32 roundings of terms of one sign, each at most 2^-24
+    assert ((rms(z).double() - ref).abs() <= ref.abs() * (torch.finfo(y).eps / 2 + 32 * 2.0 ** -24)).all()

@@ -861,3 +861,25 @@ def test_gradients_of_tensors_that_were_offloaded(pinned):
     with torch.autograd.graph.save_on_cpu(pin_memory=pinned):
         moved = grads()
     assert all(torch.equal(a, b) for a, b in zip(plain, moved))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "fp16", "bf16"])
+@pytest.mark.parametrize("scale", [0.05, 0.003])
+def test_gated_norm_default_epsilon_of_rms_modules(dtype, scale):
+    """RMSNorm(D) without an epsilon, behind and in front of a block, on small activations: the module's own formula with fp32's epsilon, and
+    the module's own output on the same inputs."""
+    from vipformer_amd.ops_block import gated_norm_residual
+    g, dt, eps = gen(22), TYPES[dtype], torch.finfo(torch.float32).eps
+    z, zero = randn(g, 40, 256, dtype=dt, scale=scale), torch.zeros(40, 256, dtype=dt, device="cuda")
+    rms = torch.nn.RMSNorm(256, device="cuda")
+    with torch.no_grad():
+        rms.weight.copy_(1.0 + randn(g, 256, scale=0.2))
+        h, _ = gated_norm_residual(zero, z, post=rms, kind="rms")
+        h2, n = gated_norm_residual(z, zero, pre=rms, kind="rms")
+        own = rms(z.float())
+    assert torch.equal(h2, z)
+    for got, post, pre, (a, b), name in ((h, (rms.weight, None), None, (zero, z), "h"), (n, None, (rms.weight, None), (z, zero), "n")):
+        ref = norm_ref(a, b, None, post, pre, "rms", 1.0, 1.0, eps, zero, zero)
+        close(got, ref[name][0], FWD_N * ref[name][1], name)
+        # torch's module in fp32 on the same values carries no more roundings than the kernel
+        close(got, own.double(), 2 * FWD_N * ref[name][1], "module")

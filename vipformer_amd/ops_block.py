@@ -256,7 +256,7 @@ def _norm_params(what, wb, kind, eps, x):
         want = {"layer": torch.nn.LayerNorm, "rms": torch.nn.RMSNorm}[kind]
         if not isinstance(wb, want) or tuple(wb.normalized_shape) != (x.shape[-1],):
             raise L.VpfError(f"gated_norm_residual: {what}: a {want.__name__} over {x.shape[-1]} channels for kind {kind!r} (got {wb})")
-        eps = torch.finfo(x.dtype).eps if wb.eps is None else wb.eps
+        eps = torch.finfo(F32).eps if wb.eps is None else wb.eps        # (what torch's module uses for fp32, fp16 and bf16 inputs alike)
         wb = (wb.weight, getattr(wb, "bias", None))
     if len(wb) != 2:
         raise L.VpfError(f"gated_norm_residual: {what} is a norm module or (weight, bias)")
