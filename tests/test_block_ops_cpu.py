@@ -295,3 +295,19 @@ def test_modules_without_an_epsilon_get_the_one_of_fp32(monkeypatch, x, y):
     ref = z.double() * torch.rsqrt((z.double() ** 2).mean(-1, keepdim=True) + eps)
     # half a step of the output and 32 fp32 roundings of terms of one sign, each at most 2^-24
     assert ((rms(z).double() - ref).abs() <= ref.abs() * (torch.finfo(y).eps / 2 + 32 * 2.0 ** -24)).all()
+
+
+def test_a_gate_parameter_that_is_not_contiguous_is_a_parameter(monkeypatch):
+    """Its gradient leaves an internal gradient scale like any other parameter's, though the kernel works on a copy of it."""
+    from vipformer_amd import ops
+    _Records(monkeypatch)
+    monkeypatch.setattr(torch, "empty_like", torch.ones_like)                   # (the kernels write nothing here: every gradient reads 1)
+    x = torch.ones(4, 32, requires_grad=True)
+    for make, want in ((lambda t: torch.nn.Parameter(t), 0.25), (lambda t: t.requires_grad_(), 1.0)):
+        for gate in (make(torch.ones(32)), make(torch.ones(64)[::2]), make(torch.ones(32, 4).t()), make(torch.ones(4, 32))):
+            with ops.internal_grad_scale() as holder:
+                h, _ = O.gated_norm_residual(x, x.detach(), gate=gate)
+            if holder.on:
+                holder.inv = torch.tensor(0.25)
+            (dgate,) = torch.autograd.grad(h, (gate,), torch.ones(4, 32))
+            assert dgate.shape == gate.shape and torch.equal(dgate, torch.full_like(dgate, want if holder.on else 1.0)), gate.stride()

@@ -205,9 +205,9 @@ class GatedNormFn(torch.autograd.Function):
     """Gradients of parameters go back through autograd, divided by the internal gradient scale the forward ran under (ops.py)."""
 
     @staticmethod
-    def forward(ctx, cfg, x, y, gate, *params):
+    def forward(ctx, cfg, gate_is_param, x, y, gate, *params):
         h, n, stats = _norm_forward(cfg, x, y, gate, params, True)
-        ctx.cfg, ctx.iscale, ctx.gate_is_param = cfg, ops._current_iscale(), isinstance(gate, torch.nn.Parameter)
+        ctx.cfg, ctx.iscale, ctx.gate_is_param = cfg, ops._current_iscale(), gate_is_param
         ctx.save_for_backward(x, y, gate, stats, *params)
         return (h, n) if n is not None else h
 
@@ -215,11 +215,11 @@ class GatedNormFn(torch.autograd.Function):
     def backward(ctx, dh, dn=None):
         _once("gated_norm_residual")
         x, y, gate, stats, *params = map(_dense, ctx.saved_tensors)
-        need = ctx.needs_input_grad
+        need = ctx.needs_input_grad[1:]
         kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = ctx.cfg
         dev, D = x.device, x.shape[-1]
         if x.numel() == 0:
-            return (None, *(torch.zeros_like(t) if t is not None and n else None for t, n in zip((x, y, gate, *params), need[1:])))
+            return (None, None, *(torch.zeros_like(t) if t is not None and n else None for t, n in zip((x, y, gate, *params), need[1:])))
         dh = dh.contiguous()
         dn = None if dn is None else dn.contiguous()
         dx = torch.empty_like(x) if need[1] else None
@@ -244,7 +244,7 @@ class GatedNormFn(torch.autograd.Function):
                 flat.mul_(inv)
             if dgate is not None and ctx.gate_is_param:
                 dgate.mul_(inv)
-        return (None, dx, dy, dgate, *grads)
+        return (None, None, dx, dy, dgate, *grads)
 
 
 _NO_PARAMS = (None, None)
@@ -305,10 +305,11 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
     _same_device("gated_norm_residual", x, y, gate, *params)
     cfg = (int(kind == "rms"), mode, gate_rows, int(post is not None), int(pre is not None), float(alpha), float(beta), float(eps_post),
            float(eps_pre))
+    gate_is_param = isinstance(gate, torch.nn.Parameter)         # (before a copy of it takes its place)
     x, y, gate = x.contiguous(), y.contiguous(), None if gate is None else gate.contiguous()
     if not _wants_grad(x, y, gate, *params):
         return _norm_forward(cfg, x, y, gate, params, False)[:2]
-    out = GatedNormFn.apply(cfg, x, y, gate, *params)
+    out = GatedNormFn.apply(cfg, gate_is_param, x, y, gate, *params)
     return out if pre is not None else (out, None)
 
 
