@@ -573,9 +573,10 @@ long vpf_gated_norm_ws(const VpfGatedNorm* a);
 /* Attention inside a sliding window with first tokens that stay visible.  n = lens[b] (clamped to 0 .. Lkv; null: Lkv) keys are in use;
  * query i stands at position p = n - Lq + i (the last query at the last key in use) and sees key j where
  *   j < n,  j <= p + right,  (j >= p - left or j < sinks),  pad[b, j] == 0        (left / right < 0: open on that side; causal: right = 0)
- * out = softmax(scale * q k^T over the visible keys) v; a query that sees no key gets zeros and passes no gradient.  Keys and values that
- * no query sees (behind n, padding, slid out of the window) are never used: they may hold anything, also NaN.  (A value that is not finite in a
- * key that some query sees reaches the queries around it, as 0 * NaN does in the product.)
+ * out = softmax(scale * q k^T over the visible keys) v; a query that sees no key gets zeros and passes no gradient, whatever it and its
+ * gradient hold.  Keys and values that no query sees (behind n, padding, slid out of the window) are never used: they may hold anything, also
+ * NaN.  (A value that is not finite in a key that some query sees reaches the queries around it, as 0 * NaN does in the product; one in a query
+ * that sees some key, or in its gradient, reaches the dk and dv of the keys around.)
  * q, out, dout, dq [B, Lq, Hq, head_dim]; k, v, dk, dv [B, Lkv, Hk, head_dim]: fp16 or bf16, 16-byte aligned, strides multiples of 8;
  * Hk divides Hq, query heads h Hq / Hk .. share key head h.  head_dim a multiple of 8 up to 128.  pad uint8 [B, Lkv], lens int32 [B] (device).
  * lse fp32 [B, Hk, Lq * Hq / Hk]: log2 of the sum of the exponentials (+inf: nothing visible); forward writes it (null: no gradient follows).

@@ -883,3 +883,33 @@ def test_gated_norm_default_epsilon_of_rms_modules(dtype, scale):
         close(got, ref[name][0], FWD_N * ref[name][1], name)
         # torch's module in fp32 on the same values carries no more roundings than the kernel
         close(got, own.double(), 2 * FWD_N * ref[name][1], "module")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lkv,Hq,Hk,dh,window,sinks", [
+    (3, 70, 70, 4, 2, 64, (0, 0), 0), (2, 200, 40, 6, 2, 72, (9, 0), 2), (64, 130, 130, 9, 3, 128, (0, 0), 1), (1, 900, 900, 2, 1, 32, (1, 1), 3),
+    (3, 300, 300, 8, 1, 96, (None, 0), 0)])
+def test_window_attention_queries_that_see_nothing_hold_anything(B, Lq, Lkv, Hq, Hk, dh, window, sinks, dtype):
+    """Queries in front of the first key and queries whose every key is padding, with NaN and infinities in them and in their gradients."""
+    from vipformer_amd.ops_block import window_attention
+    g, dt = gen(23 + dh), TYPES[dtype]
+    q, k, v = randn(g, B, Lq, Hq, dh, dtype=dt), randn(g, B, Lkv, Hk, dh, dtype=dt), randn(g, B, Lkv, Hk, dh, dtype=dt)
+    dout = randn(g, B, Lq, Hq, dh, dtype=dt)
+    pad = torch.rand(B, Lkv, generator=g, device="cuda") < 0.5
+    lens = torch.randint(Lkv // 2, Lkv + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    mask = seen_mask(B, Lq, Lkv, window, sinks, pad, lens)
+    blind = ~mask.any(-1)
+    assert blind.any() and not blind.all()
+    for t, what in ((q, (math.nan, math.inf)), (dout, (-math.inf, math.nan))):
+        t[blind] = what[0]
+        t[:, ::3][blind[:, ::3]] = what[1]
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = window_attention(q, k, v, window, sinks=sinks, pad_mask=pad, kv_lens=lens)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    zeroed = lambda t: torch.where(blind[..., None, None], 0.0, t.detach())
+    ref = attention_ref(zeroed(q), k, v, mask, dh ** -0.5, zeroed(dout))
+    attention_close(out.detach(), *ref["out"], "out")
+    for got, name in zip(grads, ("dq", "dk", "dv")):
+        attention_close(got, *ref[name], name)
+    assert float(out.detach()[blind].abs().sum()) == 0.0 and float(grads[0][blind].abs().sum()) == 0.0

@@ -578,6 +578,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
         delta = wa_half_sum(delta);
     }
     const float lse = a.lse[(size_t)bh * w.rows + rq];
+    if (lse == INFINITY) delta = 0.f;                                        // a row that sees nothing: whatever its gradient holds
     const char* kp = (const char*)((const T*)a.k + b * a.k_sb + hk * a.k_sh);
     const char* vp = (const char*)((const T*)a.v + b * a.v_sb + hk * a.v_sh);
     const uint8_t* pad = a.pad ? (const uint8_t*)a.pad + (size_t)b * a.Lkv : nullptr;
@@ -728,7 +729,10 @@ __device__ __forceinline__ WaRowRange wa_rows_of(const WaArgs& w, const WaSeen& 
     return r;
 }
 
-template <typename T, int DP, int KB>
+// BLIND: the call can have rows that see nothing (wa_blind).  They may hold anything, and 0 * NaN is NaN: their Q and dO become zeros in front of
+// the products.  A variant of its own, since around that look at every stage the compiler orders the products' reads worse (us without / with it:
+// 8192 queries, 16 + 4 heads of 128, window 2048 306 / 340; 5 x 777, 6 + 2 heads of 80, window 128 25.0 / 26.8).
+template <typename T, int DP, int KB, bool BLIND>
 __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
@@ -816,7 +820,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
             wa_dma(qb, (uint32_t)(qi * (int)a.q_sl + h * (int)a.q_sh) * (uint32_t)sizeof(T) + stage.col, at + stage.wave_byte + i * stage.ALL);
             wa_dma(gb, (uint32_t)(qi * (int)a.do_sl + h * (int)a.do_sh) * (uint32_t)sizeof(T) + stage.col, at + BUF + stage.wave_byte + i * stage.ALL);
         }
-        const int rc = min(lane, w.rows - 1 - r0);
+        const int rc = min(lane, last);                                      // (rows behind the range: its last one again, as in the stage)
         const uint32_t stat = stats_at + buf * 3 * ROWS * 4;
         if (wave == 0) wa_dma4(a.lse + (size_t)bh * w.rows + r0, 4 * rc, stat);
         if (wave == 1) wa_dma4(a.ws + (size_t)bh * w.rows + r0, 4 * rc, stat + 4 * ROWS);
@@ -831,6 +835,16 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
     __syncthreads();
     for (int t = 0; t < steps; ++t) {
         if (t + 1 < steps) load(block(t + 1), (t + 1) & 1);
+        if constexpr (BLIND) {                                               // (every wave finds the same rows)
+            if (const uint64_t blind = __ballot(stats[(t & 1) * 3 * ROWS + (wa_opaque(threadIdx.x) & 63)] == INFINITY)) {
+                for (int i = wa_opaque(threadIdx.x); i < ROWS * Tile::NC; i += KB * 128)
+                    if (blind >> (i / Tile::NC) & 1) {
+                        char* const at = lds + (t & 1) * 2 * BUF + i * 16;
+                        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(at + BUF) = make_uint4(0, 0, 0, 0);
+                    }
+                __syncthreads();
+            }
+        }
         const uint32_t sq = tiles_at + (t & 1) * 2 * BUF + 32 * qs * Tile::PITCH, qrow = wa_opaque(row_base + sq), qcol = wa_opaque(col_base + sq);
         const uint32_t vrow = VREG ? 0 : wa_opaque(row_base + tiles_at + 4 * BUF + 32 * kb * Tile::PITCH);
         const float* st = stats + (t & 1) * 3 * ROWS + 32 * qs + 4 * hl;
@@ -1001,6 +1015,8 @@ static int wa_row_blocks(const WaArgs& w)
 }
 // Walks of one length: the window leaves most of the keys out, so few tiles are cut short by the ends of the sequence.
 static int wa_runs(const WaArgs& w) { return (long)w.a.B * w.a.Hk < 8 && ((long)w.a.left + w.a.right) * 2 < w.a.Lkv; }
+// Can a row see nothing?  Not where every query stands at a key that is in use and no padding.
+static bool wa_blind(const WaArgs& w) { return w.a.pad || w.a.lens || w.a.Lq > w.a.Lkv; }
 // Where even single row blocks are too few, the keys are divided as well: one workgroup per CU (a stage of 128 keys is up to 64 KB of loads in flight),
 // each with at least two stages, and at most 64 parts (a wave of the join).
 static void wa_plan_fwd(WaArgs& w, int& rb)
@@ -1107,9 +1123,14 @@ template <typename T, int DP> static int wa_bwd(WaArgs& w, hipStream_t st)
         hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(128 * kb), lds, st, w);
         return VPF_OK;
     };
-    static VpfPerDevice done2, done4;
-    if constexpr (DP == 128) { if (w.key_tile == 128) { if (const int rc = launch(wa_dkv_kernel<T, DP, 4>, 4, done4)) return rc; } }
-    if (w.key_tile == 64) { if (const int rc = launch(wa_dkv_kernel<T, DP, 2>, 2, done2)) return rc; }
+    static VpfPerDevice done2, done4, done2b, done4b;
+    const bool blind = wa_blind(w);
+    if constexpr (DP == 128) {
+        if (w.key_tile == 128)
+            if (const int rc = blind ? launch(wa_dkv_kernel<T, DP, 4, true>, 4, done4b) : launch(wa_dkv_kernel<T, DP, 4, false>, 4, done4)) return rc;
+    }
+    if (w.key_tile == 64)
+        if (const int rc = blind ? launch(wa_dkv_kernel<T, DP, 2, true>, 2, done2b) : launch(wa_dkv_kernel<T, DP, 2, false>, 2, done2)) return rc;
     if (w.chunks) {
         hipLaunchKernelGGL((wa_sink_join_kernel<T, DP>), dim3((unsigned)(bh * w.a.sinks)), dim3(2 * DP), 0, st, w);
     }

@@ -390,7 +390,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     on the device, read by the kernels: a captured graph follows it): a preallocated cache that is filled to different lengths.
     pad_mask: bool [B, Lkv], True = this key is padding (as the ``pad_mask`` of the framework's encoders); it moves no positions.
     Keys that no query sees may hold anything, also NaN; a value that is not finite in a key that some query sees reaches the queries around it, as
-    0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros, and its (finite) gradient reaches nothing.
+    0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros; it and its gradient may hold anything and reach
+    nothing.  (In the gradients of keys and values, what is not finite in a query that sees some key, or in its gradient, reaches the keys around.)
     Key heads are shared by heads / key heads consecutive query heads.  head_dim: a multiple of 8 up to 128; scale defaults to head_dim ** -0.5.
     Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v.  There is no dropout on the weights here."""
     qs, ks = q.shape, k.shape
