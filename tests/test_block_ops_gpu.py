@@ -913,3 +913,42 @@ def test_window_attention_queries_that_see_nothing_hold_anything(B, Lq, Lkv, Hq,
     for got, name in zip(grads, ("dq", "dk", "dv")):
         attention_close(got, *ref[name], name)
     assert float(out.detach()[blind].abs().sum()) == 0.0 and float(grads[0][blind].abs().sum()) == 0.0
+
+
+def small_steps_close(got, ref, size, flushed, what):
+    """attention_close without its absolute terms: half a step of the result (and of fp16's smallest numbers, 2^-25), 8 standard deviations of the
+    weights' roundings, and `flushed`: what weights below the smallest number of their scaled fp16 form can add up to."""
+    half = torch.finfo(got.dtype).eps / 2
+    tol = half * ref.abs() + 8 * half * size + 2.0 ** -25 + flushed
+    bad = (got.double() - ref).abs() - tol
+    assert got.shape == ref.shape and torch.isfinite(got.double()).all(), what
+    assert float(bad.max()) <= 0.0, f"{what}: {int((bad > 0).sum())} of {bad.numel()} outside, worst {float((got.double() - ref).abs().max()):.3e}"
+
+
+@pytest.mark.parametrize("B,Lq,Lkv,Hq,Hk,dh,window,gsize,vsize,ksize,rows", [
+    (1, 2048, 2048, 1, 1, 64, (None, None), 1e-4, 1.0, 1.0, False), (1, 300, 8192, 2, 1, 128, (None, None), 1e-3, 1.0, 1.0, False),
+    (1, 300, 8192, 4, 2, 96, (None, None), 1e-4, 1.0, 1.0, False), (64, 200, 200, 4, 4, 128, (None, 0), 1e-5, 1.0, 1.0, True),
+    (16, 190, 190, 8, 8, 32, (40, 3), 1e-2, 1.0, 1.0, True), (2, 777, 777, 6, 2, 64, (100, 0), 1.0, 1.0, 1.0, True),
+    (1, 70, 70, 2, 1, 64, (5, 0), 300.0, 100.0, 2e-4, False), (32, 190, 190, 8, 8, 64, (33, 21), 500.0, 200.0, 1e-4, True)])
+def test_window_attention_fp16_gradients_of_any_size(B, Lq, Lkv, Hq, Hk, dh, window, gsize, vsize, ksize, rows):
+    """dS is rounded to fp16 for its products: over many keys it lies far below fp16's smallest numbers, with large values and gradients far beyond
+    its largest, while dq and dk are ordinary.  `rows`: gradients that differ by 10^4 from query to query."""
+    from vipformer_amd.ops_block import window_attention
+    g, dt = gen(24 + Lq), torch.float16
+    q, k, v = randn(g, B, Lq, Hq, dh, dtype=dt), randn(g, B, Lkv, Hk, dh, scale=ksize, dtype=dt), randn(g, B, Lkv, Hk, dh, scale=vsize, dtype=dt)
+    q = (q.float() * (1.0 if ksize == 1.0 else 0.1)).to(dt)
+    dout = randn(g, B, Lq, Hq, dh, scale=gsize)
+    if rows:
+        dout = dout * 10.0 ** -(torch.arange(Lq, device="cuda") % 5)[:, None, None]
+    dout = dout.to(dt)
+    for t in (q, k, v):
+        t.requires_grad_()
+    mask, scale = seen_mask(B, Lq, Lkv, window, 0, None, None), dh ** -0.5
+    ref = attention_ref(q, k, v, mask, scale, dout)
+    out = window_attention(q, k, v, window)
+    dq, dk, _ = torch.autograd.grad(out, (q, k, v), dout)
+    # scaled weights of a row or a key: its largest at 2^10 or more, the smallest step 2^-24 -- half of that for each of n terms, 8 deviations
+    most = 2.0 * float(dout.abs().double().sum(-1).max() * v.detach().abs().max())
+    flushed = lambda n, t: 8 * 2.0 ** -35 * most * scale * math.sqrt(n) * float(t.detach().abs().max())
+    small_steps_close(dq, *ref["dq"], flushed(Lkv, k), "dq")
+    small_steps_close(dk, *ref["dk"], flushed(Lq * Hq // Hk, q), "dk")

@@ -28,10 +28,12 @@ typedef __attribute__((ext_vector_type(16))) float wa_f32x16;
 
 template <typename T> struct WaMma;
 template <> struct WaMma<vpf_f16> {
+    static constexpr bool NARROW = true;    // 5 bits of exponent: what is rounded to it for a product is scaled first
     typedef __attribute__((ext_vector_type(8))) vpf_f16 v8;
     static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct WaMma<vpf_bf16> {
+    static constexpr bool NARROW = false;
     typedef __attribute__((ext_vector_type(8))) vpf_bf16 v8;
     static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -528,6 +530,28 @@ __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
 // ------------------------------------------------------------------ backward: queries
 // dS = P (dP - delta), dP = dO V^T, delta = sum of P dP = rowsum(dO . O);  dQ = scale dS K.  The walk over the keys is the forward kernel's.  dS is
 // rounded to the tensors' type for its product, as P is.
+// fp16 does not hold dS as it is: with gradients of 10^-4 over 2048 keys most of it lies below 2^-24, and |dP - delta| can pass 65504 where dq does
+// not.  A row here (a key in the kernel of the keys) carries a power of two for its dS, which starts at 2^WA_UP and falls whenever the row's largest
+// |dS| would pass 2^15 of it, to bring that to 2^10 .. 2^11; its sums fall with it, so nothing is rounded by it.  What then lies below fp16's
+// smallest numbers is 2^-35 of the row's largest.  It costs (fp16, us, dQ and dK / dV kernel without / with): 16 x 1025, 6 heads of 64, window 257
+// 39.8 / 41.1 and 40.7 / 43.3; 8192 queries, 16 + 4 heads of 128, window 2048 264 / 270 and 312 / 343.
+#define WA_UP 64
+#define WA_TOP 32768.f
+__device__ __forceinline__ int wa_fall(float largest) { return largest > WA_TOP ? min(0, 11 - __builtin_amdgcn_frexp_expf(largest)) : 0; }
+__device__ __forceinline__ float wa_largest(const float* v)                  // |v| of 16 values of the lane and of its partner
+{
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) m = fmaxf(m, fabsf(v[r]));
+    return wa_half_max(m);
+}
+template <int N> __device__ __forceinline__ void wa_scale(wa_f32x16* acc, int e)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = __builtin_ldexpf(acc[i][r], e);
+}
 // delta comes in three qualities.  rowsum(dO . O) is there before the walk, with O as forward had it before rounding (out + out_lo; with the
 // rounded O the error of dq against 64 bits was 1.6 instead of 1.4 times the output's own rounding); what is left in it is the rounding of
 // forward's weights, 1 / sqrt(keys) of dS's own rounding.  Where rows see few keys (WA_FEW) the walk is therefore made twice, first for
@@ -538,6 +562,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int SUBK = KS == 1 ? 64 : 32, STAGE = SUBK * KS, KST = DP / 16, DT = DP / 32, NB = SUBK / 32, BUF = STAGE * Tile::PITCH;
+    constexpr bool NARROW = WaMma<T>::NARROW;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const VpfWindowAttn& a = w.a;
     uint32_t* const pads = reinterpret_cast<uint32_t*>(lds + 4 * BUF);     // [2][STAGE / 32]: a bit for every key that is not padding
@@ -610,7 +635,8 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     auto keys_of = [&](int p) { const int lo = max(0, p - a.left); return min(p + a.right, seen.n - 1) + 1 - lo + min(a.sinks, lo); };
     const bool twice = min(keys_of(seen.off + wa_query(w, r0)), keys_of(seen.off + wa_query(w, rend - 1))) <= WA_FEW;
     const int steps = twice ? 2 * stages : stages;
-    float pdp = 0.f;
+    float pdp = 0.f, lsu = NARROW && !twice ? lse - WA_UP : lse;             // (exp2(.. - lsu): the weight times the row's power of two)
+    int up = WA_UP;
     auto joined = [&](float v) {                                             // over the lane pair and the key parts
         v = wa_half_sum(v);
         if constexpr (KS > 1) {
@@ -651,13 +677,24 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = wa_exp2(fmaf(s[r], w.c, -lse));
+                const float p = wa_exp2(fmaf(s[r], w.c, -lsu));
                 float x = p * dp[r];
                 if (!all) x = s[r] == -INFINITY ? 0.f : x;                   // what a hidden key holds stays out
                 pdp += x;
                 ds[r] = fmaf(-p, delta, x);
             }
             if (first) continue;
+            if constexpr (NARROW) {
+                const float largest = wa_largest(ds);
+                if (__any(largest > WA_TOP)) {
+                    const int e = wa_fall(largest);
+                    up += e; lsu -= (float)e;
+                    pdp = __builtin_ldexpf(pdp, e);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] = __builtin_ldexpf(ds[r], e);
+                    wa_scale<DT>(dq, e);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const typename WaMma<T>::v8 df = wa_pack8<T>(ds + 8 * i);
@@ -665,11 +702,12 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
                 for (int dt = 0; dt < DT; ++dt) dq[dt] = WaMma<T>::mma(wa_frag_col<T, DP>(kcol, dt, (32 * kb + 16 * i) * Tile::PITCH), df, dq[dt]);
             }
         }
-        if (first && step + 1 == stages) { delta = joined(pdp); pdp = 0.f; }
+        if (first && step + 1 == stages) { delta = joined(pdp); pdp = 0.f; if (NARROW) lsu = lse - WA_UP; }
         wa_stage_wait<0>();
         __syncthreads();
     }
-    if (!twice) delta = joined(pdp);
+    if (!twice) delta = joined(NARROW ? __builtin_ldexpf(pdp, -up) : pdp);
+    if constexpr (NARROW) wa_scale<DT>(dq, -up);
     if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
     if (KS > 1) {
         float* slots = reinterpret_cast<float*>(lds);
@@ -732,12 +770,13 @@ __device__ __forceinline__ WaRowRange wa_rows_of(const WaArgs& w, const WaSeen& 
 // BLIND: the call can have rows that see nothing (wa_blind).  They may hold anything, and 0 * NaN is NaN: their Q and dO become zeros in front of
 // the products.  A variant of its own, since around that look at every stage the compiler orders the products' reads worse (us without / with it:
 // 8192 queries, 16 + 4 heads of 128, window 2048 306 / 340; 5 x 777, 6 + 2 heads of 80, window 128 25.0 / 26.8).
+// Up to head dimension 64 three waves fit a SIMD (168 registers); two take 47 us instead of 41 at 16 x 1025, 6 heads of 64, window 257.
 template <typename T, int DP, int KB, bool BLIND>
-__global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
+__global__ void __launch_bounds__(KB * 128, DP <= 64 ? 3 : 2) wa_dkv_kernel(WaArgs w)
 {
     using Tile = WaTile<DP>;
     constexpr int ROWS = WA_ROWS, KST = DP / 16, DT = DP / 32, BUF = ROWS * Tile::PITCH, KT = KB * 32;
-    constexpr bool VREG = DP <= 96;
+    constexpr bool VREG = DP <= 96, NARROW = WaMma<T>::NARROW;
     extern __shared__ __attribute__((aligned(1024))) char lds[];               // [2][Q, dO][64 rows], V [KT] (!VREG), [2][lse, delta, position][64]
     const VpfWindowAttn& a = w.a;
     float* const stats = reinterpret_cast<float*>(lds + 4 * BUF + (VREG ? 0 : KT * Tile::PITCH));
@@ -773,6 +812,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
     wa_f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) { dk[dt] = wa_zero16(); dv[dt] = wa_zero16(); }
+    float up = __builtin_ldexpf(1.f, WA_UP);                                 // the key's power of two (fp16: see wa_dq_kernel)
     const int kmin = kt0 + 32 * kb, kmax = kmin + 31;
     const bool whole = !pad && kmax < seen.n;
     // the positions that see the lane's key are key - right .. key + left (a first token: no upper end; a hidden key: none): one unsigned comparison
@@ -871,7 +911,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * j + e;
                     p[r] = wa_exp2(fmaf(s[r], w.c, -ls[e]));
-                    ds[r] = p[r] * (dp[r] - de[e]);
+                    ds[r] = (NARROW ? p[r] * up : p[r]) * (dp[r] - de[e]);
                 }
             }
             if (!all) {
@@ -896,6 +936,16 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
                     }
                 }
             }
+            if constexpr (NARROW) {
+                const float largest = wa_largest(ds);
+                if (__any(largest > WA_TOP)) {
+                    const int e = wa_fall(largest);
+                    up = __builtin_ldexpf(up, e);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) ds[r] = __builtin_ldexpf(ds[r], e);
+                    wa_scale<DT>(dk, e);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const typename WaMma<T>::v8 pf = wa_pack8<T>(p + 8 * i), df = wa_pack8<T>(ds + 8 * i);
@@ -909,6 +959,7 @@ __global__ void __launch_bounds__(KB * 128, 2) wa_dkv_kernel(WaArgs w)
         wa_stage_wait<0>();
         __syncthreads();
     }
+    if constexpr (NARROW) wa_scale<DT>(dk, 1 - __builtin_amdgcn_frexp_expf(up));
     // the two halves of the rows: through LDS, dV first
     float* slot = reinterpret_cast<float*>(lds) + kb * (DT * 16 * 64) + lane;
     static_assert(KB * DT * 16 * 64 * 4 <= 4 * BUF, "the partial results fit the stage buffers");
