@@ -952,3 +952,21 @@ def test_window_attention_fp16_gradients_of_any_size(B, Lq, Lkv, Hq, Hk, dh, win
     flushed = lambda n, t: 8 * 2.0 ** -35 * most * scale * math.sqrt(n) * float(t.detach().abs().max())
     small_steps_close(dq, *ref["dq"], flushed(Lkv, k), "dq")
     small_steps_close(dk, *ref["dk"], flushed(Lq * Hq // Hk, q), "dk")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,Lq,Lkv,Hq,Hk,dh", [(1, 1, 4100, 4, 1, 128), (1, 200, 4100, 1, 1, 64), (64, 65, 4100, 8, 2, 40), (16, 200, 4100, 16, 16, 96)])
+def test_window_attention_weights_far_below_the_largest(B, Lq, Lkv, Hq, Hk, dh, dtype):
+    """A first token that takes nearly all the weight and has no value (weights of the others: 2^-24.6 of it, 2^-25 .. 2^-24 with their own
+    differences): the result is what the others hold."""
+    from vipformer_amd.ops_block import window_attention
+    g, dt = gen(25 + dh), TYPES[dtype]
+    q, k, v = torch.zeros(B, Lq, Hq, dh, device="cuda"), torch.zeros(B, Lkv, Hk, dh, device="cuda"), randn(g, B, Lkv, Hk, dh, scale=3e3) + 2e4
+    q[..., 0], q[..., 1] = 1.0, 0.25
+    k[:, 0, :, 0], v[:, 0] = 17.05, 0.0
+    k[:, 1:, :, 1] = torch.rand(B, Lkv - 1, Hk, generator=g, device="cuda") - 0.5
+    q, k, v = q.to(dt), k.to(dt), v.to(dt)
+    out = window_attention(q, k, v, scale=1.0)
+    ref = attention_ref(q, k, v, torch.ones(B, Lq, Lkv, dtype=torch.bool, device="cuda"), 1.0)["out"]
+    # scores of 17 in fp32: 2^-24 * 17 * log2(e), the sum of 4100 weights: 2^-24 a term and 2^-12 at most -- below half a step of fp16 together
+    small_steps_close(out, ref[0], ref[1], 2.0 ** -12 * ref[0].abs(), "out")

@@ -10,8 +10,9 @@
 // Layout of the products (key index in registers, row on the lane), as in attention.hip:
 //   S^T[key, row] = K[key, :] . Q[row, :]        A = K rows (LDS), B = Q (registers)
 //   O^T[d, row] += V^T[d, key] . P^T[key, row]   A = V columns (LDS, transposing reads), B = P straight from the accumulators of S^T
-// Statistics are per-lane scalars in fp32, in units of log2; P is rounded to the tensors' type for the second product (at most half a step of
-// 2^-9 / 2^-12 relative for each weight, the size of the output's own rounding).
+// Statistics are per-lane scalars in fp32, in units of log2; P is rounded to the tensors' type for the second product (at most 2^-9 / 2^-12
+// relative for each weight, the size of the output's own rounding).  fp16 has that precision down to 2^-14 only, and behind a first token that
+// takes nearly all the weight the others can lie far below: forward's weights are lifted by WaMma::LIFT powers of two (their sum with them).
 //
 // LDS tiles hold rows of NC 16-byte chunks without padding; chunk c of row r sits at c ^ swz(r).  Over 64 banks of 4 bytes a fragment read
 // takes the same chunk of 16 consecutive rows (they must differ modulo 16 chunks) and a transposing read takes 4 chunks side by side of 4
@@ -29,11 +30,13 @@ typedef __attribute__((ext_vector_type(16))) float wa_f32x16;
 template <typename T> struct WaMma;
 template <> struct WaMma<vpf_f16> {
     static constexpr bool NARROW = true;    // 5 bits of exponent: what is rounded to it for a product is scaled first
+    static constexpr float GROW = 4.f, LIFT = 11.f;     // weights up to 2^(GROW + LIFT) = 32768; full precision down to 2^-25 of the largest
     typedef __attribute__((ext_vector_type(8))) vpf_f16 v8;
     static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct WaMma<vpf_bf16> {
     static constexpr bool NARROW = false;
+    static constexpr float GROW = 8.f, LIFT = 0.f;
     typedef __attribute__((ext_vector_type(8))) vpf_bf16 v8;
     static __device__ __forceinline__ wa_f32x16 mma(v8 a, v8 b, wa_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
@@ -383,9 +386,9 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mx[j] = fmaxf(mx[j], s[j][kb][r]);
                 mx[j] = wa_half_max(mx[j]) * w.c;
-                grown = grown || mx[j] > m[j] + 8.f;
+                grown = grown || mx[j] > m[j] + WaMma<T>::GROW;
             }
-            // The running maximum only has to keep exp2 in range: it moves when a row has outgrown it by 2^8 (weights up to 256 fit every type)
+            // The running maximum only has to keep exp2 in range: it moves when a row has outgrown it by 2^GROW
             if (__any(grown)) {
 #pragma unroll
                 for (int j = 0; j < RW; ++j) {
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
                 typename WaMma<T>::v8 pf[RW][2];
 #pragma unroll
                 for (int j = 0; j < RW; ++j) {
-                    const float base = m[j] == -INFINITY ? 0.f : m[j];       // a row that has seen nothing yet: every weight is exp2(-inf)
+                    const float base = m[j] == -INFINITY ? 0.f : m[j] - WaMma<T>::LIFT;      // a row that has seen nothing yet: every weight is exp2(-inf)
                     float p[16];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) { p[r] = wa_exp2(fmaf(s[j][kb][r], w.c, -base)); l[j] += p[r]; }
@@ -489,7 +492,7 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_fwd_kernel(WaArgs w)
                 }
             }
         }
-    if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = lr == 0.f ? INFINITY : mr + log2f(lr);
+    if (a.lse && hl == 0) a.lse[(size_t)bh * w.rows + row] = lr == 0.f ? INFINITY : (mr - WaMma<T>::LIFT) + log2f(lr);
     }
 }
 
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(WA_THREADS) wa_join_kernel(WaArgs w)
         op[lane + 64 * i] = v;
         if (a.out_lo) ((T*)a.out_lo)[at * a.head_dim + lane + 64 * i] = (T)(o[i] * inv - (float)v);
     }
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : m + log2f(l);
+    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? INFINITY : (m - WaMma<T>::LIFT) + log2f(l);
 }
 
 // ------------------------------------------------------------------ backward: queries
