@@ -970,3 +970,16 @@ def test_window_attention_weights_far_below_the_largest(B, Lq, Lkv, Hq, Hk, dh, 
     ref = attention_ref(q, k, v, torch.ones(B, Lq, Lkv, dtype=torch.bool, device="cuda"), 1.0)["out"]
     # scores of 17 in fp32: 2^-24 * 17 * log2(e), the sum of 4100 weights: 2^-24 a term and 2^-12 at most -- below half a step of fp16 together
     small_steps_close(out, ref[0], ref[1], 2.0 ** -12 * ref[0].abs(), "out")
+
+
+def test_window_attention_fp16_value_gradients_of_very_many_keys():
+    """Weights of 2^-19.07 = 30.5 steps of 2^-24: dv is their sum over the queries times the gradients."""
+    from vipformer_amd.ops_block import window_attention
+    g, B, Lq, n, dh = gen(26), 1, 40, 550073, 32
+    q, k, v = torch.zeros(B, Lq, 1, dh, device="cuda").half(), randn(g, B, n, 1, dh, dtype=torch.float16), randn(g, B, n, 1, dh, dtype=torch.float16).requires_grad_()
+    dout = randn(g, B, Lq, 1, dh, dtype=torch.float16, scale=1000.0)
+    (dv,) = torch.autograd.grad(window_attention(q, k, v), (v,), dout)
+    ref = (dout.double().sum(1, keepdim=True) / n).expand(B, n, 1, dh)
+    size = ((dout.double() ** 2).sum(1, keepdim=True).sqrt() / n).expand(B, n, 1, dh)
+    # the sum of the weights in fp32, 550073 terms of one size in tiles: 2^-12 of it at most
+    small_steps_close(dv, ref, size, 2.0 ** -12 * ref.abs(), "dv")

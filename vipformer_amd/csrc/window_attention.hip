@@ -50,8 +50,10 @@ struct WaArgs {
     int key_tile, ktiles, sink_tiles, chunks, chunk_rows;      // backward: keys of a tile, tiles, those with sinks, pieces of the rows far behind those and their size
     int cycle;                  // row blocks between two common starting points of the key tiles' walks
 };
-// backward scratch: delta of every row (whole 16-byte pieces), then the pieces
+// backward scratch: delta of every row (whole 16-byte pieces), in fp16 also its lse - WA_LIFT, then the pieces
+#define WA_LIFT 15              // backward's weights are at most 1: fp16 takes them times 2^15 (full precision down to 2^-29)
 __host__ __device__ static inline size_t wa_delta_floats(const WaArgs& w) { return ((size_t)w.a.B * w.a.Hk * w.rows + 3) / 4 * 4; }
+__host__ __device__ static inline size_t wa_row_floats(const WaArgs& w) { return wa_delta_floats(w) * (w.a.dtype == VPF_T_F16 ? 2 : 1); }
 
 __device__ __forceinline__ int wa_query(const WaArgs& w, int r) { return w.g == 1 ? r : (int)__umulhi((uint32_t)r, w.magic); }
 __device__ __forceinline__ float wa_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -711,7 +713,10 @@ __global__ void __launch_bounds__(WA_THREADS, 2) wa_dq_kernel(WaArgs w)
     }
     if (!twice) delta = joined(NARROW ? __builtin_ldexpf(pdp, -up) : pdp);
     if constexpr (NARROW) wa_scale<DT>(dq, -up);
-    if (ks == 0 && hl == 0 && row < w.rows) a.ws[(size_t)bh * w.rows + row] = delta;
+    if (ks == 0 && hl == 0 && row < w.rows) {
+        a.ws[(size_t)bh * w.rows + row] = delta;
+        if (NARROW) a.ws[wa_delta_floats(w) + (size_t)bh * w.rows + row] = lse - WA_LIFT;
+    }
     if (KS > 1) {
         float* slots = reinterpret_cast<float*>(lds);
         constexpr int SLOT = DT * 16 * 64;
@@ -815,7 +820,8 @@ __global__ void __launch_bounds__(KB * 128, DP <= 64 ? 3 : 2) wa_dkv_kernel(WaAr
     wa_f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) { dk[dt] = wa_zero16(); dv[dt] = wa_zero16(); }
-    float up = __builtin_ldexpf(1.f, WA_UP);                                 // the key's power of two (fp16: see wa_dq_kernel)
+    float up = __builtin_ldexpf(1.f, WA_UP - WA_LIFT);                       // fp16: the key's power of two for dS (see wa_dq_kernel), beside P's
+    const float* const lse_of = NARROW ? a.ws + wa_delta_floats(w) : a.lse;
     const int kmin = kt0 + 32 * kb, kmax = kmin + 31;
     const bool whole = !pad && kmax < seen.n;
     // the positions that see the lane's key are key - right .. key + left (a first token: no upper end; a hidden key: none): one unsigned comparison
@@ -865,7 +871,7 @@ __global__ void __launch_bounds__(KB * 128, DP <= 64 ? 3 : 2) wa_dkv_kernel(WaAr
         }
         const int rc = min(lane, last);                                      // (rows behind the range: its last one again, as in the stage)
         const uint32_t stat = stats_at + buf * 3 * ROWS * 4;
-        if (wave == 0) wa_dma4(a.lse + (size_t)bh * w.rows + r0, 4 * rc, stat);
+        if (wave == 0) wa_dma4(lse_of + (size_t)bh * w.rows + r0, 4 * rc, stat);
         if (wave == 1) wa_dma4(a.ws + (size_t)bh * w.rows + r0, 4 * rc, stat + 4 * ROWS);
         if (wave == 2) reinterpret_cast<int*>(stats)[buf * 3 * ROWS + 2 * ROWS + lane] = seen.off + wa_query(w, r0 + rc);
     };
@@ -962,7 +968,7 @@ __global__ void __launch_bounds__(KB * 128, DP <= 64 ? 3 : 2) wa_dkv_kernel(WaAr
         wa_stage_wait<0>();
         __syncthreads();
     }
-    if constexpr (NARROW) wa_scale<DT>(dk, 1 - __builtin_amdgcn_frexp_expf(up));
+    if constexpr (NARROW) { wa_scale<DT>(dk, 1 - WA_LIFT - __builtin_amdgcn_frexp_expf(up)); wa_scale<DT>(dv, -WA_LIFT); }
     // the two halves of the rows: through LDS, dV first
     float* slot = reinterpret_cast<float*>(lds) + kb * (DT * 16 * 64) + lane;
     static_assert(KB * DT * 16 * 64 * 4 <= 4 * BUF, "the partial results fit the stage buffers");
@@ -987,7 +993,7 @@ __global__ void __launch_bounds__(KB * 128, DP <= 64 ? 3 : 2) wa_dkv_kernel(WaAr
     if (qs != 0) return;
     if (w.chunks > 0 && key < a.sinks) {                                     // a first token: one of the pieces of its sum
         const size_t piece = (size_t)bh * (w.chunks + 1) + (far ? chunk + 1 : 0);
-        float* part = a.ws + wa_delta_floats(w) + (piece * a.sinks + key) * 2 * DP;
+        float* part = a.ws + wa_row_floats(w) + (piece * a.sinks + key) * 2 * DP;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1020,7 +1026,7 @@ __global__ void __launch_bounds__(2 * DP) wa_sink_join_kernel(WaArgs w)
     const VpfWindowAttn& a = w.a;
     const int bh = blockIdx.x / a.sinks, key = blockIdx.x % a.sinks, d = threadIdx.x % DP;
     const bool is_v = threadIdx.x >= DP;
-    const float* p = a.ws + wa_delta_floats(w) + ((size_t)bh * (w.chunks + 1) * a.sinks + key) * 2 * DP + threadIdx.x;
+    const float* p = a.ws + wa_row_floats(w) + ((size_t)bh * (w.chunks + 1) * a.sinks + key) * 2 * DP + threadIdx.x;
     float s = 0.f;
 #pragma unroll 4
     for (int c = 0; c <= w.chunks; ++c) s += p[(size_t)c * a.sinks * 2 * DP];
@@ -1115,7 +1121,7 @@ static void wa_plan_bwd(WaArgs& w)
 }
 static long wa_bwd_ws(const WaArgs& w)
 {
-    return (long)wa_delta_floats(w) + (w.chunks ? (long)w.a.B * w.a.Hk * (w.chunks + 1) * w.a.sinks * 2 * wa_dp(w.a.head_dim) : 0);
+    return (long)wa_row_floats(w) + (w.chunks ? (long)w.a.B * w.a.Hk * (w.chunks + 1) * w.a.sinks * 2 * wa_dp(w.a.head_dim) : 0);
 }
 
 // more than 64 KB of LDS has to be asked for, once per kernel and device
