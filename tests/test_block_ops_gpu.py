@@ -983,3 +983,65 @@ def test_window_attention_fp16_value_gradients_of_very_many_keys():
     size = ((dout.double() ** 2).sum(1, keepdim=True).sqrt() / n).expand(B, n, 1, dh)
     # the sum of the weights in fp32, 550073 terms of one size in tiles: 2^-12 of it at most
     small_steps_close(dv, ref, size, 2.0 ** -12 * ref.abs(), "dv")
+
+
+def kernels_of(call):
+    """Names of the kernels that a call launches."""
+    from torch.profiler import ProfilerActivity, profile
+    call()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        call()
+        torch.cuda.synchronize()
+    return [e.key for e in p.key_averages()]
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dh", [72, 96, 120, 128])
+@pytest.mark.parametrize("B,L,Hq,Hk,window,sinks", [(8, 1030, 32, 8, (1023, 0), 3), (3, 4100, 16, 16, (4095, 0), 0), (2, 4200, 27, 9, (2000, 30), 70)])
+def test_window_attention_two_row_blocks_a_wave(B, L, Hq, Hk, window, sinks, dh, dtype):
+    """Long walks beside many rows: forward with two blocks of rows in a wave, rows that are no multiple of 256, first tokens, padding and lengths;
+    some heads of every sample against 64 bits."""
+    from vipformer_amd.ops_block import window_attention
+    g, dt = gen(27 + dh), TYPES[dtype]
+    q, k, v = randn(g, B, L, Hq, dh, dtype=dt), randn(g, B, L, Hk, dh, dtype=dt), randn(g, B, L, Hk, dh, dtype=dt)
+    pad = torch.rand(B, L, generator=g, device="cuda") < 0.3
+    lens = torch.tensor([L - 37 * b - (b > 0) * 300 for b in range(B)], device="cuda", dtype=torch.int32)
+    plain = lambda: window_attention(q, k, v, window, sinks=sinks)
+    names = kernels_of(plain)
+    assert any("wa_fwd_kernel" in n and ("4, 2, 1, 64" in n or "Li4ELi2ELi1ELi64E" in n) for n in names), names
+    pick = (0, Hk // 2, Hk - 1)
+    for p, n in ((None, None), (pad, None), (None, lens), (pad, lens)):
+        hidden = ~seen_mask(B, L, L, window, sinks, p, n).any(1)
+        kk, vv = k.clone(), v.clone()
+        kk[hidden], vv[hidden] = float("nan"), float("inf")
+        out = window_attention(q, kk, vv, window, sinks=sinks, pad_mask=p, kv_lens=n)
+        for b in range(B):
+            mask = seen_mask(B, L, L, window, sinks, p, n)[b:b + 1]
+            for h in pick:
+                part = lambda t, m: t[b:b + 1, :, h * m:(h + 1) * m]
+                ref = attention_ref(part(q, Hq // Hk), part(kk, 1), part(vv, 1), mask, dh ** -0.5)["out"]
+                attention_close(part(out, Hq // Hk), *ref, f"sample {b} head {h}")
+                if b and h:
+                    break
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("dh", [80, 128])
+def test_window_attention_two_row_blocks_a_wave_and_their_gradients(dh, dtype):
+    from vipformer_amd.ops_block import window_attention
+    B, L, Hq, Hk, window, sinks = 8, 1030, 32, 8, (1023, 0), 3
+    g, dt = gen(28 + dh), TYPES[dtype]
+    q, k, v = (randn(g, B, L, h, dh, dtype=dt).requires_grad_() for h in (Hq, Hk, Hk))
+    dout = randn(g, B, L, Hq, dh, dtype=dt)
+    pad = torch.rand(B, L, generator=g, device="cuda") < 0.3
+    lens = torch.tensor([L - 61 * b for b in range(B)], device="cuda", dtype=torch.int32)
+    for p, n in ((None, None), (pad, lens)):
+        out = window_attention(q, k, v, window, sinks=sinks, pad_mask=p, kv_lens=n)
+        grads = torch.autograd.grad(out, (q, k, v), dout)
+        for b, h in ((0, 0), (3, 5), (7, 7)):
+            part = lambda t, m: t.detach()[b:b + 1, :, h * m:(h + 1) * m]
+            wide = Hq // Hk
+            ref = attention_ref(part(q, wide), part(k, 1), part(v, 1), seen_mask(B, L, L, window, sinks, p, n)[b:b + 1], dh ** -0.5, part(dout, wide))
+            for got, name, m in zip((out, *grads), ("out", "dq", "dk", "dv"), (wide, wide, 1, 1)):
+                attention_close(part(got, m), *ref[name], f"{name}, sample {b}, key head {h}")
