@@ -578,7 +578,7 @@ long vpf_gated_norm_ws(const VpfGatedNorm* a);
  * NaN.  (A value that is not finite in a key that some query sees reaches the queries around it, as 0 * NaN does in the product; one in a query
  * that sees some key, or in its gradient, reaches the dk and dv of the keys around.)
  * q, out, dout, dq [B, Lq, Hq, head_dim]; k, v, dk, dv [B, Lkv, Hk, head_dim]: fp16 or bf16, 16-byte aligned, strides multiples of 8;
- * Hk divides Hq, query heads h Hq / Hk .. share key head h.  head_dim a multiple of 8 up to 128.  pad uint8 [B, Lkv], lens int32 [B] (device).
+ * Hk divides Hq, query heads h Hq / Hk .. share key head h.  head_dim a multiple of 8 up to 128.  pad uint8 [B, Lkv], lens int32 or int64 [B] (device).
  * lse fp32 [B, Hk, Lq * Hq / Hk]: log2 of the sum of the exponentials (+inf: nothing visible); forward writes it (null: no gradient follows).
  * out_lo: out's type, [B, Hk, Lq * Hq / Hk, head_dim] contiguous: what rounding took from out (null with lse).
  * backward needs q, k, v, out, out_lo, lse of the forward call and its masks; dq, dk, dv are overwritten whole.  Sums are taken in a fixed order. */
@@ -587,8 +587,8 @@ long vpf_gated_norm_ws(const VpfGatedNorm* a);
 #define VPF_WINDOW_MAX_HEADS (1L << 29)         /* backward: Hq / Hk times the head stride of q and of dout stays below it (elements) */
 typedef struct VpfWindowAttn {
     int B, Lq, Lkv, Hq, Hk, head_dim, left, right, sinks, dtype;
-    float scale; int pad_;
-    const void* q; const void* k; const void* v; const void* pad; const int* lens;
+    float scale; int lens64;            /* lens64 != 0: lens holds 64-bit numbers */
+    const void* q; const void* k; const void* v; const void* pad; const void* lens;
     void* out; float* lse; void* out_lo;
     const void* dout; void* dq; void* dk; void* dv;
     float* ws; long ws_floats;          /* vpf_window_attn_ws floats of scratch (forward: may be null where that is 0) */

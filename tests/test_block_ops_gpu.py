@@ -1045,3 +1045,16 @@ def test_window_attention_two_row_blocks_a_wave_and_their_gradients(dh, dtype):
             ref = attention_ref(part(q, wide), part(k, 1), part(v, 1), seen_mask(B, L, L, window, sinks, p, n)[b:b + 1], dh ** -0.5, part(dout, wide))
             for got, name, m in zip((out, *grads), ("out", "dq", "dk", "dv"), (wide, wide, 1, 1)):
                 attention_close(part(got, m), *ref[name], f"{name}, sample {b}, key head {h}")
+
+
+@pytest.mark.parametrize("far", [2 ** 31, 2 ** 32 + 5, 2 ** 40])
+def test_window_attention_lengths_are_clamped_in_64_bits(far):
+    from vipformer_amd.ops_block import window_attention
+    g = gen(29)
+    q, k, v = randn(g, 4, 3, 4, 64, dtype=torch.float16), *(randn(g, 4, 200, 2, 64, dtype=torch.float16) for _ in range(2))
+    lens = torch.tensor([far, -far, 17, 200], device="cuda")
+    clamped = lens.clamp(0, 200)
+    a, b, c = (window_attention(q, k, v, (50, 0), sinks=1, kv_lens=n) for n in (lens, clamped, clamped.int()))
+    strided = window_attention(q, k, v, (50, 0), sinks=1, kv_lens=torch.stack([lens, lens + 1], 1)[:, 0])
+    assert torch.equal(a, b) and torch.equal(b, c) and torch.equal(c, strided)
+    assert float(a[1].abs().sum()) == 0.0 and float(a[0].abs().sum()) > 0.0

@@ -259,7 +259,7 @@ class GatedNorm(ctypes.Structure):
 class WindowAttn(ctypes.Structure):
     """struct VpfWindowAttn (include/vipformer_hip.h)."""
     _fields_ = [("B", I), ("Lq", I), ("Lkv", I), ("Hq", I), ("Hk", I), ("head_dim", I), ("left", I), ("right", I), ("sinks", I), ("dtype", I),
-                ("scale", F), ("pad_", I),
+                ("scale", F), ("lens64", I),
                 ("q", VP), ("k", VP), ("v", VP), ("pad", VP), ("lens", VP), ("out", VP), ("lse", VP), ("out_lo", VP),
                 ("dout", VP), ("dq", VP), ("dk", VP), ("dv", VP), ("ws", VP), ("ws_floats", L_)] + \
                [(f"{t}_{s}", L_) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for s in ("sb", "sl", "sh")]

@@ -134,7 +134,7 @@ __device__ __forceinline__ WaSeen wa_seen(const WaArgs& w, int b)
 {
     WaSeen s;
     s.n = w.a.Lkv;
-    if (w.a.lens) s.n = max(0, min(w.a.lens[b], w.a.Lkv));
+    if (w.a.lens) s.n = (int)max(0L, min(w.a.lens64 ? (long)((const long long*)w.a.lens)[b] : (long)((const int*)w.a.lens)[b], (long)w.a.Lkv));
     s.off = s.n - w.a.Lq;
     return s;
 }

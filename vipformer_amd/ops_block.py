@@ -332,8 +332,8 @@ def _attn_launch(name, cfg, q, k, v, out, pad, lens, lse, lo, grads, strides, ba
     B, Lq, Hq, dh = q.shape
     _, Lkv, Hk, _ = k.shape
     dev = q.device
-    head = (B, Lq, Lkv, Hq, Hk, dh, left, right, sinks, _TYPE[q.dtype], scale, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(pad), _ptr(lens),
-            out.data_ptr(), _ptr(lse), _ptr(lo), *grads)
+    head = (B, Lq, Lkv, Hq, Hk, dh, left, right, sinks, _TYPE[q.dtype], scale, int(lens is not None and lens.dtype is torch.int64),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(pad), _ptr(lens), out.data_ptr(), _ptr(lse), _ptr(lo), *grads)
     packed = _pack_attn(*head, 0, 0, *strides)
     n = L.scratch_floats("vpf_window_attn_ws", packed, backward)
     if n:
@@ -387,7 +387,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     window = (left, right): query at position p sees keys p - left .. p + right (None: open on that side; (n, 0) is causal), and of the first
     ``sinks`` keys those up to p + right, however far behind they are.
     With n keys in use the last query stands at the last of them: query i at position n - Lq + i.  n is Lkv, or kv_lens[b] (int32 / int64 [B],
-    on the device, read by the kernels: a captured graph follows it): a preallocated cache that is filled to different lengths.
+    on the device, read by the kernels: a captured graph follows it; clamped to 0 .. Lkv): a preallocated cache that is filled to different lengths.
     pad_mask: bool [B, Lkv], True = this key is padding (as the ``pad_mask`` of the framework's encoders); it moves no positions.
     Keys that no query sees may hold anything, also NaN; a value that is not finite in a key that some query sees reaches the queries around it, as
     0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros; it and its gradient may hold anything and reach
@@ -424,8 +424,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     top = (1 << 30) - 1
     cfg = (-1 if left is None else min(left, top), -1 if right is None else min(right, top), min(sinks, top), scale)
     pad = None if pad_mask is None else pad_mask.contiguous().view(torch.uint8)
-    lens = None if kv_lens is None else kv_lens.to(torch.int32).contiguous()
+    lens = None if kv_lens is None else kv_lens.contiguous()
     if not _wants_grad(q, k, v):
         (q, sq), (k, sk), (v, sv) = _attn_ready(q), _attn_ready(k), _attn_ready(v)
         return _attn_forward(cfg, q, k, v, pad, lens, sq + sk + sv, False)[0]
+    if lens is not None and lens.dtype is torch.int64:           # (64-bit counters go on counting behind the call: backward has its own)
+        lens = lens.clone()
     return WindowAttentionFn.apply(cfg, q, k, v, pad, lens)
