@@ -7,23 +7,11 @@
 typedef _Float16 vpf_f16;
 typedef __bf16 vpf_bf16;
 
-template <typename T> struct VpfElem;
-template <> struct VpfElem<float> { static constexpr int code = VPF_T_F32; };
-template <> struct VpfElem<vpf_f16> { static constexpr int code = VPF_T_F16; };
-template <> struct VpfElem<vpf_bf16> { static constexpr int code = VPF_T_BF16; };
-
-static inline int vpf_elem_size(int code) { return code == VPF_T_F32 ? 4 : 2; }
 static inline bool vpf_elem_ok(int code) { return code == VPF_T_F32 || code == VPF_T_F16 || code == VPF_T_BF16; }
 static inline bool vpf_aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // N consecutive elements as one access of N * sizeof(T) bytes (16-byte pieces where it is larger); the caller guarantees the alignment
 template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) VpfPack { T e[N]; };
-template <typename T, int N> __device__ __forceinline__ void vpf_load(float* v, const T* p)
-{
-    const VpfPack<T, N> r = *reinterpret_cast<const VpfPack<T, N>*>(p);
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (float)r.e[i];
-}
 template <typename T, int N> __device__ __forceinline__ void vpf_store(T* p, const float* v)
 {
     VpfPack<T, N> r;
