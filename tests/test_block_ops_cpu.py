@@ -311,3 +311,20 @@ def test_a_gate_parameter_that_is_not_contiguous_is_a_parameter(monkeypatch):
                 holder.inv = torch.tensor(0.25)
             (dgate,) = torch.autograd.grad(h, (gate,), torch.ones(4, 32))
             assert dgate.shape == gate.shape and torch.equal(dgate, torch.full_like(dgate, want if holder.on else 1.0)), gate.stride()
+
+
+def test_saved_tensors_that_come_back_as_something_else_are_refused(monkeypatch):
+    """Hooks that bring back another type, shape or device: the kernels would read something else, or behind its end."""
+    rec = _Records(monkeypatch)
+    q, x, w, plan = torch.zeros(1, 4, 2, 32, dtype=torch.float16), torch.ones(2, 3, 32), torch.ones(32), O.RotaryAxes((8, 8), 32)
+    q.requires_grad_(), x.requires_grad_()
+    calls = {"rotary_axes": (q, lambda: O.rotary_axes(q, None, torch.zeros(4, 2), plan)),
+             "window_attention": (q, lambda: O.window_attention(q, q.detach(), q.detach(), kv_lens=torch.tensor([4]))),
+             "gated_norm_residual": (x, lambda: O.gated_norm_residual(x, x.detach(), post=(w, None))[0])}
+    for what, (leaf, call) in calls.items():
+        for unpack in (lambda t: t.double(), lambda t: t[..., :-1], lambda t: t.flatten(), lambda t: t.to("meta")):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                out = call()
+                n = len(rec.calls)
+                refuses(f"{what}: a saved tensor came back", torch.autograd.grad, out, (leaf,), torch.zeros_like(out))
+                assert len(rec.calls) == n, what

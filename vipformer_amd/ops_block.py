@@ -60,6 +60,26 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+_top_hooks = torch._C._autograd._top_saved_tensors_default_hooks
+
+
+def _keep(ctx, *ts) -> None:
+    ctx.save_for_backward(*ts)
+    ctx.at = None if _top_hooks(False) is not None else [_ptr(t) for t in ts]      # None: hooks take them from here
+
+
+def _kept(ctx, what: str, want):
+    """(the saved tensors, are they where they were?).  The kernels take addresses: tensors that lie elsewhere (a saved-tensor hook brought them back,
+    or their storage was filled anew) are looked at before they go there.  want(): (shape, type, device) of each, None to leave one out."""
+    ts = ctx.saved_tensors
+    if [_ptr(t) for t in ts] == ctx.at:
+        return ts, True
+    for t, w in zip(ts, want()):
+        if t is not None and (t.shape, t.dtype, t.device) != w:
+            raise L.VpfError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, it was {w[1]} {tuple(w[0])} on {w[2]}")
+    return ts, False
+
+
 def _dense(t):
     """A saved tensor that was contiguous.  (What a saved-tensor hook brings back has its values and shape; strides and address are its own.)"""
     return None if t is None else t.contiguous()
@@ -143,15 +163,15 @@ def _rotary_run(plan, pos, q, k, inverse):
 class RotaryAxesFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, pos, q, k):
-        ctx.plan = plan
-        ctx.save_for_backward(pos)
+        ctx.plan, ctx.pos = plan, (pos.shape, pos.dtype, pos.device)
+        _keep(ctx, pos)
         oq, ok = _rotary_run(plan, pos, q, k, 0)
         return oq if k is None else (oq, ok)
 
     @staticmethod
     def backward(ctx, gq, gk=None):
         _once("rotary_axes")
-        (pos,) = ctx.saved_tensors
+        ((pos,), _) = _kept(ctx, "rotary_axes", lambda: (ctx.pos,))
         return (None, None) + _rotary_run(ctx.plan, pos.contiguous(), gq, gk, 1)
 
 
@@ -208,16 +228,21 @@ class GatedNormFn(torch.autograd.Function):
     def forward(ctx, cfg, gate_is_param, x, y, gate, *params):
         h, n, stats = _norm_forward(cfg, x, y, gate, params, True)
         ctx.cfg, ctx.iscale, ctx.gate_is_param = cfg, ops._current_iscale(), gate_is_param
-        ctx.save_for_backward(x, y, gate, stats, *params)
+        ctx.y_type, ctx.gate_shape = y.dtype, None if gate is None else gate.shape
+        _keep(ctx, x, y, gate, stats, *params)
         return (h, n) if n is not None else h
 
     @staticmethod
     def backward(ctx, dh, dn=None):
         _once("gated_norm_residual")
-        x, y, gate, stats, *params = map(_dense, ctx.saved_tensors)
-        need = ctx.needs_input_grad[1:]
         kind, mode, gate_rows, has_post, has_pre, alpha, beta, eps_post, eps_pre = ctx.cfg
-        dev, D = x.device, x.shape[-1]
+        shape, dev = dh.shape, dh.device
+        D = shape[-1]
+        ts, same = _kept(ctx, "gated_norm_residual", lambda: (
+            (shape, dh.dtype, dev), (shape, ctx.y_type, dev), (ctx.gate_shape, ctx.y_type if mode == 2 else F32, dev),
+            ((4 * (dh.numel() // D),), F32, dev)) + 4 * (((D,), F32, dev),))
+        x, y, gate, stats, *params = ts if same else map(_dense, ts)
+        need = ctx.needs_input_grad[1:]
         if x.numel() == 0:
             return (None, None, *(torch.zeros_like(t) if t is not None and n else None for t, n in zip((x, y, gate, *params), need[1:])))
         dh = dh.contiguous()
@@ -359,23 +384,34 @@ class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, q, k, v, pad, lens):
         (q, sq), (k, sk), (v, sv) = _attn_ready(q, q.shape[2] // k.shape[2]), _attn_ready(k), _attn_ready(v)
-        ctx.cfg = cfg
-        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, sq + sk + sv, True)
-        ctx.save_for_backward(q, k, v, out, lse, lo, pad, lens)
+        ctx.cfg, ctx.strides, ctx.keys = cfg, sq + sk + sv, k.shape
+        out, lse, lo = _attn_forward(cfg, q, k, v, pad, lens, ctx.strides, True)
+        _keep(ctx, q, k, v, out, lse, lo, pad, lens)
+        ctx.qkv, ctx.lens64 = (q.stride(), k.stride(), v.stride()), lens is not None and lens.dtype is torch.int64
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _once("window_attention")
-        q, k, v, *rest = ctx.saved_tensors
-        out, lse, lo, pad, lens = map(_dense, rest)
-        lo = lo.clone() if lo.data_ptr() & 15 else lo
-        g = q.shape[2] // k.shape[2]
-        (q, sq), (k, sk), (v, sv), (out, so), (dout, sd) = _attn_ready(q, g), _attn_ready(k), _attn_ready(v), _attn_ready(out), _attn_ready(dout, g)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        B, Lq, Hq, dh = rows = dout.shape
+        keys, dt, dev = ctx.keys, dout.dtype, dout.device
+        ts, same = _kept(ctx, "window_attention", lambda: (
+            (rows, dt, dev), (keys, dt, dev), (keys, dt, dev), (rows, dt, dev), ((B * Lq * Hq,), F32, dev), (rows, dt, dev),
+            ((B, keys[1]), torch.uint8, dev), ((B,), torch.int64 if ctx.lens64 else torch.int32, dev)))
+        q, k, v, out, lse, lo, pad, lens = ts
+        g = Hq // keys[2]
+        if same and ctx.qkv == (q.stride(), k.stride(), v.stride()):
+            strides, so = ctx.strides, _strides(out)
+        else:
+            lse, lo, pad, lens = map(_dense, (lse, lo, pad, lens))
+            lo = lo.clone() if lo.data_ptr() & 15 else lo
+            (q, sq), (k, sk), (v, sv), (out, so) = _attn_ready(q, g), _attn_ready(k), _attn_ready(v), _attn_ready(out)
+            strides = sq + sk + sv
+        dout, sd = _attn_ready(dout, g)
+        dq, dk, dv = (torch.empty(shape, dtype=dt, device=dev) for shape in (rows, keys, keys))
         sdq, sdk = _strides(dq), _strides(dk)
         _attn_launch("vpf_window_attn_bwd", ctx.cfg, q, k, v, out, pad, lens, lse, lo, (dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()),
-                     sq + sk + sv + so + sd + sdq + sdk + sdk, 1)
+                     strides + so + sd + sdq + sdk + sdk, 1)
         return None, dq, dk, dv, None, None
 
 
