@@ -583,7 +583,7 @@ long vpf_gated_norm_ws(const VpfGatedNorm* a);
  * out_lo: out's type, [B, Hk, Lq * Hq / Hk, head_dim] contiguous: what rounding took from out (null with lse).
  * backward needs q, k, v, out, out_lo, lse of the forward call and its masks; dq, dk, dv are overwritten whole.  Sums are taken in a fixed order. */
 #define VPF_WINDOW_MAX_DIM 128
-#define VPF_WINDOW_MAX_STRIDE (1L << 23)        /* token and head strides stay below it (elements) */
+#define VPF_WINDOW_MAX_STRIDE (1L << 23)        /* token strides stay below it (elements) */
 #define VPF_WINDOW_MAX_HEADS (1L << 29)         /* backward: Hq / Hk times the head stride of q and of dout stays below it (elements) */
 typedef struct VpfWindowAttn {
     int B, Lq, Lkv, Hq, Hk, head_dim, left, right, sinks, dtype;

@@ -328,3 +328,17 @@ def test_saved_tensors_that_come_back_as_something_else_are_refused(monkeypatch)
                 n = len(rec.calls)
                 refuses(f"{what}: a saved tensor came back", torch.autograd.grad, out, (leaf,), torch.zeros_like(out))
                 assert len(rec.calls) == n, what
+
+
+def test_window_attention_takes_long_caches_with_the_heads_first_as_they_are():
+    """[B, heads, tokens, head_dim] caches of more than 65536 tokens: where a head begins is no offset inside a stage."""
+    cache = torch.empty(2, 4, 70000, 128, dtype=torch.bfloat16, device="meta").transpose(1, 2)
+    t, strides = O._attn_ready(cache)
+    assert t is cache and strides == (4 * 70000 * 128, 128, 70000 * 128)
+    rows = torch.empty_strided((1, 3, 2, 8), (0, 1 << 23, 8, 1), dtype=torch.float16, device="meta")
+    assert O._attn_ready(rows)[1] == (0, 16, 8)                                 # tokens are
+    fwd = L.lib().vpf_window_attn_fwd
+    fwd.argtypes = L.SIGS["vpf_window_attn_fwd"]
+    args = dict(B=1, Lq=1, Lkv=70000, Hq=4, Hk=4, head_dim=128, left=-1, right=0, dtype=2, scale=0.1, q=16, k=16, v=16, out=16, k_sl=128, v_sl=128)
+    assert fwd(ctypes.byref(L.WindowAttn(**args, k_sh=1 << 40, v_sh=1 << 40)), None) == -5      # (no scratch: nothing is launched)
+    assert fwd(ctypes.byref(L.WindowAttn(**{**args, "k_sl": 1 << 23})), None) == -2

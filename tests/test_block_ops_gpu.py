@@ -1058,3 +1058,27 @@ def test_window_attention_lengths_are_clamped_in_64_bits(far):
     strided = window_attention(q, k, v, (50, 0), sinks=1, kv_lens=torch.stack([lens, lens + 1], 1)[:, 0])
     assert torch.equal(a, b) and torch.equal(b, c) and torch.equal(c, strided)
     assert float(a[1].abs().sum()) == 0.0 and float(a[0].abs().sum()) > 0.0
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_window_attention_heads_first_caches_beyond_32_bits(train):
+    """Heads that lie 70000 x 128 elements apart, the last of 250 beyond 2^31 elements: single tokens, and (3 heads) a prompt with its gradients, as
+    over a copy with the tokens first."""
+    from vipformer_amd.ops_block import window_attention
+    g = gen(30)
+    B, heads = (2, 3) if train else (1, 250)
+    cache = torch.empty(B, heads, 70000, 128, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    k, v = (t.transpose(1, 2) for t in ((cache, cache.flip(1)) if train else (cache, cache)))
+    lens = torch.tensor([70000, 65537][:B], device="cuda")
+    Lq = 40 if train else 1
+    q = randn(g, B, Lq, heads, 128, dtype=torch.bfloat16)
+    runs = []
+    for a, b in ((k, v), (k.contiguous(), v.contiguous())):
+        leaves = [t.detach().requires_grad_(train) for t in (q, a, b)]
+        out = window_attention(*leaves, (69000, 0), sinks=2, kv_lens=lens)
+        grads = torch.autograd.grad(out, leaves, q) if train else ()
+        runs.append([out.detach(), *grads])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    m = seen_mask(B, Lq, 70000, (69000, 0), 2, None, lens)
+    last = slice(heads - 1, heads)
+    attention_close(runs[0][0][:, :, last], *attention_ref(q[:, :, last], k[:, :, last], v[:, :, last], m, 128 ** -0.5)["out"], "last head")

@@ -1061,10 +1061,11 @@ static int wa_prepare(const VpfWindowAttn* args, WaArgs& w)
     return VPF_OK;
 }
 // 16-byte rows; the offsets inside a stage are 32-bit byte offsets: 127 keys' strides below 2^31, and in the dK / dV kernel a row's query
-// (at most 63 of them, 32 where heads share a key head) and head: 2 (2^28 + 2^29) bytes with the heads of a key head below 2^29 elements
+// (at most 63 of them, 32 where heads share a key head) and head: 2 (2^28 + 2^29) bytes with the heads of a key head below 2^29 elements.  Where a
+// head or a sample begins is found in 64 bits.
 static bool wa_aligned(const void* p, long sb, long sl, long sh)
 {
-    return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < VPF_WINDOW_MAX_STRIDE && sh >= 0 && sh < VPF_WINDOW_MAX_STRIDE;
+    return vpf_aligned(p, 16) && sb % 8 == 0 && sl % 8 == 0 && sh % 8 == 0 && sl >= 0 && sl < VPF_WINDOW_MAX_STRIDE && sh >= 0;
 }
 
 // Row blocks of 32 per workgroup (4, 2 or 1; the waves that are left split a stage's keys): as many as leave a workgroup for each of the 256 CUs.

@@ -341,10 +341,10 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
 # --------------------------------------------------------------------------- attention inside a sliding window
 def _attn_ready(t: torch.Tensor, shared: int = 0):
     """(tensor, its batch, token and head stride).  16-byte rows: a contiguous last dimension, an aligned base, strides that are multiples of 8
-    elements, those of tokens and heads below 2^23 and, for a backward pass over ``shared`` heads of a key head, those heads together below
-    2^29; everything else is copied."""
+    elements, those of tokens below 2^23 and, for a backward pass over ``shared`` heads of a key head, those heads together below 2^29;
+    everything else is copied."""
     st = sb, sl, sh = _strides(t)
-    if (sb | sl | sh) & 7 or sl >= 1 << 23 or sh >= 1 << 23 or shared * sh >= 1 << 29 or t.stride(3) != 1 or t.data_ptr() & 15:
+    if (sb | sl | sh) & 7 or sl >= 1 << 23 or shared * sh >= 1 << 29 or t.stride(3) != 1 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         st = _strides(t)
     return t, st
