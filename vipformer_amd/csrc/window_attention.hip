@@ -1103,7 +1103,7 @@ static long wa_fwd_ws(const WaArgs& w) { return w.splits > 1 ? (long)w.splits * 
 
 // Key tiles of 128 at head dimension 128 where that leaves a workgroup for each CU (the stages of Q and dO then serve twice the keys), else of 64.
 // The rows behind a sink tile's own window are cut into pieces about as long as the row range of an ordinary tile, where that leaves more than
-// one of them: at most 32 pieces (they are fp32 scratch), none where the first tokens fill more than 8 tiles (enough workgroups by themselves).
+// one of them: about 32 pieces, at most 33 (they are fp32 scratch), none where the first tokens fill more than 8 tiles (enough workgroups by themselves).
 static void wa_plan_bwd(WaArgs& w)
 {
     const VpfWindowAttn& a = w.a;

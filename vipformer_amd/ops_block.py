@@ -7,9 +7,10 @@ LayerNorm and residual pieces of ops.py:
 
 Heads are a dimension of their own ([B, L, heads, head_dim], any strides whose last dimension is contiguous: slices of one projection's
 output go in as they are).  fp16 and bf16 are chosen by the tensors, per call; the library's build-time operand type does not matter here.
-Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once (backward mode), and may be captured into a HIP graph once
-it has run there (a RotaryAxes makes its tables at its first use on a device).  As everywhere in torch, a backward pass is captured only while no
-eager graph of the same leaves is alive (train.GraphedStep).
+Every operator is asynchronous on torch's current stream of the tensors' device, differentiable once (in backward mode; a forward-mode tangent
+raises), and may be captured into a HIP graph once it has run there (a RotaryAxes makes its tables at its first use on a device).  As everywhere
+in torch, a backward pass is captured only while no eager graph of the same leaves is alive (train.GraphedStep).  Saved tensors may travel
+through hooks (offload, recomputation); what comes back with another type, shape or device is refused.
 """
 from __future__ import annotations
 
@@ -298,7 +299,7 @@ def gated_norm_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.T
     x: the residual stream, y: the block's output, both [..., D] with D <= 8192; x is fp32, or x and y are of one type (fp16, bf16).  h has
     x's type, n has y's; n is taken from h before h is rounded.
     post / pre: (weight, bias) with fp32 [D] tensors or None entries, a LayerNorm / RMSNorm module, or None for no norm there.
-    kind: "layer" or "rms" (biased variance, ``eps`` inside the root) for both norms; a module brings its own eps.
+    kind: "layer" or "rms" (biased variance, ``eps`` inside the root) for both norms; a module brings its own eps (None: that of fp32).
     gate: None, fp32 [D], one fp32 row of D per sample (x [B, ..., D]: gate [B, 1, .., D]), or one of x's shape and y's type."""
     shape = x.shape
     if len(shape) < 1 or shape != y.shape or not 1 <= shape[-1] <= 8192:
@@ -423,13 +424,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     window = (left, right): query at position p sees keys p - left .. p + right (None: open on that side; (n, 0) is causal), and of the first
     ``sinks`` keys those up to p + right, however far behind they are.
     With n keys in use the last query stands at the last of them: query i at position n - Lq + i.  n is Lkv, or kv_lens[b] (int32 / int64 [B],
-    on the device, read by the kernels: a captured graph follows it; clamped to 0 .. Lkv): a preallocated cache that is filled to different lengths.
+    on the device, read by the kernels: a captured graph follows it; clamped to 0 .. Lkv): a preallocated cache that is filled to different
+    lengths.
     pad_mask: bool [B, Lkv], True = this key is padding (as the ``pad_mask`` of the framework's encoders); it moves no positions.
     Keys that no query sees may hold anything, also NaN; a value that is not finite in a key that some query sees reaches the queries around it, as
     0 * NaN does in the product of weights and values.  A query that sees nothing gets zeros; it and its gradient may hold anything and reach
     nothing.  (In the gradients of keys and values, what is not finite in a query that sees some key, or in its gradient, reaches the keys around.)
     Key heads are shared by heads / key heads consecutive query heads.  head_dim: a multiple of 8 up to 128; scale defaults to head_dim ** -0.5.
-    Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v.  There is no dropout on the weights here."""
+    Returns a new contiguous [B, Lq, heads, head_dim]; gradients for q, k and v (until then a call keeps the result twice: what its rounding took
+    away, and 4 bytes a query and head).  There is no dropout on the weights here."""
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or ks != v.shape or ks[0] != qs[0] or ks[3] != qs[3] or ks[2] < 1 or qs[2] < 1 or qs[2] % ks[2]:
         raise L.VpfError(f"window_attention: q [B, Lq, heads, head_dim], k and v [B, Lkv, key heads, head_dim], key heads dividing heads (got "
