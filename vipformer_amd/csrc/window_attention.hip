@@ -10,7 +10,7 @@
 // Layout of the products (key index in registers, row on the lane), as in attention.hip:
 //   S^T[key, row] = K[key, :] . Q[row, :]        A = K rows (LDS), B = Q (registers)
 //   O^T[d, row] += V^T[d, key] . P^T[key, row]   A = V columns (LDS, transposing reads), B = P straight from the accumulators of S^T
-// Statistics are per-lane scalars in fp32, in units of log2; P is rounded to the tensors' type for the second product (at most 2^-9 / 2^-12
+// Statistics are per-lane scalars in fp32, in units of log2; P is rounded to the tensors' type for the second product (at most 2^-8 / 2^-11
 // relative for each weight, the size of the output's own rounding).  fp16 has that precision down to 2^-14 only, and behind a first token that
 // takes nearly all the weight the others can lie far below: forward's weights are lifted by WaMma::LIFT powers of two (their sum with them).
 //
